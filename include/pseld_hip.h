@@ -486,6 +486,23 @@ int pseld_gru_multi_bwd(int dtype, int n, const void* const* dseq, const void* c
 int pseld_gru_gate_bwd(int dtype, const void* dh, long dh_stride, const void* carry, const void* gates, const void* hprev,
                        long hp_stride, void* dgi, long dgi_stride, void* dgh, void* dhprev, int B, int H, void* stream);
 
+/* ---- gated linear recurrence over packed recordings (decoders on whole recordings and running streams) ---------------------
+ * z = sigmoid(g), h_t = z_t h_{t-1} + (1 - z_t) n_t per channel: nn.GRU's update rule (model_utilities.py:249-252) without the recurrent
+ * product, so the frames of a recording compose in parallel. Recordings lie back to back: recording s is rows start[s] .. start[s] + len[s]
+ * (device int arrays, seqs of each; rows = the sum of the lengths, max_len the longest, both host values). g, n, h rows at strides ldg, ldn, ldh
+ * (multiples of 4 elements, addresses on 4-element boundaries), C a multiple of 8. reverse: every recording runs from its last row to its first.
+ * h0 [seqs, C] (NULL: zeros) -> h and h_last [seqs, C] (= h0 for an empty recording). states: f32 [pseld_linrec_states(rows, seqs), C], what the
+ * backward needs besides g and n (NULL: not wanted). bwd: dh, dh_last (NULL: zeros) -> dg, dn, dh0 (NULL: not wanted). All state
+ * arrays are f32. workspace: pseld_linrec_workspace bytes (0: none needed). Deterministic. */
+long pseld_linrec_workspace(long rows, int seqs, int max_len, int C);
+long pseld_linrec_states(long rows, int seqs);
+int pseld_linrec_fwd(int dtype, const void* g, long ldg, const void* n, long ldn, const float* h0, void* h, long ldh, float* h_last,
+                     float* states, const int* start, const int* len, int seqs, long rows, int max_len, int C, int reverse,
+                     float* workspace, long workspace_bytes, void* stream);
+int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void* g, long ldg, const void* n, long ldn, const float* states,
+                     const float* dh_last, void* dg, long lddg, void* dn, long lddn, float* dh0, const int* start, const int* len,
+                     int seqs, long rows, int max_len, int C, int reverse, float* workspace, long workspace_bytes, void* stream);
+
 /* ---- output head ---------------------------------------------------------------------------------------------------
  * htsat.py:526-534 (token -> [C,2,32] map) + im2col of accdoa.py:230 tscam_conv((2,3), pad (0,1)):
  * tok [B,64,C] -> A [B*32, C*6] (k = c*6 + cf*3 + dt, matching the conv weight's [D, C, 2, 3] flattening).

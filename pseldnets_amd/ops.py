@@ -1565,3 +1565,139 @@ def sdpa_small_bwd(q, k, v, attn, dout, B, T, heads, mask=None, mask_scale=1.0):
                                       float(mask_scale), _lib.ptr(attn), _lib.ptr(dout), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(scratch),
                                       B, T, D, heads, _lib.ptr(ws), ws.numel() * 4, _lib.stream_ptr()), "pseld_sdpa_small_bwd")
     return dq, dk, dv
+
+
+# ---------------------------------------------------------------------------------------------------------
+# packed recordings: what the sequence operators (csrc/linrec.hip, csrc/packed_attn.hip) run over
+class PackedPlan:
+    """Recordings of different lengths laid back to back: recording s holds rows q_start[s] .. q_start[s] + q_lens[s] of every [rows, ...] tensor.
+    Keys and values lie the same way with their own lengths, or in slabs of a fixed capacity (a cache) of which the first k_len[s] rows
+    count. k_len is a device tensor: a stream that appends a frame to its slab adds to it in place (also inside a captured graph); the kernels
+    hold it to 0 .. capacity. Everything else is fixed when the plan is made."""
+
+    def __init__(self, q_lens, k_lens, k_cap, device):
+        q_lens = [int(n) for n in q_lens]
+        own_keys = k_lens is not None or k_cap is not None
+        k_lens = q_lens if k_lens is None else [int(n) for n in k_lens]
+        caps = k_lens if k_cap is None else [int(n) for n in (k_cap if hasattr(k_cap, '__iter__') else [k_cap] * len(q_lens))]
+        if not q_lens:
+            raise _lib.PseldError("packed_plan: no recordings")
+        if len(k_lens) != len(q_lens) or len(caps) != len(q_lens):
+            raise _lib.PseldError("packed_plan: q_lens, k_lens and k_cap must name the same recordings")
+        if min(q_lens) < 0 or min(k_lens) < 0 or any(n > c for n, c in zip(k_lens, caps)):
+            raise _lib.PseldError("packed_plan: lengths must be >= 0 and at most the capacity")
+        if sum(q_lens) >= 1 << 31 or sum(caps) >= 1 << 31 or len(q_lens) > 1 << 20:
+            raise _lib.PseldError("packed_plan: at most 2^31 - 1 rows and 2^20 recordings")
+        self.device = torch.device(device)
+        if self.device.type != 'cuda':
+            raise _lib.PseldError("packed_plan: the plan must live on the MI355X (no CPU fallback)")
+        if self.device.index is None:
+            self.device = torch.device('cuda', torch.cuda.current_device())
+        self.q_lens, self.k_caps, self.self_keys = q_lens, caps, not own_keys
+        self.seqs, self.rows, self.max_q = len(q_lens), sum(q_lens), max(q_lens)
+        self.k_rows, self.max_k = sum(caps), max(caps)
+        T = _PACKED_TILE
+        # work lists, heaviest tile first: (recording, first row) of every 128-row tile of queries and of keys, ordered for
+        # full attention (by the other side's length) and for causal attention (by how much of the other side the mask leaves)
+        pairs = list(enumerate(zip(q_lens, caps)))
+        qf = [(-k, s, q0) for s, (q, k) in pairs for q0 in range(0, q, T)]
+        qc = [(-(k - q + q0), s, q0) for s, (q, k) in pairs for q0 in range(0, q, T)]
+        kf = [(-q, s, k0) for s, (q, k) in pairs for k0 in range(0, k, T)]
+        kc = [(-min(q, k - k0), s, k0) for s, (q, k) in pairs for k0 in range(0, k, T)]
+        self.q_tiles, self.k_tiles = len(qf), len(kf)
+        host, at = [], {}
+
+        def put(name, values):
+            host.extend([0] * (-len(host) % 4))
+            at[name] = len(host)
+            host.extend(values)
+
+        def starts(lens):
+            out, n = [], 0
+            for x in lens:
+                out.append(n)
+                n += x
+            return out
+        put('q_start', starts(q_lens)); put('q_len', q_lens); put('k_start', starts(caps)); put('k_cap', caps); put('k_len', k_lens)
+        for name, tiles in (('q_tile', qf), ('q_tile_causal', qc), ('k_tile', kf), ('k_tile_causal', kc)):
+            put(name, [x for _, s, r in sorted(tiles) for x in (s, r)])
+        self._ints = torch.tensor(host, dtype=torch.int32).to(self.device)
+        self._ptr = {k: self._ints.data_ptr() + 4 * v for k, v in at.items()}
+        self.k_len = self._ints[at['k_len']:at['k_len'] + self.seqs]
+
+
+_PACKED_TILE = 128
+
+
+def packed_plan(q_lens, k_lens=None, k_cap=None, device='cuda'):
+    """The plan of a batch of recordings (see PackedPlan). q_lens: frames of each recording. k_lens: keys of each where they differ from the
+    queries (recording s's queries are its last q_lens[s] positions); k_cap: rows reserved for each recording's keys (one number or one
+    per recording). Make it once per batch, outside captured graphs."""
+    return PackedPlan(q_lens, k_lens, k_cap, device)
+
+
+def _rows_ok(what, plan, dtype, *ts):
+    """2-D row operands of the plan: on its device, of one type, unit column stride, one row per frame."""
+    if plan.device.index != torch.cuda.current_device():
+        raise _lib.PseldError(f"{what}: the plan lives on {plan.device}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in ts:
+        if t is None:
+            continue
+        if t.device != plan.device:
+            raise _lib.PseldError(f"{what}: operands must live on the plan's device {plan.device}, one is on {t.device}")
+        if t.dtype != dtype:
+            raise _lib.PseldError(f"{what}: operands must share one dtype ({dtype} and {t.dtype})")
+        if t.dim() != 2 or t.shape[0] != plan.rows or t.shape != ts[0].shape or t.stride(1) != 1:
+            raise _lib.PseldError(f"{what}: operands must be [rows of the plan = {plan.rows}, C] with unit stride along their columns, one is "
+                                  f"{tuple(t.shape)} with strides {t.stride()}")
+
+
+def _state_ok(what, plan, C, *ts):
+    for t in ts:
+        if t is not None and (t.device != plan.device or t.dtype != torch.float32 or tuple(t.shape) != (plan.seqs, C) or not t.is_contiguous()):
+            raise _lib.PseldError(f"{what}: states must be contiguous float32 [recordings = {plan.seqs}, C = {C}] on {plan.device}")
+
+
+def _linrec_ws(plan, C):
+    """Scratch of its own per call (segment compositions), from the caching allocator: nothing is shared between streams or captured graphs."""
+    nbytes = _lib.lib().pseld_linrec_workspace(plan.rows, plan.seqs, plan.max_q, C)
+    return (torch.empty(nbytes // 4, dtype=torch.float32, device=plan.device), nbytes) if nbytes else (None, 0)
+
+
+def linrec_fwd(g, n, plan, h0=None, reverse=False, need_saved=True, out=None):
+    """z = sigmoid(g), h_t = z_t h_{t-1} + (1 - z_t) n_t over every recording of the plan (from its last frame to its first when
+    reverse). g, n [rows, C] (row-strided views allowed), h0 f32 [recordings, C] or None (zeros).
+    Returns (h [rows, C], h_last f32 [recordings, C], what linrec_bwd needs or None)."""
+    _rows_ok("linrec_fwd", plan, g.dtype, g, n, out)
+    C = g.shape[1]
+    _state_ok("linrec_fwd", plan, C, h0)
+    L = _lib.lib()
+    h = torch.empty((plan.rows, C), dtype=g.dtype, device=g.device) if out is None else out
+    h_last = torch.empty((plan.seqs, C), dtype=torch.float32, device=g.device)
+    states = torch.empty((L.pseld_linrec_states(plan.rows, plan.seqs), C), dtype=torch.float32, device=g.device) if need_saved else None
+    ws, nbytes = _linrec_ws(plan, C)
+    rc = L.pseld_linrec_fwd(dtype_code(g), _lib.ptr(g), g.stride(0), _lib.ptr(n), n.stride(0), _lib.ptr(h0), _lib.ptr(h), h.stride(0),
+                            _lib.ptr(h_last), _lib.ptr(states), plan._ptr['q_start'], plan._ptr['q_len'], plan.seqs, plan.rows, plan.max_q, C,
+                            int(bool(reverse)), _lib.ptr(ws), nbytes, _lib.stream_ptr())
+    _lib.check(rc, "pseld_linrec_fwd")
+    return h, h_last, states
+
+
+def linrec_bwd(dh, g, n, saved, plan, dh_last=None, h0=None, reverse=False, dg=None, dn=None):
+    """Gradients of linrec_fwd for dh [rows, C] and dh_last f32 [recordings, C] (or None): (dg, dn, dh0 or None where h0 is None).
+    dg, dn: optional outputs (row-strided views allowed, e.g. the halves of the gates' projection's gradient)."""
+    _rows_ok("linrec_bwd", plan, g.dtype, g, n, dh, dg, dn)
+    C = g.shape[1]
+    _state_ok("linrec_bwd", plan, C, h0, dh_last)
+    L = _lib.lib()
+    if saved is None or tuple(saved.shape) != (L.pseld_linrec_states(plan.rows, plan.seqs), C) or saved.dtype != torch.float32 or saved.device != plan.device:
+        raise _lib.PseldError("linrec_bwd: saved must be what linrec_fwd(need_saved=True) returned for this plan")
+    dg = torch.empty((plan.rows, C), dtype=g.dtype, device=g.device) if dg is None else dg
+    dn = torch.empty((plan.rows, C), dtype=g.dtype, device=g.device) if dn is None else dn
+    dh0 = torch.empty((plan.seqs, C), dtype=torch.float32, device=g.device) if h0 is not None else None
+    ws, nbytes = _linrec_ws(plan, C)
+    rc = L.pseld_linrec_bwd(dtype_code(g), _lib.ptr(dh), dh.stride(0), _lib.ptr(g), g.stride(0), _lib.ptr(n), n.stride(0), _lib.ptr(saved),
+                            _lib.ptr(dh_last), _lib.ptr(dg), dg.stride(0), _lib.ptr(dn), dn.stride(0), _lib.ptr(dh0), plan._ptr['q_start'],
+                            plan._ptr['q_len'], plan.seqs, plan.rows, plan.max_q, C, int(bool(reverse)), _lib.ptr(ws), nbytes, _lib.stream_ptr())
+    _lib.check(rc, "pseld_linrec_bwd")
+    return dg, dn, dh0
