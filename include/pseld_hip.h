@@ -503,6 +503,32 @@ int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void* g, long l
                      const float* dh_last, void* dg, long lddg, void* dn, long lddn, float* dh0, const int* start, const int* len,
                      int seqs, long rows, int max_len, int C, int reverse, float* workspace, long workspace_bytes, void* stream);
 
+/* ---- attention over packed recordings ----------------------------------------------------------------------------------
+ * Beside pseld_mhsa (one length, all pairs, head_dim 64): recordings of different lengths back to back, causal or full, hq query heads that share
+ * hkv key heads, head sizes D = multiples of 8 up to 128, keys in slabs of a capacity (a cache), a learned relative position bias by
+ * buckets, and calls of few rows (the next frame of running streams), which share the keys between workgroups.
+ *   S = scale q k^T + table[bucket(key position - query position), head], P = softmax over the keys that the mask leaves, out = P v,
+ *   lse[row, head] = log sum exp S;  a row without keys: out 0, lse -inf. Query i of a recording stands at position i + k_len - q_len; causal: keys
+ *   behind a query's position are masked. |table| is taken to be below 1e37.
+ * plan: HOST array of 16 longs {seqs, rows, max_q, k_rows, max_k, q_tiles, k_tiles, then device int arrays as addresses: q_start[seqs],
+ * q_len[seqs], k_start[seqs], k_cap[seqs], k_len[seqs], q_tile[q_tiles][2], q_tile_causal, k_tile[k_tiles][2], k_tile_causal}: a tile is
+ * (recording, first row) of 128 rows of queries or of capacity, heaviest first. k_len may change between calls; it is held to 0 .. k_cap.
+ * strides: HOST array of longs, {row stride, head stride} in elements of q, k, v, out (bwd: dout, q, k, v, out, dq, dk, dv), whole
+ * 16-byte pieces; unit stride inside a head. table f32 [buckets, hq] or NULL; lut (device ints): the bucket of every distance
+ * -max_distance .. max_distance, then [buckets][2] first and last distance of each (none: first > last).
+ * bwd: dq, dk, dv (rows between k_len and k_cap get zeros) and, where dtable is not NULL, dtable (f32, accumulate: added to). With bf16 operands and a
+ * table gradient the sums that enter it are formed from f32 probabilities. Deterministic (no floating atomics between lanes).
+ * workspace: the matching *_workspace bytes (buckets = 0: no table; bwd: no table gradient), 16-byte aligned. */
+long pseld_packed_attn_fwd_workspace(const long* plan, int hq, int hkv, int D, int buckets);
+int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const long* strides,
+                          const long* plan, int hq, int hkv, int D, int causal, float scale, const float* table, const int* lut,
+                          int buckets, int max_distance, float* workspace, long workspace_bytes, void* stream);
+long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int buckets);
+int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                          void* dq, void* dk, void* dv, const long* strides, const long* plan, int hq, int hkv, int D, int causal, float scale,
+                          const float* table, const int* lut, int buckets, int max_distance, float* dtable, int accumulate,
+                          float* workspace, long workspace_bytes, void* stream);
+
 /* ---- output head ---------------------------------------------------------------------------------------------------
  * htsat.py:526-534 (token -> [C,2,32] map) + im2col of accdoa.py:230 tscam_conv((2,3), pad (0,1)):
  * tok [B,64,C] -> A [B*32, C*6] (k = c*6 + cf*3 + dt, matching the conv weight's [D, C, 2, 3] flattening).

@@ -1,0 +1,1096 @@
+// Attention over packed recordings, forward and backward, gfx950: recordings of different lengths back to back, causal or full, query heads that
+// share key heads, a learned relative position bias by buckets, head sizes that are multiples of 8 up to 128, bf16 and f32.
+//
+//   S = scale q k^T + bias[bucket(key position - query position)],  P = softmax over the keys the mask leaves,  out = P v,  lse = log sum exp S
+//   (a row that the mask leaves nothing: out 0, lse -inf).  Backward: delta = sum_j P dP (= sum_d dO O), dP = dO v^T, dS = P (dP - delta),
+//   dq = scale dS k, dk = scale dS^T q (over the query heads that share the key head), dv = P^T dO, dtable[b] = sum of dS over the pairs of bucket b.
+//
+// No score matrix exists in HBM. Scores are computed TRANSPOSED in the forward and dq kernels (accumulator rows = keys, lanes = queries), so a
+// query's maximum and sum are lane-local but for one exchange of the wave's halves, and the probabilities are the B operand of the second
+// product as they stand; the dk/dv kernel has lanes = keys for the same reason. K / V (Q / dO) tiles of 64 rows reach LDS by LDS-DMA, two
+// buffers, one barrier per tile; rows are lane-linear with their 16-byte pieces XOR-swizzled on the source address (image_swizzle),
+// which leaves both the row reads and the transposed reads free of bank conflicts without padding. Rows past a recording's end are never
+// addressed: the DMA repeats the last row and the mask drops it, so what a cache holds behind its length does not matter.
+//
+// bias: the table column of the workgroup's head is laid out by DISTANCE in LDS once (dist_fill); a tile whose distances are all at or past the
+// last bucket adds one constant instead (it goes into the exponent's offset for free), the others read their diagonal's values.
+// Its gradient: every wave adds its dS to LDS sums by distance, one copy per half wave, so that no two lanes of an instruction meet and
+// the order of additions is fixed; sums per workgroup are folded to buckets, and a last launch adds the workgroups in order, in 64 bits.
+// With bf16 operands O comes from rounded probabilities, so delta = dO O would be off by 2^-9 of itself - too coarse for the table's f32
+// gradient, whose sums cancel. There delta = sum_j P dP is computed in its own pass over the keys (DELTA mode) from f32 P and dP.
+#include "common.h"
+#include "mma_frag.h"
+#include <type_traits>
+
+namespace {
+
+constexpr int KT = 64;          // rows of a streamed tile
+constexpr int WR = 32;          // rows of a wave's own tile
+constexpr int TILE = 128;       // rows of a workgroup's own tile (four waves)
+constexpr int NEAR_PAD = 96;    // a tile that touches a distance below max_distance has none past max_distance + KT + WR - 2
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Strides { long rs, hs; };        // bytes between rows and between heads
+
+struct PAttnArgs {
+    const char *q, *k, *v, *dout, *o;
+    char *out, *dq, *dk, *dv;
+    Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
+    float* lse;                 // [rows, hq]
+    float* delta;               // [rows, hq]
+    const int *q_start, *q_len, *k_start, *k_cap, *k_len, *tiles;
+    int seqs, hq, hkv, D, causal, nsplit;
+    float scale, c;             // c = scale * log2(e)
+    const float* table; const int* lut; const int* ranges;      // [buckets, hq]; bucket of distance -max .. max; [buckets, 2] first and last distance
+    int buckets, maxd;
+    float* part;                // dtable: [tiles, hq, buckets]; split dk/dv: [nsplit, 2, rows of the tiles' list, D]; few rows: see there
+    int chunk, max_rows;        // few rows: keys per workgroup, rows reserved per key head
+};
+
+// Two waves per SIMD where 256 registers hold a wave's accumulators and operands: the compiler then keeps the accumulators in vector registers
+// (with more, it moves them to accumulation registers and back around every softmax). f32 operands of heads above 32 take the whole file.
+template <typename T, int DP> constexpr int waves_per_simd() { return sizeof(T) == 2 || DP == 32 ? 2 : 1; }
+
+// ---- LDS images: rows of DP elements, lane-linear, 16-byte pieces swizzled inside the row ------------------------------------------
+template <int RB> __device__ __forceinline__ int image_swizzle(int row) {
+    if constexpr (RB == 64) return (row >> 2) & 3;
+    else if constexpr (RB == 128) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
+    else return (row & 7) << 1;
+}
+template <typename T, int DP> struct Image {
+    static constexpr int RB = DP * (int)sizeof(T);
+    using M = AMma<T>;
+    using Frag = typename M::Frag;
+    // 8 consecutive elements 16 kk + 8 h2 .. of one row
+    static __device__ __forceinline__ Frag row_frag(const char* base, int row, int kk, int h2) {
+        const int f = image_swizzle<RB>(row);
+        if constexpr (sizeof(T) == 2) return *(const bf16x8*)(base + row * RB + (((2 * kk + h2) ^ f) << 4));
+        else {
+            const f32x4 a = *(const f32x4*)(base + row * RB + (((4 * kk + 2 * h2) ^ f) << 4));
+            const f32x4 b = *(const f32x4*)(base + row * RB + (((4 * kk + 2 * h2 + 1) ^ f) << 4));
+            Frag x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { x.v[j] = a[j]; x.v[4 + j] = b[j]; }
+            return x;
+        }
+    }
+    // element j = M[row0 + 8 (j >> 2) + 4 h2 + (j & 3)][col0 + (lane & 31)], the k order of an accumulator operand; row0 a multiple of 16
+    static __device__ __forceinline__ Frag col_frag(const char* base, int row0, int col0, int lane) {
+        if constexpr (sizeof(T) == 2) {
+            const int i = lane & 15, qq = i >> 2, p = i & 3, gsel = (lane >> 4) & 1, h2 = lane >> 5;
+            const int ra = row0 + 4 * h2 + qq, rb = ra + 8, ch = (col0 >> 3) + 2 * gsel + (p >> 1);
+            const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(base + ra * RB + ((ch ^ image_swizzle<RB>(ra)) << 4) + (p & 1) * 8));
+            const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(base + rb * RB + ((ch ^ image_swizzle<RB>(rb)) << 4) + (p & 1) * 8));
+            short8v s;
+            s[0] = lo[0]; s[1] = lo[1]; s[2] = lo[2]; s[3] = lo[3];
+            s[4] = hi[0]; s[5] = hi[1]; s[6] = hi[2]; s[7] = hi[3];
+            return __builtin_bit_cast(bf16x8, s);
+        } else {
+            const int col = col0 + (lane & 31), h2 = lane >> 5;
+            Frag x;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = row0 + 8 * (j >> 2) + 4 * h2 + (j & 3);
+                x.v[j] = *(const float*)(base + row * RB + (((col >> 2) ^ image_swizzle<RB>(row)) << 4) + (col & 3) * 4);
+            }
+            return x;
+        }
+    }
+};
+// the wave's operand rows straight from global memory: 8 elements at 16 kk + 8 h2 of the lane's row, zeros past the head's size
+template <typename T, int DP>
+__device__ __forceinline__ typename AMma<T>::Frag global_frag(const char* row, int kk, int h2, int D) {
+    typename AMma<T>::Frag f;
+    const int d = 16 * kk + 8 * h2;
+    if constexpr (sizeof(T) == 2) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (d < D) v = *(const f32x4*)(row + d * 2);
+        f = __builtin_bit_cast(bf16x8, v);
+    } else {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+        if (d < D) { x = *(const f32x4*)(row + d * 4); y = *(const f32x4*)(row + d * 4 + 16); }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { f.v[j] = x[j]; f.v[4 + j] = y[j]; }
+    }
+    return f;
+}
+
+// one LDS-DMA wave-instruction: 64 lanes x 16 B from (uniform base + per-lane 32-bit offset) to 1 KiB of LDS at a uniform address.
+// Inline asm, its waits counted by hand: the compiler would drain it in front of every fragment read.
+__device__ __forceinline__ void pa_dma(unsigned lds_dst, const void* sbase, unsigned voff) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(lds_dst), "s"(sbase) : "memory");
+}
+__device__ __forceinline__ const char* uniform_ptr(const char* p) {
+    const unsigned long long v = (unsigned long long)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+    return (const char*)(((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char*)p; }
+
+#define PA_SYNC_TILE()                                                  \
+    do {                                                                \
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");     \
+        __builtin_amdgcn_sched_barrier(0);                              \
+        __builtin_amdgcn_s_barrier();                                   \
+        __builtin_amdgcn_sched_barrier(0);                              \
+        asm volatile("" ::: "memory");                                  \
+    } while (0)
+
+// A stream of ROWS-row tiles of one operand into LDS by NW waves. Offsets of a whole tile are computed once; a tile that ends inside takes
+// its rows past the end from the last one.
+template <typename T, int DP, int ROWS, int NW> struct Stream {
+    static constexpr int RB = DP * (int)sizeof(T);
+    static constexpr int NI = ROWS * RB / 1024 / NW;       // wave-instructions per wave
+    static_assert(NI >= 1 && NI * NW * 1024 == ROWS * RB, "whole instructions per wave");
+    unsigned voff[NI];
+    unsigned rs;
+    int wave, lane, pieces;
+    __device__ __forceinline__ unsigned at(int j, int limit) const {
+        const int lin = (wave * NI + j) * 1024 + lane * 16, row = lin / RB, pos = (lin % RB) >> 4;
+        const int piece = min(pos ^ image_swizzle<RB>(row), pieces - 1);
+        return (unsigned)min(row, limit) * rs + (unsigned)piece * 16;
+    }
+    __device__ __forceinline__ void init(long row_bytes, int D, int w) {
+        wave = w; lane = threadIdx.x & 63; rs = (unsigned)row_bytes; pieces = D * (int)sizeof(T) / 16;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) voff[j] = at(j, ROWS - 1);
+    }
+    // base: first row of the tile (uniform); rows: rows that exist from there on (> 0)
+    __device__ __forceinline__ void load(const char* base, int rows, unsigned lds) const {
+        const char* b = uniform_ptr(base);
+        if (rows >= ROWS) {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) pa_dma(__builtin_amdgcn_readfirstlane(lds + (wave * NI + j) * 1024), b, voff[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) pa_dma(__builtin_amdgcn_readfirstlane(lds + (wave * NI + j) * 1024), b, at(j, rows - 1));
+        }
+    }
+};
+
+// ---- relative position bias by distance ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ int dist_count(int maxd) { return 2 * (maxd + NEAR_PAD) + 1; }
+__device__ __forceinline__ float bias_at(const PAttnArgs& a, int rel, int head) {
+    const int r = max(-a.maxd, min(a.maxd, rel));
+    return a.table[(long)a.lut[r + a.maxd] * a.hq + head] * LOG2E;
+}
+// dist[i] = log2(e) * bias of distance i - maxd - NEAR_PAD
+__device__ __forceinline__ void dist_fill(float* dist, const PAttnArgs& a, int head, int threads) {
+    const int n = dist_count(a.maxd);
+    for (int i = threadIdx.x; i < n; i += threads) dist[i] = bias_at(a, i - a.maxd - NEAR_PAD, head);
+}
+
+template <int N> __device__ __forceinline__ void zero_acc(f32x16 (&z)[N]) {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[t][e] = 0.f;
+}
+__device__ __forceinline__ float half_swap_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+
+// a transposed result z (rows = d in registers, lane & 31 = row of the output) x mul -> global rows. bf16: the halves trade 4-element pieces so that
+// a lane stores 16 bytes
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(char* row, bool live, const f32x16 (&z)[DP / 32], float mul, int D, int h2) {
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int g = 0; g < 4; g += 2) {
+                unsigned pc[2][2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    bf16x2 lo, hi;
+                    lo[0] = (bf16_t)(z[dt][4 * (g + i)] * mul); lo[1] = (bf16_t)(z[dt][4 * (g + i) + 1] * mul);
+                    hi[0] = (bf16_t)(z[dt][4 * (g + i) + 2] * mul); hi[1] = (bf16_t)(z[dt][4 * (g + i) + 3] * mul);
+                    pc[i][0] = __builtin_bit_cast(unsigned, lo); pc[i][1] = __builtin_bit_cast(unsigned, hi);
+                }
+                // half 0 keeps its piece g and takes the other half's piece g, half 1 its piece g + 1 and half 0's piece g + 1
+                const auto a = __builtin_amdgcn_permlane32_swap(pc[0][0], pc[1][0], false, false);
+                const auto b = __builtin_amdgcn_permlane32_swap(pc[0][1], pc[1][1], false, false);
+                const int d = dt * 32 + 8 * (g + h2);
+                typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+                if (live && d < D) *(u32x4*)(row + d * 2) = u32x4{a[0], b[0], a[1], b[1]};
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = dt * 32 + 8 * g + 4 * h2;
+                if (live && d < D) *(f32x4*)(row + d * 4) = f32x4{z[dt][4 * g] * mul, z[dt][4 * g + 1] * mul, z[dt][4 * g + 2] * mul, z[dt][4 * g + 3] * mul};
+            }
+        }
+    }
+}
+
+// z (rows = d) += M[tile rows][d]^T x, x = accumulator tiles whose rows are the tile's rows t0 * 32 ..
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void acc_product(f32x16 (&z)[DP / 32], const f32x16 (&x)[NT], const char* tile, int t0, int lane) {
+    using I = Image<T, DP>;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const typename I::Frag fx = I::M::from_acc(x[t], s);
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) I::M::mma(I::col_frag(tile, (t0 + t) * 32 + 16 * s, dt * 32, lane), fx, z[dt]);
+        }
+}
+
+// The running maximum, sum and output of a wave's 32 queries (lane & 31), keys in accumulator rows.
+template <int DP> struct Softmax {
+    f32x16 ot[DP / 32];
+    float m, l;                 // log2 units; l holds the lane half's own keys
+    __device__ __forceinline__ void init() { zero_acc(ot); m = -__builtin_inff(); l = 0.f; }
+    // x: raw products; score = x * c + off. The maximum may lag by up to 2^8 (the sums are f32, the probabilities keep their relative
+    // rounding), so most tiles do not touch the output accumulators.
+    template <int NT> __device__ __forceinline__ void step(f32x16 (&x)[NT], float c, float off) {
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
+        mx = half_swap_max(mx);
+        mx = fmaf(mx, c, off);
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ot[dt][e] *= alpha;
+        }
+        const float sub = off - (m == -__builtin_inff() ? 0.f : m);
+        float ps = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(x[t][e], c, sub));
+                x[t][e] = p;
+                ps += p;
+            }
+        l += ps;
+    }
+};
+
+// Adds the bias of a tile's own diagonal values: x = x * c + dist[key - query]; d points at the entry of (accumulator row 0, this lane's query)
+template <int NT, int SIGN> __device__ __forceinline__ void add_near_bias(f32x16 (&x)[NT], float c, const float* d) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[t][e] = fmaf(x[t][e], c, d[SIGN * (t * 32 + (e & 3) + 8 * (e >> 2))]);
+}
+// keeps rows <= lim (rows counted from the tile's first, lim already less 4 * (lane >> 5))
+template <int NT> __device__ __forceinline__ void mask_rows(f32x16 (&x)[NT], int lim, float with) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[t][e] = (t * 32 + (e & 3) + 8 * (e >> 2)) <= lim ? x[t][e] : with;
+}
+
+// which recording, rows and head a workgroup of the query-tiled kernels owns. Heads fastest, the query heads of one key head a multiple of
+// hkv apart: with hkv a multiple of the eight XCDs every key head's tiles stay on one XCD's L2
+struct QTile {
+    int seq, q0, q_len, k_len, off, head, kvh, nk;
+    long q_row, k_row;
+};
+__device__ __forceinline__ QTile q_tile_of(const PAttnArgs& a) {
+    QTile t;
+    const int p = blockIdx.x % a.hq, ti = blockIdx.x / a.hq;
+    t.kvh = p % a.hkv;
+    t.head = t.kvh * (a.hq / a.hkv) + p / a.hkv;
+    t.seq = a.tiles[2 * ti];
+    t.q0 = a.tiles[2 * ti + 1];
+    t.q_len = a.q_len[t.seq];
+    t.k_len = max(0, min(a.k_len[t.seq], a.k_cap[t.seq]));
+    t.off = t.k_len - t.q_len;
+    t.q_row = a.q_start[t.seq];
+    t.k_row = a.k_start[t.seq];
+    t.nk = a.causal ? max(0, min(t.k_len, t.q0 + TILE + t.off)) : t.k_len;
+    return t;
+}
+
+// ---- forward: 128 queries of one (recording, head), a wave 32 --------------------------------------------------------------------------
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fwd_kernel(PAttnArgs a) {
+    using I = Image<T, DP>;
+    constexpr int TB = KT * I::RB;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];      // 2 x (K tile | V tile) | bias by distance
+    float* dist = (float*)(smem + 4 * TB);
+    const QTile w = q_tile_of(a);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
+    const int qi = w.q0 + wave * WR + r;
+    const bool live = qi < w.q_len;
+    const long qrow = w.q_row + min(qi, w.q_len - 1);
+    const char* kb = a.k + w.k_row * a.sk.rs + (long)w.kvh * a.sk.hs;
+    const char* vb = a.v + w.k_row * a.sv.rs + (long)w.kvh * a.sv.hs;
+    Stream<T, DP, KT, 4> ks, vs;
+    ks.init(a.sk.rs, a.D, wave);
+    vs.init(a.sv.rs, a.D, wave);
+    const unsigned lds0 = lds_addr(smem);
+    const int nt = (w.nk + KT - 1) / KT;
+    if (nt) { ks.load(kb, w.k_len, lds0); vs.load(vb, w.k_len, lds0 + TB); }
+    if constexpr (BIAS) dist_fill(dist, a, w.head, 256);
+    typename I::Frag fq[DP / 16];
+    {
+        const char* row = a.q + qrow * a.sq.rs + (long)w.head * a.sq.hs;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) fq[kk] = global_frag<T, DP>(row, kk, h2, a.D);
+    }
+    const int qpos = qi + w.off, qw0 = w.q0 + wave * WR + w.off;        // the lane's and the wave's first query position
+    const int klim = a.causal ? min(w.k_len - 1, qpos) : w.k_len - 1;
+    const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;   // every query of the wave sees keys up to here,
+    const int wlim1 = w.q0 + wave * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;     // none sees one past here
+    float far_lo = 0.f, far_hi = 0.f;
+    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, w.head); far_hi = bias_at(a, a.maxd, w.head); }
+    Softmax<DP> sm;
+    sm.init();
+    for (int i = 0; i < nt; ++i) {
+        const char* kt = smem + (i & 1) * 2 * TB;
+        const char* vt = kt + TB;
+        const int k0 = i * KT;
+        PA_SYNC_TILE();
+        if (i + 1 < nt) {
+            const unsigned dst = lds0 + ((i + 1) & 1) * 2 * TB;
+            ks.load(kb + (long)(k0 + KT) * a.sk.rs, w.k_len - k0 - KT, dst);
+            vs.load(vb + (long)(k0 + KT) * a.sv.rs, w.k_len - k0 - KT, dst + TB);
+        }
+        if (k0 > wlim1) continue;
+        f32x16 st[2];
+        zero_acc(st);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) I::M::mma(I::row_frag(kt, t * 32 + r, kk, h2), fq[kk], st[t]);
+        float c = a.c, off = 0.f;
+        if constexpr (BIAS) {
+            const int lo = k0 - (qw0 + WR - 1), hi = k0 + KT - 1 - qw0;      // the tile's smallest and largest distance
+            if (hi <= -a.maxd) off = far_lo;
+            else if (lo >= a.maxd) off = far_hi;
+            else { add_near_bias<2, 1>(st, c, dist + (k0 + 4 * h2 - qpos + a.maxd + NEAR_PAD)); c = 1.f; }
+        }
+        if (k0 + KT - 1 > wlim0) mask_rows<2>(st, klim - k0 - 4 * h2, -__builtin_inff());
+        sm.template step<2>(st, c, off);
+        acc_product<T, DP, 2>(sm.ot, st, vt, 0, lane);
+    }
+    const float l = sm.l + __shfl_xor(sm.l, 32, 64);
+    store_rows<T, DP>(a.out + qrow * a.so.rs + (long)w.head * a.so.hs, live, sm.ot, l > 0.f ? 1.f / l : 0.f, a.D, h2);
+    if (live && h2 == 0) a.lse[qrow * a.hq + w.head] = l > 0.f ? (sm.m + __log2f(l)) * LN2 : -__builtin_inff();
+}
+
+// ---- few rows: a step of running streams ------------------------------------------------------------------------------------------------
+// A recording's q_len x (hq / hkv) rows of one key head fit one 32-row operand. A workgroup takes `chunk` keys of one (recording, key head), its
+// waves 32-key blocks in turn; a wave streams its own blocks through its own LDS (no barrier in the loop) and the waves' maxima, sums
+// and outputs are joined through LDS. More than one chunk per recording: f32 partials and a joining launch, both in a fixed order. HBM
+// bound: K and V are read once for all rows that share them.
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
+    using I = Image<T, DP>;
+    constexpr int BB = WR * I::RB;                         // one block of K or V
+    extern __shared__ __attribute__((aligned(1024))) char smem[];      // waves x 2 x (K | V) | (waves + 1) x 32 x (m, l) | table | lut
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
+    const int kvh = blockIdx.x % a.hkv, rest = blockIdx.x / a.hkv, split = rest % a.nsplit, seq = rest / a.nsplit;
+    const int G = a.hq / a.hkv, q_len = a.q_len[seq];
+    const int k_len = max(0, min(a.k_len[seq], a.k_cap[seq])), rows = q_len * G;
+    const int kbeg = split * a.chunk, kend = min(k_len, kbeg + a.chunk);
+    if (rows == 0 || (kbeg >= k_len && split)) return;     // chunk 0 answers for a recording without keys
+    float* ml = (float*)(smem + NW * 4 * BB);
+    float* all = ml + NW * 64;                             // the waves' joined (m, l)
+    float* tab = all + 64;
+    unsigned short* lut = (unsigned short*)(tab + a.buckets * G);
+    const int off = k_len - q_len;
+    if constexpr (BIAS) {
+        if (kend - 1 - off > -a.maxd) {                    // some key is near some query
+            for (int i = threadIdx.x; i < a.buckets * G; i += 64 * NW) tab[i] = a.table[(long)(i / G) * a.hq + kvh * G + i % G] * LOG2E;
+            for (int i = threadIdx.x; i <= 2 * a.maxd; i += 64 * NW) lut[i] = (unsigned short)a.lut[i];
+        }
+        __syncthreads();
+    }
+    const int rr = min(r, rows - 1), qi = rr / G, g = rr - qi * G;
+    const long qrow = (long)a.q_start[seq] + qi;
+    typename I::Frag fq[DP / 16];
+    {
+        const char* row = a.q + qrow * a.sq.rs + (long)(kvh * G + g) * a.sq.hs;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) fq[kk] = global_frag<T, DP>(row, kk, h2, a.D);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing of the compiler's stays in flight among the counted DMAs
+    const int qpos = qi + off, klim = a.causal ? min(k_len - 1, qpos) : k_len - 1;
+    float far_lo = 0.f, far_hi = 0.f;
+    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, kvh * G + g); far_hi = bias_at(a, a.maxd, kvh * G + g); }
+    const char* kb = a.k + (long)a.k_start[seq] * a.sk.rs + (long)kvh * a.sk.hs;
+    const char* vb = a.v + (long)a.k_start[seq] * a.sv.rs + (long)kvh * a.sv.hs;
+    Stream<T, DP, WR, 1> ks, vs;
+    ks.init(a.sk.rs, a.D, 0);
+    vs.init(a.sv.rs, a.D, 0);
+    char* mine = smem + wave * 4 * BB;
+    const unsigned lds0 = lds_addr(mine);
+    Softmax<DP> sm;
+    sm.init();
+    const int first = kbeg + wave * WR;
+    if (BIAS) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (first < kend) { ks.load(kb + (long)first * a.sk.rs, k_len - first, lds0); vs.load(vb + (long)first * a.sv.rs, k_len - first, lds0 + BB); }
+    int par = 0;
+    for (int k0 = first; k0 < kend; k0 += NW * WR, par ^= 1) {
+        const int nx = k0 + NW * WR;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the last block's reads are done with the buffer that is filled next
+        if (nx < kend) {
+            const unsigned dst = lds0 + (par ^ 1) * 2 * BB;
+            ks.load(kb + (long)nx * a.sk.rs, k_len - nx, dst);
+            vs.load(vb + (long)nx * a.sv.rs, k_len - nx, dst + BB);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Stream<T, DP, WR, 1>::NI) : "memory");
+        } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        const char* kt = mine + par * 2 * BB;
+        f32x16 st[1];
+        zero_acc(st);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) I::M::mma(I::row_frag(kt, r, kk, h2), fq[kk], st[0]);
+        float c = a.c, o = 0.f;
+        if constexpr (BIAS) {
+            const int lo = k0 - (k_len - 1), hi = min(k0 + WR, kend) - 1 - off;      // over every query of the recording
+            if (hi <= -a.maxd) o = far_lo;
+            else if (lo >= a.maxd) o = far_hi;
+            else {
+                const int base = k0 + 4 * h2 - qpos + a.maxd;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int i = max(0, min(2 * a.maxd, base + (e & 3) + 8 * (e >> 2)));
+                    st[0][e] = fmaf(st[0][e], c, tab[lut[i] * G + g]);
+                }
+                c = 1.f;
+            }
+        }
+        if (a.causal ? k0 + WR - 1 > min(k_len - 1, off) || k0 + WR > kend : k0 + WR > kend) mask_rows<1>(st, min(klim, kend - 1) - k0 - 4 * h2, -__builtin_inff());
+        sm.template step<1>(st, c, o);
+        acc_product<T, DP, 1>(sm.ot, st, kt + BB, 0, lane);
+    }
+    // join the waves
+    const float l = sm.l + __shfl_xor(sm.l, 32, 64);
+    if (h2 == 0) { ml[wave * 64 + r] = sm.m; ml[wave * 64 + 32 + r] = l; }
+    __syncthreads();
+    float mt = -__builtin_inff(), lt = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) mt = fmaxf(mt, ml[x * 64 + r]);
+#pragma unroll
+    for (int x = 0; x < NW; ++x) { const float mx = ml[x * 64 + r]; lt += mx == -__builtin_inff() ? 0.f : ml[x * 64 + 32 + r] * __builtin_amdgcn_exp2f(mx - mt); }
+    const float f = sm.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sm.m - mt);
+    constexpr int PITCH = DP + 4;                          // floats per row of a wave's output image: 32 rows of 4-float pieces fall in different banks
+    static_assert(32 * PITCH * 4 <= 4 * BB, "the output image fits the wave's buffers");
+    float* oi = (float*)mine;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int gg = 0; gg < 4; ++gg)
+            *(f32x4*)(oi + r * PITCH + dt * 32 + 8 * gg + 4 * h2) = f32x4{sm.ot[dt][4 * gg] * f, sm.ot[dt][4 * gg + 1] * f, sm.ot[dt][4 * gg + 2] * f, sm.ot[dt][4 * gg + 3] * f};
+    if (wave == 0 && h2 == 0) { all[r] = mt; all[32 + r] = lt; }
+    __syncthreads();
+    const long pslot = ((long)(seq * a.hkv + kvh) * a.nsplit + split) * a.max_rows;
+    for (int i = threadIdx.x; i < rows * (a.D / 4); i += 64 * NW) {
+        const int row = i / (a.D / 4), d = (i - row * (a.D / 4)) * 4;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < NW; ++x) s += *(const f32x4*)((const float*)(smem + x * 4 * BB) + row * PITCH + d);
+        const float m = all[row], lr = all[32 + row];
+        if (a.nsplit > 1) {
+            float* p = a.part + (pslot + row) * (a.D + 4);
+            *(f32x4*)(p + 4 + d) = s;
+            if (d == 0) { p[0] = m; p[1] = lr; }
+        } else {
+            const int qj = row / G, head = kvh * G + row - qj * G;
+            const long qr = (long)a.q_start[seq] + qj;
+            const float inv = lr > 0.f ? 1.f / lr : 0.f;
+            store4<T>(a.out + qr * a.so.rs + (long)head * a.so.hs + d * (int)sizeof(T), s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
+            if (d == 0) a.lse[qr * a.hq + head] = lr > 0.f ? (m + __log2f(lr)) * LN2 : -__builtin_inff();
+        }
+    }
+}
+// one wave joins the chunks of one (row, head): weights from the chunks' maxima and sums, then a weighted sum in chunk order
+template <typename T>
+__global__ __launch_bounds__(64) void packed_attn_join_kernel(PAttnArgs a) {
+    extern __shared__ float wgt[];
+    const int G = a.hq / a.hkv, lane = threadIdx.x;
+    const int row = blockIdx.x % a.max_rows, rest = blockIdx.x / a.max_rows, kvh = rest % a.hkv, seq = rest / a.hkv;
+    if (row >= a.q_len[seq] * G) return;
+    const int k_len = max(0, min(a.k_len[seq], a.k_cap[seq]));
+    const int n = max(1, (k_len + a.chunk - 1) / a.chunk);
+    const float* p = a.part + ((long)(seq * a.hkv + kvh) * a.nsplit * a.max_rows + row) * (a.D + 4);
+    const long step = (long)a.max_rows * (a.D + 4);
+    float m = -__builtin_inff();
+    for (int i = lane; i < n; i += 64) m = fmaxf(m, p[i * step]);
+    m = wave_max(m);
+    float l = 0.f;
+    for (int i = lane; i < n; i += 64) {
+        const float mi = p[i * step], w = mi == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mi - m);
+        wgt[i] = w;
+        l += w * p[i * step + 1];
+    }
+    l = wave_sum(l);
+    __syncthreads();
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int qj = row / G, head = kvh * G + row - qj * G;
+    const long qr = (long)a.q_start[seq] + qj;
+    // 16-lane groups take the chunks in turn, 8 elements a lane; the four groups' sums meet by shuffles
+    const int dl = (lane & 15) * 8, grp = lane >> 4;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (dl < a.D) {
+#pragma unroll 4
+        for (int i = grp; i < n; i += 4) {
+            float x[8];
+            load8<float>(p + i * step + 4 + dl, x);
+            const float w = wgt[i];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] = fmaf(w, x[j], s[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        s[j] += __shfl_xor(s[j], 16, 64);
+        s[j] += __shfl_xor(s[j], 32, 64);
+        s[j] *= inv;
+    }
+    if (grp == 0 && dl < a.D) store8<T>((T*)(a.out + qr * a.so.rs + (long)head * a.so.hs) + dl, s);
+    if (lane == 0) a.lse[qr * a.hq + head] = l > 0.f ? (m + __log2f(l)) * LN2 : -__builtin_inff();
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------------------------------
+// delta[row, head] = sum_d dO O; 16 lanes per (row, head)
+template <typename T>
+__global__ __launch_bounds__(256) void packed_attn_delta_kernel(PAttnArgs a, long n) {
+    const long i = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int d = (threadIdx.x & 15) * 8;
+    float s = 0.f;
+    if (i < n && d < a.D) {
+        const long row = i / a.hq;
+        const int head = (int)(i - row * a.hq);
+        float x[8], y[8];
+        load8<T>((const T*)(a.o + row * a.so.rs + (long)head * a.so.hs) + d, x);
+        load8<T>((const T*)(a.dout + row * a.sdo.rs + (long)head * a.sdo.hs) + d, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(x[j], y[j], s);
+    }
+    s = group_sum<16>(s);
+    if (i < n && d == 0) a.delta[i] = s;
+}
+
+enum { DQ = 0, DQ_TABLE = 1, DELTA = 2 };
+
+// dq (and the table's gradient), tiled like the forward; DELTA: only delta = sum_j P dP
+// (f32 heads of 128 with the table: two buffers and the sums for 1024 distances would not fit 160 KB, so that variant has one buffer)
+template <typename T, int DP, int MODE> constexpr int dq_buffers() { return sizeof(T) == 4 && DP == 128 && MODE == DQ_TABLE ? 1 : 2; }
+template <typename T, int DP, bool BIAS, int MODE>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq_kernel(PAttnArgs a) {
+    using I = Image<T, DP>;
+    constexpr int TB = KT * I::RB, NB = dq_buffers<T, DP, MODE>();
+    extern __shared__ __attribute__((aligned(1024))) char smem[];      // NB x (K | V) | bias by distance | sums by distance, 8 copies | 8 floats
+    float* dist = (float*)(smem + NB * 2 * TB);
+    const int ndist = BIAS ? dist_count(a.maxd) : 0;
+    float* hist = dist + ndist;
+    const QTile w = q_tile_of(a);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
+    const int qi = w.q0 + wave * WR + r;
+    const bool live = qi < w.q_len;
+    const long qrow = w.q_row + min(qi, w.q_len - 1);
+    const char* kb = a.k + w.k_row * a.sk.rs + (long)w.kvh * a.sk.hs;
+    const char* vb = a.v + w.k_row * a.sv.rs + (long)w.kvh * a.sv.hs;
+    Stream<T, DP, KT, 4> ks, vs;
+    ks.init(a.sk.rs, a.D, wave);
+    vs.init(a.sv.rs, a.D, wave);
+    const unsigned lds0 = lds_addr(smem);
+    const int nt = (w.nk + KT - 1) / KT;
+    if (nt) { ks.load(kb, w.k_len, lds0); vs.load(vb, w.k_len, lds0 + TB); }
+    if constexpr (BIAS) dist_fill(dist, a, w.head, 256);
+    if constexpr (MODE == DQ_TABLE)
+        for (int i = threadIdx.x; i < 8 * ndist; i += 256) hist[i] = 0.f;
+    typename I::Frag fq[DP / 16], fo[DP / 16];
+    {
+        const char* row = a.q + qrow * a.sq.rs + (long)w.head * a.sq.hs;
+        const char* dor = a.dout + qrow * a.sdo.rs + (long)w.head * a.sdo.hs;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) { fq[kk] = global_frag<T, DP>(row, kk, h2, a.D); fo[kk] = global_frag<T, DP>(dor, kk, h2, a.D); }
+    }
+    const long si = qrow * a.hq + w.head;
+    const float lse = a.lse[si];
+    const float lse2 = live && lse > -__builtin_inff() ? lse * LOG2E : __builtin_inff();      // +inf: every probability of the row is 0
+    float dl = 0.f;
+    if constexpr (MODE != DELTA) dl = a.delta[si];
+    const int qpos = qi + w.off, qw0 = w.q0 + wave * WR + w.off;
+    const int klim = a.causal ? min(w.k_len - 1, qpos) : w.k_len - 1;
+    const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;
+    const int wlim1 = w.q0 + wave * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;
+    float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f;
+    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, w.head); far_hi = bias_at(a, a.maxd, w.head); }
+    f32x16 dq[DP / 32];
+    zero_acc(dq);
+    for (int i = 0; i < nt; ++i) {
+        const char* kt = smem + (NB == 2 ? i & 1 : 0) * 2 * TB;
+        const char* vt = kt + TB;
+        const int k0 = i * KT;
+        PA_SYNC_TILE();
+        if (NB == 1 && i) {
+            ks.load(kb + (long)k0 * a.sk.rs, w.k_len - k0, lds0);
+            vs.load(vb + (long)k0 * a.sv.rs, w.k_len - k0, lds0 + TB);
+            PA_SYNC_TILE();
+        }
+        if (NB == 2 && i + 1 < nt) {
+            const unsigned dst = lds0 + ((i + 1) & 1) * 2 * TB;
+            ks.load(kb + (long)(k0 + KT) * a.sk.rs, w.k_len - k0 - KT, dst);
+            vs.load(vb + (long)(k0 + KT) * a.sv.rs, w.k_len - k0 - KT, dst + TB);
+        }
+        if (k0 > wlim1) continue;
+        f32x16 st[2], dp[2];
+        zero_acc(st);
+        zero_acc(dp);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                I::M::mma(I::row_frag(kt, t * 32 + r, kk, h2), fq[kk], st[t]);
+                I::M::mma(I::row_frag(vt, t * 32 + r, kk, h2), fo[kk], dp[t]);
+            }
+        float c = a.c, off = 0.f;
+        int where = 0;                       // of the tile's distances: -1 / 1 all at or past -maxd / maxd, 0 near
+        const int di = k0 + 4 * h2 - qpos + a.maxd + NEAR_PAD;
+        if constexpr (BIAS) {
+            const int lo = k0 - (qw0 + WR - 1), hi = k0 + KT - 1 - qw0;
+            if (hi <= -a.maxd) { off = far_lo; where = -1; }
+            else if (lo >= a.maxd) { off = far_hi; where = 1; }
+            else { add_near_bias<2, 1>(st, c, dist + di); c = 1.f; }
+        }
+        if (k0 + KT - 1 > wlim0) mask_rows<2>(st, klim - k0 - 4 * h2, -__builtin_inff());
+        const float sub = off - lse2;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e], c, sub));
+                if constexpr (MODE == DELTA) dl = fmaf(p, dp[t][e], dl);
+                else st[t][e] = p * (dp[t][e] - dl);
+            }
+        if constexpr (MODE == DQ_TABLE) {
+            if (where == 0) {
+                float* hp = hist + (wave * 2 + h2) * ndist + di;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float*)(hp + t * 32 + (e & 3) + 8 * (e >> 2)), st[t][e], 0, 0, false);
+            } else {
+                float s = 0.f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s += st[t][e];
+                if (where < 0) sum_lo += s; else sum_hi += s;
+            }
+        }
+        if constexpr (MODE != DELTA) acc_product<T, DP, 2>(dq, st, kt, 0, lane);
+    }
+    if constexpr (MODE == DELTA) {
+        dl += __shfl_xor(dl, 32, 64);
+        if (live && h2 == 0) a.delta[si] = dl;
+    } else store_rows<T, DP>(a.dq + qrow * a.sdq.rs + (long)w.head * a.sdq.hs, live, dq, a.scale, a.D, h2);
+    if constexpr (MODE == DQ_TABLE) {
+        float* far = hist + 8 * ndist;
+        sum_lo = wave_sum(sum_lo);
+        sum_hi = wave_sum(sum_hi);
+        if (lane == 0) { far[wave * 2] = sum_lo; far[wave * 2 + 1] = sum_hi; }
+        __syncthreads();
+        for (int i = threadIdx.x; i < ndist; i += 256) {
+            float s = 0.f;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) s += hist[x * ndist + i];
+            dist[i] = s;
+        }
+        __syncthreads();
+        float* part = a.part + ((long)(blockIdx.x / a.hq) * a.hq + w.head) * a.buckets;
+        for (int b = threadIdx.x; b < a.buckets; b += 256) {
+            const int first = a.ranges[2 * b], last = a.ranges[2 * b + 1];      // distances of the bucket; none: first > last
+            float s = 0.f;
+            if (first <= last) {
+                const int i0 = first <= -a.maxd ? 0 : first + a.maxd + NEAR_PAD, i1 = last >= a.maxd ? ndist - 1 : last + a.maxd + NEAR_PAD;
+                if (first <= -a.maxd) s += far[0] + far[2] + far[4] + far[6];
+                if (last >= a.maxd) s += far[1] + far[3] + far[5] + far[7];
+                for (int i = i0; i <= i1; ++i) s += dist[i];
+            }
+            part[b] = s;
+        }
+    }
+}
+
+// dtable[b, head] (+)= sum over the query tiles, in their order, in 64 bits; one workgroup per (head, 16 buckets)
+__global__ __launch_bounds__(256) void packed_attn_table_kernel(const float* part, float* dtable, int tiles, int hq, int buckets, int accumulate) {
+    __shared__ double acc[16][16];
+    const int head = blockIdx.x % hq, b = (blockIdx.x / hq) * 16 + (threadIdx.x & 15), g = threadIdx.x >> 4;
+    double s = 0.0;
+    if (b < buckets)
+        for (int i = g; i < tiles; i += 16) s += (double)part[((long)i * hq + head) * buckets + b];
+    acc[g][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (g == 0 && b < buckets) {
+        for (int i = 1; i < 16; ++i) s += acc[i][threadIdx.x];
+        float* d = dtable + (long)b * hq + head;
+        *d = accumulate ? (float)(s + (double)*d) : (float)s;
+    }
+}
+
+// dk, dv: 128 keys of one (recording, key head), a wave 32 (lanes = keys); the query heads of the group and the 64-query tiles stream by.
+// nsplit > 1: the stream is shared between nsplit workgroups, f32 partials are added in order by packed_attn_dkv_join_kernel.
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dkv_kernel(PAttnArgs a) {
+    using I = Image<T, DP>;
+    constexpr int TB = KT * I::RB;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];      // 2 x (Q | dO) | 2 x (lse | delta) x 64 | bias by distance
+    float* stat = (float*)(smem + 4 * TB);
+    float* dist = stat + 4 * KT;
+    const int kvh = blockIdx.x % a.hkv, rest = blockIdx.x / a.hkv, split = rest % a.nsplit, ti = rest / a.nsplit;
+    const int seq = a.tiles[2 * ti], kt0 = a.tiles[2 * ti + 1];
+    const int q_len = a.q_len[seq], k_cap = a.k_cap[seq], k_len = max(0, min(a.k_len[seq], k_cap)), off = k_len - q_len, G = a.hq / a.hkv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
+    const int kw0 = kt0 + wave * WR, key = kw0 + r;
+    const long krow = (long)a.k_start[seq] + min(key, k_cap - 1);
+    const bool live = key < k_cap;                         // rows between a recording's length and its capacity get zeros
+    f32x16 dk[DP / 32], dv[DP / 32];
+    zero_acc(dk);
+    zero_acc(dv);
+    // query tiles from the first that a key of this tile is seen by
+    const int qfirst = kt0 >= k_len ? q_len : a.causal ? max(0, kt0 - off) / KT * KT : 0;
+    const int per = qfirst < q_len ? (q_len - qfirst + KT - 1) / KT : 0, total = per * G;
+    const int i0 = (int)((long)total * split / a.nsplit), i1 = (int)((long)total * (split + 1) / a.nsplit);
+    if (i0 < i1) {
+        typename I::Frag fk[DP / 16], fv[DP / 16];
+        {
+            const long kr = (long)a.k_start[seq] + min(key, k_len - 1);
+            const char* krp = a.k + kr * a.sk.rs + (long)kvh * a.sk.hs;
+            const char* vrp = a.v + kr * a.sv.rs + (long)kvh * a.sv.hs;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) { fk[kk] = global_frag<T, DP>(krp, kk, h2, a.D); fv[kk] = global_frag<T, DP>(vrp, kk, h2, a.D); }
+        }
+        Stream<T, DP, KT, 4> qs, os;
+        qs.init(a.sq.rs, a.D, wave);
+        os.init(a.sdo.rs, a.D, wave);
+        const unsigned lds0 = lds_addr(smem);
+        float reg = 0.f;                                   // threads 0..63: lse of the next tile, 64..127: delta
+        auto fetch = [&](int it, unsigned dst) {
+            const int g = it / per, q0 = qfirst + (it - g * per) * KT, head = kvh * G + g;
+            const long row = (long)a.q_start[seq] + q0;
+            if (threadIdx.x < 2 * KT) {
+                const int j = threadIdx.x & (KT - 1);
+                const bool in = q0 + j < q_len;
+                const long s = (row + min(j, q_len - 1 - q0)) * a.hq + head;
+                if (threadIdx.x < KT) {
+                    const float x = a.lse[s];
+                    reg = in && x > -__builtin_inff() ? x * LOG2E : __builtin_inff();
+                } else reg = in ? a.delta[s] : 0.f;
+            }
+            qs.load(a.q + row * a.sq.rs + (long)head * a.sq.hs, q_len - q0, dst);
+            os.load(a.dout + row * a.sdo.rs + (long)head * a.sdo.hs, q_len - q0, dst + TB);
+        };
+        fetch(i0, lds0);
+        int held = -1;                                     // the head whose bias LDS holds
+        float far_lo = 0.f, far_hi = 0.f;
+        for (int it = i0; it < i1; ++it) {
+            const int par = (it - i0) & 1, g = it / per, q0 = qfirst + (it - g * per) * KT;
+            const char* qt = smem + par * 2 * TB;
+            const char* ot = qt + TB;
+            float* ls = stat + par * 2 * KT;
+            if (threadIdx.x < 2 * KT) ls[threadIdx.x] = reg;
+            if constexpr (BIAS) {
+                if (g != held) {                           // uniform; the last tile's readers are past the barrier below before anything is overwritten
+                    if (held >= 0) __syncthreads();
+                    held = g;
+                    dist_fill(dist, a, kvh * G + g, 256);
+                    far_lo = bias_at(a, -a.maxd, kvh * G + g);
+                    far_hi = bias_at(a, a.maxd, kvh * G + g);
+                }
+            }
+            PA_SYNC_TILE();
+            if (it + 1 < i1) fetch(it + 1, lds0 + (par ^ 1) * 2 * TB);
+            const int qp0 = q0 + off;                      // position of the tile's first query
+            if (kw0 >= k_len || (a.causal && qp0 + KT - 1 < kw0)) continue;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x16 s[1], dp[1];
+                zero_acc(s);
+                zero_acc(dp);
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    I::M::mma(I::row_frag(qt, t * 32 + r, kk, h2), fk[kk], s[0]);      // rows = queries, lanes = keys
+                    I::M::mma(I::row_frag(ot, t * 32 + r, kk, h2), fv[kk], dp[0]);
+                }
+                float c = a.c, bo = 0.f;
+                const int qt0 = qp0 + t * 32;
+                if constexpr (BIAS) {
+                    const int lo = kw0 - (qt0 + 31), hi = kw0 + WR - 1 - qt0;
+                    if (hi <= -a.maxd) bo = far_lo;
+                    else if (lo >= a.maxd) bo = far_hi;
+                    else { add_near_bias<1, -1>(s, c, dist + (key - qt0 - 4 * h2 + a.maxd + NEAR_PAD)); c = 1.f; }
+                }
+                if (kw0 + WR > k_len || (a.causal && qt0 < kw0 + WR - 1)) {            // some pair is masked: keep key < k_len and query >= key
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int qp = qt0 + (e & 3) + 8 * (e >> 2) + 4 * h2;
+                        s[0][e] = key < k_len && (!a.causal || qp >= key) ? s[0][e] : -__builtin_inff();
+                    }
+                }
+#pragma unroll
+                for (int gq = 0; gq < 4; ++gq) {
+                    const f32x4 lv = *(const f32x4*)(ls + t * 32 + 8 * gq + 4 * h2);
+                    const f32x4 dl = *(const f32x4*)(ls + KT + t * 32 + 8 * gq + 4 * h2);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = 4 * gq + i;
+                        const float p = __builtin_amdgcn_exp2f(fmaf(s[0][e], c, bo - lv[i]));
+                        s[0][e] = p;
+                        dp[0][e] = p * (dp[0][e] - dl[i]);
+                    }
+                }
+                acc_product<T, DP, 1>(dv, s, ot, t, lane);
+                acc_product<T, DP, 1>(dk, dp, qt, t, lane);
+            }
+        }
+    }
+    if (a.nsplit == 1) {
+        store_rows<T, DP>(a.dk + krow * a.sdk.rs + (long)kvh * a.sdk.hs, live, dk, a.scale, a.D, h2);
+        store_rows<T, DP>(a.dv + krow * a.sdv.rs + (long)kvh * a.sdv.hs, live, dv, 1.f, a.D, h2);
+    } else {
+        float* p = a.part + ((((long)ti * a.hkv + kvh) * a.nsplit + split) * 2 * TILE + wave * WR + r) * DP;
+        store_rows<float, DP>((char*)p, true, dk, a.scale, DP, h2);
+        store_rows<float, DP>((char*)(p + (long)TILE * DP), true, dv, 1.f, DP, h2);
+    }
+}
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(PAttnArgs a) {
+    const int kvh = blockIdx.x % a.hkv, ti = blockIdx.x / a.hkv, seq = a.tiles[2 * ti], kt0 = a.tiles[2 * ti + 1];
+    const int rows = min(TILE, a.k_cap[seq] - kt0);
+    const float* p = a.part + ((long)ti * a.hkv + kvh) * a.nsplit * 2 * TILE * DP;
+    for (int i = threadIdx.x; i < 2 * rows * (DP / 8); i += 256) {
+        const int which = i >= rows * (DP / 8), j = i - which * rows * (DP / 8), row = j / (DP / 8), d = (j % (DP / 8)) * 8;
+        if (d >= a.D) continue;
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < a.nsplit; ++x) {
+            float y[8];
+            load8<float>(p + ((long)(x * 2 + which) * TILE + row) * DP + d, y);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s[k] += y[k];
+        }
+        const Strides st = which ? a.sdv : a.sdk;
+        store8<T>((T*)((which ? a.dv : a.dk) + ((long)a.k_start[seq] + kt0 + row) * st.rs + (long)kvh * st.hs) + d, s);
+    }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------------------------------
+// more than 64 KB of LDS has to be asked for (on the current device)
+int ask_lds(const void* kernel, int bytes) {
+    return bytes > 65536 && hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess;
+}
+
+struct Plan {                   // the host array of pseld_hip.h
+    long seqs, rows, max_q, k_rows, max_k, q_tiles, k_tiles;
+    const int *q_start, *q_len, *k_start, *k_cap, *k_len, *q_tile, *q_tile_causal, *k_tile, *k_tile_causal;
+};
+Plan plan_of(const long* p) {
+    Plan x;
+    x.seqs = p[0]; x.rows = p[1]; x.max_q = p[2]; x.k_rows = p[3]; x.max_k = p[4]; x.q_tiles = p[5]; x.k_tiles = p[6];
+    const int** a[] = {&x.q_start, &x.q_len, &x.k_start, &x.k_cap, &x.k_len, &x.q_tile, &x.q_tile_causal, &x.k_tile, &x.k_tile_causal};
+    for (int i = 0; i < 9; ++i) *a[i] = (const int*)p[7 + i];
+    return x;
+}
+int pad_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+constexpr int LDS_MAX = 160 * 1024;
+constexpr int FEW_TABLE = 4096;          // table entries of one key head's group that the few-rows kernel keeps in LDS
+
+// The few-rows kernel takes the call when one key head's query rows of every recording fit its 32-row operand.
+bool few_rows(const Plan& p, int hq, int hkv, int buckets) { return p.max_q * (hq / hkv) <= WR && (long)buckets * (hq / hkv) <= FEW_TABLE; }
+// keys per workgroup: about four workgroups per CU, whole rounds of the four waves' blocks; a recording of up to 512 keys stays whole (one
+// launch instead of two)
+int few_chunk(const Plan& p, int hkv) {
+    if (p.max_k <= 512) return 512;
+    const long want = (p.k_rows * hkv + 1023) / 1024;
+    const long c = (want + 127) / 128 * 128;
+    return (int)(c < 256 ? 256 : c > 8192 ? 8192 : c);
+}
+int few_splits(const Plan& p, int hkv) { const int c = few_chunk(p, hkv); return p.max_k > c ? (int)((p.max_k + c - 1) / c) : 1; }
+// workgroups that share a key tile's stream of queries: enough for two workgroups per CU, no more than the longest stream has tiles
+int dkv_splits(const Plan& p, int hq, int hkv) {
+    const long wgs = p.k_tiles * hkv, longest = (p.max_q + KT - 1) / KT * (hq / hkv);
+    if (wgs == 0 || wgs >= 512) return 1;
+    long n = (512 + wgs - 1) / wgs;
+    if (n > longest / 2) n = longest / 2;
+    return n < 1 ? 1 : n > 32 ? 32 : (int)n;
+}
+bool delta_pass(int dtype, bool table_grad) { return table_grad && dtype == PSELD_BF16; }
+
+int check(const char* name, int dtype, const Plan& p, int hq, int hkv, int D, float scale, const float* table, const int* lut, int buckets, int maxd) {
+    PSELD_CHECK_ARG(dtype == PSELD_F32 || dtype == PSELD_BF16, "%s: unknown dtype", name);
+    PSELD_CHECK_ARG(p.seqs > 0 && p.rows >= 0 && p.k_rows >= 0 && p.max_q >= 0 && p.max_k >= 0 && p.q_start && p.q_len && p.k_start && p.k_cap && p.k_len, "%s: bad plan", name);
+    PSELD_CHECK_ARG(hkv > 0 && hq >= hkv && hq % hkv == 0 && hq <= 1024, "%s: query heads must be a multiple of the key heads, at most 1024", name);
+    PSELD_CHECK_ARG(D > 0 && D % 8 == 0 && D <= 128, "%s: head sizes are multiples of 8 up to 128", name);
+    PSELD_CHECK_ARG(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", name);
+    PSELD_CHECK_ARG(!table || (lut && buckets > 0 && buckets <= 512 && maxd > 0 && maxd <= 1024), "%s: position buckets: at most 512 over distances of at most 1024", name);
+    return PSELD_OK;
+}
+int check_operand(const char* name, const char* what, int dtype, const void* ptr, const long* st, Strides& out, bool needed) {
+    const int e = dtype == PSELD_BF16 ? 2 : 4;
+    PSELD_CHECK_ARG(!needed || ptr, "%s: null pointer (%s)", name, what);
+    PSELD_CHECK_ARG(((uintptr_t)ptr & 15) == 0 && st[0] * e % 16 == 0 && st[1] * e % 16 == 0, "%s: %s: address, row and head strides must be whole 16-byte pieces", name, what);
+    PSELD_CHECK_ARG(st[0] >= 0 && st[0] < (1l << 23) && st[1] >= 0, "%s: %s: row stride out of range", name, what);
+    out.rs = st[0] * e;
+    out.hs = st[1] * e;
+    return PSELD_OK;
+}
+
+#define PA_TRY(x) do { const int rc__ = (x); if (rc__) return rc__; } while (0)
+#define PA_LAUNCH(kernel, grid, block, lds, ...)                                                                             \
+    do {                                                                                                                     \
+        const long g__ = (grid);                                                                                             \
+        if (g__ > 0) {                                                                                                       \
+            PSELD_CHECK_ARG(g__ < (1l << 31), "packed_attn: too many tiles x heads for one launch");                         \
+            if (ask_lds((const void*)&kernel, (lds))) { pseld_set_error("packed_attn: cannot reserve LDS"); return PSELD_ERR_HIP; }       \
+            hipLaunchKernelGGL(kernel, dim3((unsigned)g__), dim3(block), (lds), s, __VA_ARGS__);                             \
+        }                                                                                                                    \
+    } while (0)
+
+int dist_bytes(const PAttnArgs& a) { return a.table ? (2 * (a.maxd + NEAR_PAD) + 1) * 4 : 0; }
+
+template <typename T, int DP, bool BIAS>
+int run_fwd(PAttnArgs& a, const Plan& p, hipStream_t s) {
+    constexpr int TB = KT * DP * (int)sizeof(T);
+    if (few_rows(p, a.hq, a.hkv, BIAS ? a.buckets : 0)) {
+        constexpr int NW = DP * sizeof(T) > 256 ? 2 : 4;
+        const int G = a.hq / a.hkv;
+        a.chunk = few_chunk(p, a.hkv);
+        a.nsplit = few_splits(p, a.hkv);
+        a.max_rows = (int)p.max_q * G;
+        const int lds = NW * 4 * WR * DP * (int)sizeof(T) + (NW + 1) * 256 + (BIAS ? a.buckets * G * 4 + (2 * a.maxd + 1) * 2 : 0);
+        PA_LAUNCH((packed_attn_few_kernel<T, DP, NW, BIAS>), p.seqs * a.nsplit * a.hkv, 64 * NW, lds, a);
+        if (a.nsplit > 1) PA_LAUNCH((packed_attn_join_kernel<T>), p.seqs * a.hkv * a.max_rows, 64, a.nsplit * 4, a);
+        return PSELD_OK;
+    }
+    a.tiles = a.causal ? p.q_tile_causal : p.q_tile;
+    PA_LAUNCH((packed_attn_fwd_kernel<T, DP, BIAS>), p.q_tiles * a.hq, 256, 4 * TB + dist_bytes(a), a);
+    return PSELD_OK;
+}
+template <typename T, int DP, bool BIAS>
+int run_bwd(PAttnArgs& a, const Plan& p, float* dtable, int accumulate, hipStream_t s) {
+    constexpr int TB = KT * DP * (int)sizeof(T);
+    const int nd = dist_bytes(a);
+    a.tiles = a.causal ? p.q_tile_causal : p.q_tile;
+    if constexpr (BIAS && sizeof(T) == 2) {
+        if (dtable) PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DELTA>), p.q_tiles * a.hq, 256, 4 * TB + nd, a);
+    }
+    if (!delta_pass(sizeof(T) == 2 ? PSELD_BF16 : PSELD_F32, BIAS && dtable)) PA_LAUNCH((packed_attn_delta_kernel<T>), (p.rows * a.hq + 15) / 16, 256, 0, a, p.rows * a.hq);
+    bool table_done = false;
+    if constexpr (BIAS) {
+        if (dtable) {
+            float* part = a.part;
+            PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ_TABLE>), p.q_tiles * a.hq, 256, (dq_buffers<T, DP, DQ_TABLE>()) * 2 * TB + 9 * nd + 64, a);
+            PA_LAUNCH(packed_attn_table_kernel, (long)a.hq * ((a.buckets + 15) / 16), 256, 0, part, dtable, (int)p.q_tiles, a.hq, a.buckets, accumulate);
+            a.part += p.q_tiles * a.hq * a.buckets;
+            a.part = (float*)(((uintptr_t)a.part + 15) & ~(uintptr_t)15);
+            table_done = true;
+        }
+    }
+    if (!table_done) PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ>), p.q_tiles * a.hq, 256, 4 * TB + nd, a);
+    a.tiles = a.causal ? p.k_tile_causal : p.k_tile;
+    a.nsplit = dkv_splits(p, a.hq, a.hkv);
+    PA_LAUNCH((packed_attn_dkv_kernel<T, DP, BIAS>), p.k_tiles * a.hkv * a.nsplit, 256, 4 * TB + 4 * KT * 4 + nd, a);
+    if (a.nsplit > 1) PA_LAUNCH((packed_attn_dkv_join_kernel<T, DP>), p.k_tiles * a.hkv, 256, 0, a);
+    return PSELD_OK;
+}
+template <typename T, typename F> int by_head_size(int D, bool bias, F&& f) {
+    if (D <= 32) return bias ? f(std::integral_constant<int, 32>{}, std::true_type{}) : f(std::integral_constant<int, 32>{}, std::false_type{});
+    if (D <= 64) return bias ? f(std::integral_constant<int, 64>{}, std::true_type{}) : f(std::integral_constant<int, 64>{}, std::false_type{});
+    return bias ? f(std::integral_constant<int, 128>{}, std::true_type{}) : f(std::integral_constant<int, 128>{}, std::false_type{});
+}
+void fill(PAttnArgs& a, const Plan& p, int hq, int hkv, int D, int causal, float scale, const float* table, const int* lut, int buckets, int maxd) {
+    a.q_start = p.q_start; a.q_len = p.q_len; a.k_start = p.k_start; a.k_cap = p.k_cap; a.k_len = p.k_len;
+    a.seqs = (int)p.seqs; a.hq = hq; a.hkv = hkv; a.D = D; a.causal = causal; a.nsplit = 1;
+    a.scale = scale; a.c = scale * LOG2E;
+    a.table = table; a.lut = lut; a.buckets = table ? buckets : 0; a.maxd = table ? maxd : 0;
+    a.ranges = lut ? lut + 2 * maxd + 1 : nullptr;
+}
+
+}  // namespace
+
+extern "C" long pseld_packed_attn_fwd_workspace(const long* plan, int hq, int hkv, int D, int buckets) {
+    if (!plan || hkv <= 0 || hq < hkv || hq % hkv) return 0;
+    const Plan p = plan_of(plan);
+    if (!few_rows(p, hq, hkv, buckets)) return 0;
+    const long n = few_splits(p, hkv);
+    return n > 1 ? p.seqs * hkv * n * p.max_q * (hq / hkv) * (D + 4) * (long)sizeof(float) : 0;
+}
+
+extern "C" int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const long* strides,
+                                     const long* plan, int hq, int hkv, int D, int causal, float scale, const float* table, const int* lut,
+                                     int buckets, int max_distance, float* workspace, long workspace_bytes, void* stream) {
+    PSELD_CHECK_ARG(plan && strides, "packed_attn_fwd: null pointer");
+    const Plan p = plan_of(plan);
+    PA_TRY(check("packed_attn_fwd", dtype, p, hq, hkv, D, scale, table, lut, buckets, max_distance));
+    PAttnArgs a{};
+    const bool rows = p.rows > 0, keys = rows && p.k_rows > 0;
+    PA_TRY(check_operand("packed_attn_fwd", "q", dtype, q, strides, a.sq, rows));
+    PA_TRY(check_operand("packed_attn_fwd", "k", dtype, k, strides + 2, a.sk, keys));
+    PA_TRY(check_operand("packed_attn_fwd", "v", dtype, v, strides + 4, a.sv, keys));
+    PA_TRY(check_operand("packed_attn_fwd", "out", dtype, out, strides + 6, a.so, rows));
+    PSELD_CHECK_ARG(!rows || lse, "packed_attn_fwd: null pointer (lse)");
+    const long need = pseld_packed_attn_fwd_workspace(plan, hq, hkv, D, table ? buckets : 0);
+    PSELD_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "packed_attn_fwd: workspace too small");
+    if (!rows) return PSELD_OK;
+    a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.out = (char*)out; a.lse = lse; a.part = workspace;
+    fill(a, p, hq, hkv, D, causal, scale, table, lut, buckets, max_distance);
+    const hipStream_t s = (hipStream_t)stream;
+    const int rc = dtype == PSELD_BF16
+        ? by_head_size<bf16_t>(D, table, [&](auto dp, auto bias) { return run_fwd<bf16_t, decltype(dp)::value, decltype(bias)::value>(a, p, s); })
+        : by_head_size<float>(D, table, [&](auto dp, auto bias) { return run_fwd<float, decltype(dp)::value, decltype(bias)::value>(a, p, s); });
+    if (rc) return rc;
+    PSELD_LAUNCH_CHECK("packed_attn_fwd");
+    return PSELD_OK;
+}
+
+extern "C" long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int buckets) {
+    if (!plan || hkv <= 0 || hq < hkv || hq % hkv) return 0;
+    const Plan p = plan_of(plan);
+    const long n = dkv_splits(p, hq, hkv);
+    return ((p.rows * hq + 3) / 4 * 4 + p.q_tiles * hq * buckets + 4 + (n > 1 ? p.k_tiles * hkv * n * 2 * TILE * pad_of(D) : 0)) * (long)sizeof(float);
+}
+
+extern "C" int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                                     void* dq, void* dk, void* dv, const long* strides, const long* plan, int hq, int hkv, int D, int causal, float scale,
+                                     const float* table, const int* lut, int buckets, int max_distance, float* dtable, int accumulate,
+                                     float* workspace, long workspace_bytes, void* stream) {
+    PSELD_CHECK_ARG(plan && strides, "packed_attn_bwd: null pointer");
+    const Plan p = plan_of(plan);
+    PA_TRY(check("packed_attn_bwd", dtype, p, hq, hkv, D, scale, table, lut, buckets, max_distance));
+    PSELD_CHECK_ARG(!dtable || table, "packed_attn_bwd: a table gradient needs the table");
+    PAttnArgs a{};
+    const bool rows = p.rows > 0, keys = p.k_rows > 0;
+    const char* n = "packed_attn_bwd";
+    PA_TRY(check_operand(n, "dout", dtype, dout, strides, a.sdo, rows));
+    PA_TRY(check_operand(n, "q", dtype, q, strides + 2, a.sq, rows));
+    PA_TRY(check_operand(n, "k", dtype, k, strides + 4, a.sk, keys));
+    PA_TRY(check_operand(n, "v", dtype, v, strides + 6, a.sv, keys));
+    PA_TRY(check_operand(n, "out", dtype, out, strides + 8, a.so, rows));
+    PA_TRY(check_operand(n, "dq", dtype, dq, strides + 10, a.sdq, rows));
+    PA_TRY(check_operand(n, "dk", dtype, dk, strides + 12, a.sdk, keys));
+    PA_TRY(check_operand(n, "dv", dtype, dv, strides + 14, a.sdv, keys));
+    PSELD_CHECK_ARG(!rows || lse, "packed_attn_bwd: null pointer (lse)");
+    const long need = pseld_packed_attn_bwd_workspace(plan, hq, hkv, D, dtable ? buckets : 0);
+    PSELD_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, "packed_attn_bwd: workspace too small");
+    a.dout = (const char*)dout; a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (const char*)out; a.lse = const_cast<float*>(lse);
+    a.dq = (char*)dq; a.dk = (char*)dk; a.dv = (char*)dv;
+    a.delta = workspace;
+    a.part = workspace + (p.rows * hq + 3) / 4 * 4;
+    fill(a, p, hq, hkv, D, causal, scale, table, lut, buckets, max_distance);
+    const hipStream_t s = (hipStream_t)stream;
+    const int rc = dtype == PSELD_BF16
+        ? by_head_size<bf16_t>(D, table, [&](auto dp, auto bias) { return run_bwd<bf16_t, decltype(dp)::value, decltype(bias)::value>(a, p, dtable, accumulate, s); })
+        : by_head_size<float>(D, table, [&](auto dp, auto bias) { return run_bwd<float, decltype(dp)::value, decltype(bias)::value>(a, p, dtable, accumulate, s); });
+    if (rc) return rc;
+    PSELD_LAUNCH_CHECK("packed_attn_bwd");
+    return PSELD_OK;
+}

@@ -1624,6 +1624,9 @@ class PackedPlan:
         self._ints = torch.tensor(host, dtype=torch.int32).to(self.device)
         self._ptr = {k: self._ints.data_ptr() + 4 * v for k, v in at.items()}
         self.k_len = self._ints[at['k_len']:at['k_len'] + self.seqs]
+        names = ('q_start', 'q_len', 'k_start', 'k_cap', 'k_len', 'q_tile', 'q_tile_causal', 'k_tile', 'k_tile_causal')
+        self._desc = (ctypes.c_long * 16)(self.seqs, self.rows, self.max_q, self.k_rows, self.max_k, self.q_tiles, self.k_tiles,
+                                          *(self._ptr[k] for k in names))
 
 
 _PACKED_TILE = 128
@@ -1701,3 +1704,135 @@ def linrec_bwd(dh, g, n, saved, plan, dh_last=None, h0=None, reverse=False, dg=N
                             plan._ptr['q_len'], plan.seqs, plan.rows, plan.max_q, C, int(bool(reverse)), _lib.ptr(ws), nbytes, _lib.stream_ptr())
     _lib.check(rc, "pseld_linrec_bwd")
     return dg, dn, dh0
+
+
+class RelposBuckets:
+    """Buckets of relative positions (key - query) for a learned bias table [num_buckets, heads]. Bidirectional: half the buckets for keys behind
+    the query and the query itself, half for keys ahead; otherwise all of them for keys behind and bucket 0 for every key ahead. The first
+    half of a side's n buckets hold one distance each; bucket e + k (e = n // 2, K = n - e) starts where
+    floor(K log(distance / e) / log(max_distance / e)) reaches k, the last one runs on without end. The borders are found in whole numbers:
+    distance^K e^k >= max_distance^k e^K."""
+
+    def __init__(self, num_buckets, max_distance, bidirectional, device):
+        side = num_buckets // 2 if bidirectional else num_buckets
+        e = side // 2
+        if side < 2 or (bidirectional and num_buckets % 2) or num_buckets > 512:
+            raise _lib.PseldError("relpos_buckets: 2 to 512 buckets, an even number (at least 4) for both directions")
+        if not e < max_distance <= 1024:
+            raise _lib.PseldError(f"relpos_buckets: max_distance must lie above the {e} one-distance buckets of a side and be at most 1024")
+        K = side - e
+        of_dist, k = [], 0
+        for n in range(max_distance + 1):
+            if n < e:
+                of_dist.append(n)
+                continue
+            while k + 1 < K and n ** K * e ** (k + 1) >= max_distance ** (k + 1) * e ** K:
+                k += 1
+            of_dist.append(e + k)
+        lut = [of_dist[-r] if r <= 0 else side + of_dist[r] if bidirectional else 0 for r in range(-max_distance, max_distance + 1)]
+        first, last = {}, {}
+        for r, b in zip(range(-max_distance, max_distance + 1), lut):
+            first.setdefault(b, r)
+            last[b] = r
+        ranges = [x for b in range(num_buckets) for x in (first.get(b, 1), last.get(b, 0))]
+        self.num_buckets, self.max_distance, self.bidirectional = num_buckets, max_distance, bidirectional
+        self.host_lut = lut
+        self.device = torch.device(device)
+        if self.device.type == 'cuda':
+            if self.device.index is None:
+                self.device = torch.device('cuda', torch.cuda.current_device())
+            self._ints = torch.tensor(lut + ranges, dtype=torch.int32).to(self.device)
+
+
+def relpos_buckets(num_buckets=32, max_distance=128, bidirectional=True, device='cuda'):
+    """The buckets of a learned relative position bias (see RelposBuckets); make them once, outside captured graphs."""
+    return RelposBuckets(num_buckets, max_distance, bidirectional, device)
+
+
+def _heads_ok(what, plan, dtype, named, rows):
+    """[rows, heads, D] operands on the plan's device: one type, unit stride inside a head."""
+    for name, t in named:
+        if t.device != plan.device:
+            raise _lib.PseldError(f"{what}: {name} must live on the plan's device {plan.device}, it is on {t.device}")
+        if t.dtype != dtype:
+            raise _lib.PseldError(f"{what}: operands must share one dtype ({name} is {t.dtype}, not {dtype})")
+        if t.dim() != 3 or t.shape[0] != rows or t.stride(2) != 1:
+            raise _lib.PseldError(f"{what}: {name} must be [rows = {rows}, heads, head size] with unit stride inside a head, it is {tuple(t.shape)} "
+                                  f"with strides {t.stride()}")
+
+
+def _packed_attn_args(what, plan, q, k, v, scale, bias_table, buckets):
+    if plan.device.index != torch.cuda.current_device():
+        raise _lib.PseldError(f"{what}: the plan lives on {plan.device}, the current device is cuda:{torch.cuda.current_device()}")
+    _heads_ok(what, plan, q.dtype, (('q', q),), plan.rows)
+    _heads_ok(what, plan, q.dtype, (('k', k), ('v', v)), plan.k_rows)
+    hq, D, hkv = q.shape[1], q.shape[2], k.shape[1]
+    if k.shape[2] != D or v.shape != k.shape:
+        raise _lib.PseldError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} must have one head size, k and v one shape")
+    if (bias_table is None) != (buckets is None):
+        raise _lib.PseldError(f"{what}: bias_table and buckets come together")
+    if buckets is not None:
+        if buckets.device != plan.device or bias_table.device != plan.device or bias_table.dtype != torch.float32 or not bias_table.is_contiguous() or \
+                tuple(bias_table.shape) != (buckets.num_buckets, hq):
+            raise _lib.PseldError(f"{what}: bias_table must be contiguous float32 [buckets = {buckets.num_buckets}, query heads = {hq}] on {plan.device}")
+    return hq, hkv, D, float(scale) if scale is not None else D ** -0.5
+
+
+def _table_args(bias_table, buckets):
+    return (bias_table.data_ptr(), buckets._ints.data_ptr(), buckets.num_buckets, buckets.max_distance) if buckets is not None else (None, None, 0, 0)
+
+
+def _head_strides(*ts):
+    return (ctypes.c_long * (2 * len(ts)))(*[s for t in ts for s in t.stride()[:2]])
+
+
+def packed_attn_fwd(q, k, v, plan, causal=False, scale=None, bias_table=None, buckets=None, out=None):
+    """Attention of every recording of the plan: q [rows, query heads, D], k, v [key rows, key heads, D] (views of a projection's output or
+    of a cache allowed; query heads a multiple of key heads) -> (out [rows, query heads, D], lse f32 [rows, query heads]). Query i of a recording
+    stands at position i + k_len - q_len; causal masks the keys behind a query's position. A row without keys gives 0 and -inf. scale: D^-1/2 where None.
+    bias_table f32 [buckets, query heads] with buckets = relpos_buckets(...): bias_table[bucket(key position - query position), head]
+    is added to the scaled scores. Key rows past a recording's k_len are never read."""
+    hq, hkv, D, scale = _packed_attn_args("packed_attn_fwd", plan, q, k, v, scale, bias_table, buckets)
+    L = _lib.lib()
+    if out is None:
+        out = torch.empty((plan.rows, hq, D), dtype=q.dtype, device=q.device)
+    else:
+        _heads_ok("packed_attn_fwd", plan, q.dtype, (('out', out),), plan.rows)
+        if out.shape != q.shape:
+            raise _lib.PseldError("packed_attn_fwd: out must have q's shape")
+    lse = torch.empty((plan.rows, hq), dtype=torch.float32, device=q.device)
+    table, lut, nb, md = _table_args(bias_table, buckets)
+    nbytes = L.pseld_packed_attn_fwd_workspace(plan._desc, hq, hkv, D, nb) if hkv and hq % hkv == 0 else 0
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None      # its own per call: nothing shared between streams
+    rc = L.pseld_packed_attn_fwd(dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _head_strides(q, k, v, out),
+                                 plan._desc, hq, hkv, D, int(bool(causal)), scale, table, lut, nb, md, _lib.ptr(ws), nbytes, _lib.stream_ptr())
+    _lib.check(rc, "pseld_packed_attn_fwd")
+    return out, lse
+
+
+def packed_attn_bwd(dout, q, k, v, out, lse, plan, causal=False, scale=None, bias_table=None, buckets=None, dbias_table=None, accumulate=False,
+                    dq=None, dk=None, dv=None):
+    """Gradients of packed_attn_fwd (same plan, lengths and options; out and lse are what it returned): (dq, dk, dv). dbias_table f32 [buckets, query heads]:
+    written (accumulate: added to) where given. dq, dk, dv: optional outputs (e.g. the parts of the projection's gradient)."""
+    hq, hkv, D, scale = _packed_attn_args("packed_attn_bwd", plan, q, k, v, scale, bias_table, buckets)
+    dq = torch.empty((plan.rows, hq, D), dtype=q.dtype, device=q.device) if dq is None else dq
+    dk = torch.empty((plan.k_rows, hkv, D), dtype=q.dtype, device=q.device) if dk is None else dk
+    dv = torch.empty((plan.k_rows, hkv, D), dtype=q.dtype, device=q.device) if dv is None else dv
+    _heads_ok("packed_attn_bwd", plan, q.dtype, (('dout', dout), ('out', out), ('dq', dq)), plan.rows)
+    _heads_ok("packed_attn_bwd", plan, q.dtype, (('dk', dk), ('dv', dv)), plan.k_rows)
+    if not (dout.shape == out.shape == dq.shape == q.shape and dk.shape == dv.shape == k.shape):
+        raise _lib.PseldError("packed_attn_bwd: dout, out and dq must have q's shape, dk and dv k's")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (plan.rows, hq) or not lse.is_contiguous() or lse.device != plan.device:
+        raise _lib.PseldError("packed_attn_bwd: lse must be what packed_attn_fwd returned")
+    if dbias_table is not None and (buckets is None or dbias_table.dtype != torch.float32 or dbias_table.shape != bias_table.shape or
+                                    not dbias_table.is_contiguous() or dbias_table.device != plan.device):
+        raise _lib.PseldError("packed_attn_bwd: dbias_table must be contiguous float32 of bias_table's shape, beside bias_table and buckets")
+    L = _lib.lib()
+    table, lut, nb, md = _table_args(bias_table, buckets)
+    nbytes = L.pseld_packed_attn_bwd_workspace(plan._desc, hq, hkv, D, nb if dbias_table is not None else 0) if hkv and hq % hkv == 0 else 0
+    ws = torch.empty((nbytes + 15) // 16 * 4, dtype=torch.float32, device=q.device)
+    rc = L.pseld_packed_attn_bwd(dtype_code(q), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+                                 dk.data_ptr(), dv.data_ptr(), _head_strides(dout, q, k, v, out, dq, dk, dv), plan._desc, hq, hkv, D, int(bool(causal)),
+                                 scale, table, lut, nb, md, _lib.ptr(dbias_table), int(bool(accumulate)), _lib.ptr(ws), nbytes, _lib.stream_ptr())
+    _lib.check(rc, "pseld_packed_attn_bwd")
+    return dq, dk, dv
