@@ -510,8 +510,8 @@ int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void* g, long l
  *   S = scale q k^T + table[bucket(key position - query position), head], P = softmax over the keys that the mask leaves, out = P v,
  *   lse[row, head] = log sum exp S;  a row without keys: out 0, lse -inf. Query i of a recording stands at position i + k_len - q_len; causal: keys
  *   behind a query's position are masked. |table| is taken to be below 1e37.
- * plan: HOST array of 16 longs {seqs, rows, max_q, k_rows, max_k, q_tiles, k_tiles, then device int arrays as addresses: q_start[seqs],
- * q_len[seqs], k_start[seqs], k_cap[seqs], k_len[seqs], q_tile[q_tiles][2], q_tile_causal, k_tile[k_tiles][2], k_tile_causal}: a tile is
+ * plan: HOST array of 18 longs {seqs, rows, max_q, k_rows, max_k, q_tiles, k_tiles, the 64-query tiles that the key tiles meet, summed: full and
+ * causal, then device int arrays as addresses: q_start[seqs], q_len[seqs], k_start[seqs], k_cap[seqs], k_len[seqs], q_tile[q_tiles][2], q_tile_causal, k_tile[k_tiles][2], k_tile_causal}: a tile is
  * (recording, first row) of 128 rows of queries or of capacity, heaviest first. k_len may change between calls; it is held to 0 .. k_cap.
  * strides: HOST array of longs, {row stride, head stride} in elements of q, k, v, out (bwd: dout, q, k, v, out, dq, dk, dv), whole
  * 16-byte pieces; unit stride inside a head. table f32 [buckets, hq] or NULL; lut (device ints): the bucket of every distance
@@ -523,7 +523,7 @@ long pseld_packed_attn_fwd_workspace(const long* plan, int hq, int hkv, int D, i
 int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const long* strides,
                           const long* plan, int hq, int hkv, int D, int causal, float scale, const float* table, const int* lut,
                           int buckets, int max_distance, float* workspace, long workspace_bytes, void* stream);
-long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int buckets);
+long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int causal, int buckets);
 int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
                           void* dq, void* dk, void* dv, const long* strides, const long* plan, int hq, int hkv, int D, int causal, float scale,
                           const float* table, const int* lut, int buckets, int max_distance, float* dtable, int accumulate,

@@ -39,12 +39,13 @@ struct PAttnArgs {
     float* lse;                 // [rows, hq]
     float* delta;               // [rows, hq]
     const int *q_start, *q_len, *k_start, *k_cap, *k_len, *tiles;
-    int seqs, hq, hkv, D, causal, nsplit;
+    int seqs, hq, hkv, D, causal;
+    int nsplit, chunk;          // parts of a recording's keys and keys per part (few rows); of a key tile's query tiles and tiles per part (dk, dv)
     float scale, c;             // c = scale * log2(e)
     const float* table; const int* lut; const int* ranges;      // [buckets, hq]; bucket of distance -max .. max; [buckets, 2] first and last distance
     int buckets, maxd;
-    float* part;                // dtable: [tiles, hq, buckets]; split dk/dv: [nsplit, 2, rows of the tiles' list, D]; few rows: see there
-    int chunk, max_rows;        // few rows: keys per workgroup, rows reserved per key head
+    float* part;                // dtable: [tiles, hq, buckets]; split dk/dv: [tiles, hkv, nsplit, 2, TILE, DP]; few rows: see there
+    int max_rows;               // few rows: rows reserved per key head
 };
 
 // Two waves per SIMD where 256 registers hold a wave's accumulators and operands: the compiler then keeps the accumulators in vector registers
@@ -57,41 +58,67 @@ template <int RB> __device__ __forceinline__ int image_swizzle(int row) {
     else if constexpr (RB == 128) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
     else return (row & 7) << 1;
 }
+typedef __attribute__((address_space(3))) const char* lds_cptr;
+// A lane's reads of an image. The swizzle only XORs bits inside a row, so a lane keeps three offsets for the tile at hand and reaches every piece by
+// XOR with a constant and the instruction's immediate. at() hides the offsets from loop-invariant motion: hoisted, the dozens of
+// XORed addresses cost more registers than recomputing them per tile costs time (the dk/dv kernel for 128 spilled 60 registers).
 template <typename T, int DP> struct Image {
     static constexpr int RB = DP * (int)sizeof(T);
     using M = AMma<T>;
     using Frag = typename M::Frag;
-    // 8 consecutive elements 16 kk + 8 h2 .. of one row
-    static __device__ __forceinline__ Frag row_frag(const char* base, int row, int kk, int h2) {
-        const int f = image_swizzle<RB>(row);
-        if constexpr (sizeof(T) == 2) return *(const bf16x8*)(base + row * RB + (((2 * kk + h2) ^ f) << 4));
+    struct Lane { unsigned row, lo, hi; };
+    static __device__ __forceinline__ Lane lane_offsets(int lane) {
+        const int r = lane & 31, h2 = lane >> 5;
+        Lane l;
+        if constexpr (sizeof(T) == 2) {
+            const int ra = 4 * h2 + ((lane & 15) >> 2), rb = ra + 8, p = lane & 3, ch = 2 * ((lane >> 4) & 1) + (p >> 1);
+            l.row = r * RB + ((h2 ^ image_swizzle<RB>(r)) << 4);
+            l.lo = ra * RB + ((ch ^ image_swizzle<RB>(ra)) << 4) + (p & 1) * 8;
+            l.hi = rb * RB + ((ch ^ image_swizzle<RB>(rb)) << 4) + (p & 1) * 8;
+        } else {
+            l.row = r * RB + (((2 * h2) ^ image_swizzle<RB>(r)) << 4);
+            l.lo = l.hi = 0;
+        }
+        return l;
+    }
+    static __device__ __forceinline__ void move(Lane& l, unsigned by) {
+        l.row += by;
+        l.lo += by;
+        asm volatile("" : "+v"(l.row));
+        if constexpr (sizeof(T) == 2) {
+            l.hi += by;
+            asm volatile("" : "+v"(l.lo), "+v"(l.hi));
+        }
+    }
+    static __device__ __forceinline__ Lane at(Lane l, unsigned tile) { move(l, tile); return l; }
+    // elements 16 kk + 8 h2 .. + 7 of image row 32 t + (lane & 31); off: bytes from the tile that l stands for (a multiple of 1024)
+    static __device__ __forceinline__ Frag row_frag(const Lane& l, int t, int kk, int off = 0) {
+        if constexpr (sizeof(T) == 2) return *(const __attribute__((address_space(3))) bf16x8*)(lds_cptr)(uintptr_t)((l.row ^ (kk << 5)) + t * 32 * RB + off);
         else {
-            const f32x4 a = *(const f32x4*)(base + row * RB + (((4 * kk + 2 * h2) ^ f) << 4));
-            const f32x4 b = *(const f32x4*)(base + row * RB + (((4 * kk + 2 * h2 + 1) ^ f) << 4));
+            const f32x4 a = *(const __attribute__((address_space(3))) f32x4*)(lds_cptr)(uintptr_t)((l.row ^ (kk << 6)) + t * 32 * RB + off);
+            const f32x4 b = *(const __attribute__((address_space(3))) f32x4*)(lds_cptr)(uintptr_t)((l.row ^ (kk << 6) ^ 16) + t * 32 * RB + off);
             Frag x;
 #pragma unroll
             for (int j = 0; j < 4; ++j) { x.v[j] = a[j]; x.v[4 + j] = b[j]; }
             return x;
         }
     }
-    // element j = M[row0 + 8 (j >> 2) + 4 h2 + (j & 3)][col0 + (lane & 31)], the k order of an accumulator operand; row0 a multiple of 16
-    static __device__ __forceinline__ Frag col_frag(const char* base, int row0, int col0, int lane) {
+    // element j = M[row0 + 8 (j >> 2) + 4 h2 + (j & 3)][32 dt + (lane & 31)], the k order of an accumulator operand; row0 a multiple of 16
+    static __device__ __forceinline__ Frag col_frag(const Lane& l, int row0, int dt, int lane, int off = 0) {
         if constexpr (sizeof(T) == 2) {
-            const int i = lane & 15, qq = i >> 2, p = i & 3, gsel = (lane >> 4) & 1, h2 = lane >> 5;
-            const int ra = row0 + 4 * h2 + qq, rb = ra + 8, ch = (col0 >> 3) + 2 * gsel + (p >> 1);
-            const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(base + ra * RB + ((ch ^ image_swizzle<RB>(ra)) << 4) + (p & 1) * 8));
-            const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(base + rb * RB + ((ch ^ image_swizzle<RB>(rb)) << 4) + (p & 1) * 8));
+            const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(lds_cptr)(uintptr_t)((l.lo ^ (dt << 6)) + row0 * RB + off));
+            const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(lds_cptr)(uintptr_t)((l.hi ^ (dt << 6)) + row0 * RB + off));
             short8v s;
             s[0] = lo[0]; s[1] = lo[1]; s[2] = lo[2]; s[3] = lo[3];
             s[4] = hi[0]; s[5] = hi[1]; s[6] = hi[2]; s[7] = hi[3];
             return __builtin_bit_cast(bf16x8, s);
         } else {
-            const int col = col0 + (lane & 31), h2 = lane >> 5;
+            const int col = 32 * dt + (lane & 31), h2 = lane >> 5;
             Frag x;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int row = row0 + 8 * (j >> 2) + 4 * h2 + (j & 3);
-                x.v[j] = *(const float*)(base + row * RB + (((col >> 2) ^ image_swizzle<RB>(row)) << 4) + (col & 3) * 4);
+                x.v[j] = *(const __attribute__((address_space(3))) float*)(lds_cptr)(uintptr_t)(l.lo + row * RB + (((col >> 2) ^ image_swizzle<RB>(row)) << 4) + (col & 3) * 4 + off);
             }
             return x;
         }
@@ -138,34 +165,41 @@ __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(
         asm volatile("" ::: "memory");                                  \
     } while (0)
 
-// A stream of ROWS-row tiles of one operand into LDS by NW waves. Offsets of a whole tile are computed once; a tile that ends inside takes
-// its rows past the end from the last one.
-template <typename T, int DP, int ROWS, int NW> struct Stream {
+// A stream of ROWS-row tiles of one operand into LDS by NW waves. The swizzle repeats after NP instructions, so NP lane offsets serve a whole
+// tile and the rest is added to the uniform base. A tile that ends inside takes its rows past the end from the last one. LAZY: the offsets are
+// computed anew for every tile (where registers are short: spilled, each one's reload waits behind the DMAs already in flight).
+template <typename T, int DP, int ROWS, int NW, bool LAZY = false> struct Stream {
     static constexpr int RB = DP * (int)sizeof(T);
     static constexpr int NI = ROWS * RB / 1024 / NW;       // wave-instructions per wave
-    static_assert(NI >= 1 && NI * NW * 1024 == ROWS * RB, "whole instructions per wave");
-    unsigned voff[NI];
+    static constexpr int RPI = 1024 / RB;                  // rows per instruction
+    static constexpr int NP = RB == 64 ? 1 : RB == 512 ? 4 : 2;
+    static_assert(NI >= NP && NI % NP == 0 && NI * NW * 1024 == ROWS * RB, "whole swizzle periods per wave");
+    unsigned voff[LAZY ? 1 : NP];
     unsigned rs;
-    int wave, lane, pieces;
-    __device__ __forceinline__ unsigned at(int j, int limit) const {
-        const int lin = (wave * NI + j) * 1024 + lane * 16, row = lin / RB, pos = (lin % RB) >> 4;
-        const int piece = min(pos ^ image_swizzle<RB>(row), pieces - 1);
-        return (unsigned)min(row, limit) * rs + (unsigned)piece * 16;
+    int wave, pieces;
+    __device__ __forceinline__ unsigned offset(int lane, int row0, int limit) const {
+        const int row = row0 + lane * 16 / RB;
+        return (unsigned)min(row, limit) * rs + (unsigned)min(((lane * 16 % RB) >> 4) ^ image_swizzle<RB>(row), pieces - 1) * 16;
     }
     __device__ __forceinline__ void init(long row_bytes, int D, int w) {
-        wave = w; lane = threadIdx.x & 63; rs = (unsigned)row_bytes; pieces = D * (int)sizeof(T) / 16;
+        wave = w; rs = (unsigned)row_bytes; pieces = D * (int)sizeof(T) / 16;
+        if constexpr (!LAZY)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) voff[j] = at(j, ROWS - 1);
+            for (int j = 0; j < NP; ++j) voff[j] = offset(threadIdx.x & 63, j * RPI, ROWS);
     }
     // base: first row of the tile (uniform); rows: rows that exist from there on (> 0)
     __device__ __forceinline__ void load(const char* base, int rows, unsigned lds) const {
-        const char* b = uniform_ptr(base);
+        const unsigned dst = __builtin_amdgcn_readfirstlane(lds + wave * NI * 1024);
+        int lane = threadIdx.x & 63;
+        if constexpr (LAZY) asm volatile("" : "+v"(lane));
         if (rows >= ROWS) {
+            const char* b = uniform_ptr(base + (long)(wave * NI * RPI) * rs);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) pa_dma(__builtin_amdgcn_readfirstlane(lds + (wave * NI + j) * 1024), b, voff[j]);
+            for (int j = 0; j < NI; ++j) pa_dma(dst + j * 1024, b + (long)(j / NP * NP * RPI) * rs, LAZY ? offset(lane, j % NP * RPI, ROWS) : voff[LAZY ? 0 : j % NP]);
         } else {
+            const char* b = uniform_ptr(base);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) pa_dma(__builtin_amdgcn_readfirstlane(lds + (wave * NI + j) * 1024), b, at(j, rows - 1));
+            for (int j = 0; j < NI; ++j) pa_dma(dst + j * 1024, b, offset(lane, (wave * NI + j) * RPI, rows - 1));
         }
     }
 };
@@ -182,6 +216,10 @@ __device__ __forceinline__ void dist_fill(float* dist, const PAttnArgs& a, int h
     for (int i = threadIdx.x; i < n; i += threads) dist[i] = bias_at(a, i - a.maxd - NEAR_PAD, head);
 }
 
+// Keeps the scheduler from requesting a whole product's operands at once where the accumulators leave no registers for them
+template <bool TIGHT> __device__ __forceinline__ void pace() {
+    if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
+}
 template <int N> __device__ __forceinline__ void zero_acc(f32x16 (&z)[N]) {
 #pragma unroll
     for (int t = 0; t < N; ++t)
@@ -224,9 +262,9 @@ __device__ __forceinline__ void store_rows(char* row, bool live, const f32x16 (&
     }
 }
 
-// z (rows = d) += M[tile rows][d]^T x, x = accumulator tiles whose rows are the tile's rows t0 * 32 ..
-template <typename T, int DP, int NT>
-__device__ __forceinline__ void acc_product(f32x16 (&z)[DP / 32], const f32x16 (&x)[NT], const char* tile, int t0, int lane) {
+// z (rows = d) += M[tile rows][d]^T x, x = accumulator tiles whose rows are the image's rows 32 t0 ..
+template <typename T, int DP, int NT, bool TIGHT = false>
+__device__ __forceinline__ void acc_product(f32x16 (&z)[DP / 32], const f32x16 (&x)[NT], const typename Image<T, DP>::Lane& l, int t0, int lane, int off) {
     using I = Image<T, DP>;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -234,7 +272,8 @@ __device__ __forceinline__ void acc_product(f32x16 (&z)[DP / 32], const f32x16 (
         for (int s = 0; s < 2; ++s) {
             const typename I::Frag fx = I::M::from_acc(x[t], s);
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) I::M::mma(I::col_frag(tile, (t0 + t) * 32 + 16 * s, dt * 32, lane), fx, z[dt]);
+            for (int dt = 0; dt < DP / 32; ++dt) I::M::mma(I::col_frag(l, (t0 + t) * 32 + 16 * s, dt, lane, off), fx, z[dt]);
+            pace<TIGHT>();
         }
 }
 
@@ -332,6 +371,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
     ks.init(a.sk.rs, a.D, wave);
     vs.init(a.sv.rs, a.D, wave);
     const unsigned lds0 = lds_addr(smem);
+    const typename I::Lane im0 = I::lane_offsets(lane);
     const int nt = (w.nk + KT - 1) / KT;
     if (nt) { ks.load(kb, w.k_len, lds0); vs.load(vb, w.k_len, lds0 + TB); }
     if constexpr (BIAS) dist_fill(dist, a, w.head, 256);
@@ -350,8 +390,6 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
     Softmax<DP> sm;
     sm.init();
     for (int i = 0; i < nt; ++i) {
-        const char* kt = smem + (i & 1) * 2 * TB;
-        const char* vt = kt + TB;
         const int k0 = i * KT;
         PA_SYNC_TILE();
         if (i + 1 < nt) {
@@ -360,12 +398,13 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
             vs.load(vb + (long)(k0 + KT) * a.sv.rs, w.k_len - k0 - KT, dst + TB);
         }
         if (k0 > wlim1) continue;
+        const typename I::Lane im = I::at(im0, lds0 + (i & 1) * 2 * TB);
         f32x16 st[2];
         zero_acc(st);
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) I::M::mma(I::row_frag(kt, t * 32 + r, kk, h2), fq[kk], st[t]);
+            for (int t = 0; t < 2; ++t) I::M::mma(I::row_frag(im, t, kk), fq[kk], st[t]);
         float c = a.c, off = 0.f;
         if constexpr (BIAS) {
             const int lo = k0 - (qw0 + WR - 1), hi = k0 + KT - 1 - qw0;      // the tile's smallest and largest distance
@@ -375,7 +414,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
         }
         if (k0 + KT - 1 > wlim0) mask_rows<2>(st, klim - k0 - 4 * h2, -__builtin_inff());
         sm.template step<2>(st, c, off);
-        acc_product<T, DP, 2>(sm.ot, st, vt, 0, lane);
+        acc_product<T, DP, 2>(sm.ot, st, im, 0, lane, TB);
     }
     const float l = sm.l + __shfl_xor(sm.l, 32, 64);
     store_rows<T, DP>(a.out + qrow * a.so.rs + (long)w.head * a.so.hs, live, sm.ot, l > 0.f ? 1.f / l : 0.f, a.D, h2);
@@ -429,6 +468,7 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
     vs.init(a.sv.rs, a.D, 0);
     char* mine = smem + wave * 4 * BB;
     const unsigned lds0 = lds_addr(mine);
+    const typename I::Lane im0 = I::lane_offsets(lane);
     Softmax<DP> sm;
     sm.init();
     const int first = kbeg + wave * WR;
@@ -445,11 +485,11 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Stream<T, DP, WR, 1>::NI) : "memory");
         } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        const char* kt = mine + par * 2 * BB;
+        const typename I::Lane im = I::at(im0, lds0 + par * 2 * BB);
         f32x16 st[1];
         zero_acc(st);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) I::M::mma(I::row_frag(kt, r, kk, h2), fq[kk], st[0]);
+        for (int kk = 0; kk < DP / 16; ++kk) I::M::mma(I::row_frag(im, 0, kk), fq[kk], st[0]);
         float c = a.c, o = 0.f;
         if constexpr (BIAS) {
             const int lo = k0 - (k_len - 1), hi = min(k0 + WR, kend) - 1 - off;      // over every query of the recording
@@ -467,7 +507,7 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
         }
         if (a.causal ? k0 + WR - 1 > min(k_len - 1, off) || k0 + WR > kend : k0 + WR > kend) mask_rows<1>(st, min(klim, kend - 1) - k0 - 4 * h2, -__builtin_inff());
         sm.template step<1>(st, c, o);
-        acc_product<T, DP, 1>(sm.ot, st, kt + BB, 0, lane);
+        acc_product<T, DP, 1>(sm.ot, st, im, 0, lane, BB);
     }
     // join the waves
     const float l = sm.l + __shfl_xor(sm.l, 32, 64);
@@ -579,17 +619,50 @@ __global__ __launch_bounds__(256) void packed_attn_delta_kernel(PAttnArgs a, lon
 
 enum { DQ = 0, DQ_TABLE = 1, DELTA = 2 };
 
-// dq (and the table's gradient), tiled like the forward; DELTA: only delta = sum_j P dP
+// Adds a wave's 32 x 64 dS (lanes = queries) to its sums by distance; h points at the entry of distance (tile's first key - wave's first query). The
+// tile goes through LDS as [query][key]; in step q lane l reads key (q + l - 31) mod 64 of query q: over the 32 steps every element is read once, and what
+// a lane sees is one diagonal key - query = l - 31 while q + l >= 31 and one diagonal l + 33 before. (One LDS float atomic per element
+// instead took 67 cycles each: 200 us of the dq kernel for 12 recordings of 100-1200 frames, 16 heads of 64, where this takes 85.)
+constexpr int DIAG_PITCH = 68, DIAG = 32 * DIAG_PITCH;      // floats; 16-byte pieces of eight rows fall in different banks
+typedef __attribute__((address_space(3))) float* lds_fptr;
+typedef __attribute__((address_space(3))) f32x4* lds_f4ptr;
+__device__ __forceinline__ void add_diagonals(unsigned m, unsigned h, const f32x16 (&x)[2], int lane) {
+    const int r = lane & 31, h2 = lane >> 5;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *(lds_f4ptr)(uintptr_t)(m + (r * DIAG_PITCH + 4 * h2) * 4 + (t * 32 + 8 * g) * 4) = f32x4{x[t][4 * g], x[t][4 * g + 1], x[t][4 * g + 2], x[t][4 * g + 3]};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // a wave's LDS operations run in order; this keeps the compiler's order too
+    float all = 0.f, before = 0.f;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) {
+        const float v = *(lds_fptr)(uintptr_t)(m + (((lane + q + 33) & 63) << 2) + q * DIAG_PITCH * 4);
+        all += v;
+        if (q < 31) before += lane < 31 - q ? v : 0.f;
+        if ((q & 7) == 7) pace<true>();
+    }
+    const unsigned a = h + (lane - 31) * 4;
+    *(lds_fptr)(uintptr_t)a = *(lds_fptr)(uintptr_t)a + (all - before);
+    asm volatile("" ::: "memory");
+    if (lane < 31) *(lds_fptr)(uintptr_t)(a + 64 * 4) = *(lds_fptr)(uintptr_t)(a + 64 * 4) + before;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
 // (f32 heads of 128 with the table: two buffers and the sums for 1024 distances would not fit 160 KB, so that variant has one buffer)
 template <typename T, int DP, int MODE> constexpr int dq_buffers() { return sizeof(T) == 4 && DP == 128 && MODE == DQ_TABLE ? 1 : 2; }
+// dq (and the table's gradient), tiled like the forward; DELTA: only delta = sum_j P dP
 template <typename T, int DP, bool BIAS, int MODE>
 __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq_kernel(PAttnArgs a) {
     using I = Image<T, DP>;
     constexpr int TB = KT * I::RB, NB = dq_buffers<T, DP, MODE>();
-    extern __shared__ __attribute__((aligned(1024))) char smem[];      // NB x (K | V) | bias by distance | sums by distance, 8 copies | 8 floats
+    constexpr bool TIGHT = DP == 128;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];      // NB x (K | V) | bias by distance | then (DQ_TABLE) sums by distance, a copy per wave | 8 floats | 4 x DIAG
     float* dist = (float*)(smem + NB * 2 * TB);
     const int ndist = BIAS ? dist_count(a.maxd) : 0;
     float* hist = dist + ndist;
+    float* far = hist + 4 * ndist;
+    const unsigned diag = (lds_addr(far + 8) + 15) & ~15u;
     const QTile w = q_tile_of(a);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
     const int qi = w.q0 + wave * WR + r;
@@ -601,11 +674,12 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
     ks.init(a.sk.rs, a.D, wave);
     vs.init(a.sv.rs, a.D, wave);
     const unsigned lds0 = lds_addr(smem);
+    const typename I::Lane im0 = I::lane_offsets(lane);
     const int nt = (w.nk + KT - 1) / KT;
     if (nt) { ks.load(kb, w.k_len, lds0); vs.load(vb, w.k_len, lds0 + TB); }
     if constexpr (BIAS) dist_fill(dist, a, w.head, 256);
     if constexpr (MODE == DQ_TABLE)
-        for (int i = threadIdx.x; i < 8 * ndist; i += 256) hist[i] = 0.f;
+        for (int i = threadIdx.x; i < 4 * ndist; i += 256) hist[i] = 0.f;
     typename I::Frag fq[DP / 16], fo[DP / 16];
     {
         const char* row = a.q + qrow * a.sq.rs + (long)w.head * a.sq.hs;
@@ -627,8 +701,6 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
     f32x16 dq[DP / 32];
     zero_acc(dq);
     for (int i = 0; i < nt; ++i) {
-        const char* kt = smem + (NB == 2 ? i & 1 : 0) * 2 * TB;
-        const char* vt = kt + TB;
         const int k0 = i * KT;
         PA_SYNC_TILE();
         if (NB == 1 && i) {
@@ -642,6 +714,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
             vs.load(vb + (long)(k0 + KT) * a.sv.rs, w.k_len - k0 - KT, dst + TB);
         }
         if (k0 > wlim1) continue;
+        const typename I::Lane im = I::at(im0, lds0 + (NB == 2 ? i & 1 : 0) * 2 * TB);
         f32x16 st[2], dp[2];
         zero_acc(st);
         zero_acc(dp);
@@ -649,8 +722,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                I::M::mma(I::row_frag(kt, t * 32 + r, kk, h2), fq[kk], st[t]);
-                I::M::mma(I::row_frag(vt, t * 32 + r, kk, h2), fo[kk], dp[t]);
+                I::M::mma(I::row_frag(im, t, kk), fq[kk], st[t]);
+                I::M::mma(I::row_frag(im, t, kk, TB), fo[kk], dp[t]);
+                if (t) pace<TIGHT>();
             }
         float c = a.c, off = 0.f;
         int where = 0;                       // of the tile's distances: -1 / 1 all at or past -maxd / maxd, 0 near
@@ -673,12 +747,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
             }
         if constexpr (MODE == DQ_TABLE) {
             if (where == 0) {
-                float* hp = hist + (wave * 2 + h2) * ndist + di;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float*)(hp + t * 32 + (e & 3) + 8 * (e >> 2)), st[t][e], 0, 0, false);
+                add_diagonals(diag + wave * DIAG * 4, lds_addr(hist) + (wave * ndist + k0 - qw0 + a.maxd + NEAR_PAD) * 4, st, lane);
             } else {
                 float s = 0.f;
 #pragma unroll
@@ -688,14 +757,13 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
                 if (where < 0) sum_lo += s; else sum_hi += s;
             }
         }
-        if constexpr (MODE != DELTA) acc_product<T, DP, 2>(dq, st, kt, 0, lane);
+        if constexpr (MODE != DELTA) acc_product<T, DP, 2, TIGHT>(dq, st, im, 0, lane, 0);
     }
     if constexpr (MODE == DELTA) {
         dl += __shfl_xor(dl, 32, 64);
         if (live && h2 == 0) a.delta[si] = dl;
     } else store_rows<T, DP>(a.dq + qrow * a.sdq.rs + (long)w.head * a.sdq.hs, live, dq, a.scale, a.D, h2);
     if constexpr (MODE == DQ_TABLE) {
-        float* far = hist + 8 * ndist;
         sum_lo = wave_sum(sum_lo);
         sum_hi = wave_sum(sum_hi);
         if (lane == 0) { far[wave * 2] = sum_lo; far[wave * 2 + 1] = sum_hi; }
@@ -703,7 +771,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
         for (int i = threadIdx.x; i < ndist; i += 256) {
             float s = 0.f;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) s += hist[x * ndist + i];
+            for (int x = 0; x < 4; ++x) s += hist[x * ndist + i];
             dist[i] = s;
         }
         __syncthreads();
@@ -738,13 +806,20 @@ __global__ __launch_bounds__(256) void packed_attn_table_kernel(const float* par
     }
 }
 
+// first query tile that a key of the tile is seen by, and how many workgroups share a key tile's stream of `total` query tiles
+__device__ __forceinline__ int dkv_first(const PAttnArgs& a, int kt0, int q_len, int k_len) {
+    return kt0 >= k_len ? q_len : a.causal ? max(0, kt0 - (k_len - q_len)) / KT * KT : 0;
+}
+__device__ __forceinline__ int dkv_parts(int total, int most, int chunk) { return max(1, min(most, (total + chunk - 1) / chunk)); }
+
 // dk, dv: 128 keys of one (recording, key head), a wave 32 (lanes = keys); the query heads of the group and the 64-query tiles stream by.
-// nsplit > 1: the stream is shared between nsplit workgroups, f32 partials are added in order by packed_attn_dkv_join_kernel.
+// A stream of more than `chunk` tiles is shared between up to nsplit workgroups: f32 partials, added in order by packed_attn_dkv_join_kernel.
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dkv_kernel(PAttnArgs a) {
     using I = Image<T, DP>;
     constexpr int TB = KT * I::RB;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];      // 2 x (Q | dO) | 2 x (lse | delta) x 64 | bias by distance
+    constexpr bool TIGHT = DP == 128;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];      // 2 x (Q | dO) | 2 x (lse | -delta) x 64 | bias by distance
     float* stat = (float*)(smem + 4 * TB);
     float* dist = stat + 4 * KT;
     const int kvh = blockIdx.x % a.hkv, rest = blockIdx.x / a.hkv, split = rest % a.nsplit, ti = rest / a.nsplit;
@@ -752,15 +827,14 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
     const int q_len = a.q_len[seq], k_cap = a.k_cap[seq], k_len = max(0, min(a.k_len[seq], k_cap)), off = k_len - q_len, G = a.hq / a.hkv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
     const int kw0 = kt0 + wave * WR, key = kw0 + r;
-    const long krow = (long)a.k_start[seq] + min(key, k_cap - 1);
-    const bool live = key < k_cap;                         // rows between a recording's length and its capacity get zeros
     f32x16 dk[DP / 32], dv[DP / 32];
     zero_acc(dk);
     zero_acc(dv);
-    // query tiles from the first that a key of this tile is seen by
-    const int qfirst = kt0 >= k_len ? q_len : a.causal ? max(0, kt0 - off) / KT * KT : 0;
+    const int qfirst = dkv_first(a, kt0, q_len, k_len);
     const int per = qfirst < q_len ? (q_len - qfirst + KT - 1) / KT : 0, total = per * G;
-    const int i0 = (int)((long)total * split / a.nsplit), i1 = (int)((long)total * (split + 1) / a.nsplit);
+    const int ns = dkv_parts(total, a.nsplit, a.chunk);
+    if (split >= ns) return;
+    const int i0 = (int)((long)total * split / ns), i1 = (int)((long)total * (split + 1) / ns);
     if (i0 < i1) {
         typename I::Frag fk[DP / 16], fv[DP / 16];
         {
@@ -770,11 +844,12 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) { fk[kk] = global_frag<T, DP>(krp, kk, h2, a.D); fv[kk] = global_frag<T, DP>(vrp, kk, h2, a.D); }
         }
-        Stream<T, DP, KT, 4> qs, os;
+        Stream<T, DP, KT, 4, TIGHT> qs, os;
         qs.init(a.sq.rs, a.D, wave);
         os.init(a.sdo.rs, a.D, wave);
         const unsigned lds0 = lds_addr(smem);
-        float reg = 0.f;                                   // threads 0..63: lse of the next tile, 64..127: delta
+        typename I::Lane im = I::at(I::lane_offsets(lane), lds0 + 2 * TB);      // moved to the other buffer at every tile
+        float reg = 0.f;                                   // threads 0..63: lse of the next tile, 64..127: -delta
         auto fetch = [&](int it, unsigned dst) {
             const int g = it / per, q0 = qfirst + (it - g * per) * KT, head = kvh * G + g;
             const long row = (long)a.q_start[seq] + q0;
@@ -785,7 +860,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
                 if (threadIdx.x < KT) {
                     const float x = a.lse[s];
                     reg = in && x > -__builtin_inff() ? x * LOG2E : __builtin_inff();
-                } else reg = in ? a.delta[s] : 0.f;
+                } else reg = in ? -a.delta[s] : 0.f;
             }
             qs.load(a.q + row * a.sq.rs + (long)head * a.sq.hs, q_len - q0, dst);
             os.load(a.dout + row * a.sdo.rs + (long)head * a.sdo.hs, q_len - q0, dst + TB);
@@ -795,8 +870,6 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
         float far_lo = 0.f, far_hi = 0.f;
         for (int it = i0; it < i1; ++it) {
             const int par = (it - i0) & 1, g = it / per, q0 = qfirst + (it - g * per) * KT;
-            const char* qt = smem + par * 2 * TB;
-            const char* ot = qt + TB;
             float* ls = stat + par * 2 * KT;
             if (threadIdx.x < 2 * KT) ls[threadIdx.x] = reg;
             if constexpr (BIAS) {
@@ -809,6 +882,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
                 }
             }
             PA_SYNC_TILE();
+            I::move(im, par ? 2 * TB : -2 * TB);
             if (it + 1 < i1) fetch(it + 1, lds0 + (par ^ 1) * 2 * TB);
             const int qp0 = q0 + off;                      // position of the tile's first query
             if (kw0 >= k_len || (a.causal && qp0 + KT - 1 < kw0)) continue;
@@ -816,11 +890,17 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
             for (int t = 0; t < 2; ++t) {
                 f32x16 s[1], dp[1];
                 zero_acc(s);
-                zero_acc(dp);
+#pragma unroll
+                for (int gq = 0; gq < 4; ++gq) {           // dP - delta: the product starts from -delta of the row's query
+                    const f32x4 dl = *(const f32x4*)(ls + KT + t * 32 + 8 * gq + 4 * h2);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dp[0][4 * gq + i] = dl[i];
+                }
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
-                    I::M::mma(I::row_frag(qt, t * 32 + r, kk, h2), fk[kk], s[0]);      // rows = queries, lanes = keys
-                    I::M::mma(I::row_frag(ot, t * 32 + r, kk, h2), fv[kk], dp[0]);
+                    I::M::mma(I::row_frag(im, t, kk), fk[kk], s[0]);      // rows = queries, lanes = keys
+                    I::M::mma(I::row_frag(im, t, kk, TB), fv[kk], dp[0]);
+                    if (kk & 1) pace<TIGHT>();
                 }
                 float c = a.c, bo = 0.f;
                 const int qt0 = qp0 + t * 32;
@@ -840,39 +920,46 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
 #pragma unroll
                 for (int gq = 0; gq < 4; ++gq) {
                     const f32x4 lv = *(const f32x4*)(ls + t * 32 + 8 * gq + 4 * h2);
-                    const f32x4 dl = *(const f32x4*)(ls + KT + t * 32 + 8 * gq + 4 * h2);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int e = 4 * gq + i;
                         const float p = __builtin_amdgcn_exp2f(fmaf(s[0][e], c, bo - lv[i]));
                         s[0][e] = p;
-                        dp[0][e] = p * (dp[0][e] - dl[i]);
+                        dp[0][e] *= p;
                     }
                 }
-                acc_product<T, DP, 1>(dv, s, ot, t, lane);
-                acc_product<T, DP, 1>(dk, dp, qt, t, lane);
+                acc_product<T, DP, 1, TIGHT>(dv, s, im, t, lane, TB);
+                acc_product<T, DP, 1, TIGHT>(dk, dp, im, t, lane, 0);
             }
         }
     }
-    if (a.nsplit == 1) {
-        store_rows<T, DP>(a.dk + krow * a.sdk.rs + (long)kvh * a.sdk.hs, live, dk, a.scale, a.D, h2);
-        store_rows<T, DP>(a.dv + krow * a.sdv.rs + (long)kvh * a.sdv.hs, live, dv, 1.f, a.D, h2);
+    int own = lane;                                        // found again here: nothing of the outputs' addresses lives through the loop
+    asm volatile("" : "+v"(own));
+    const int orow = wave * WR + (own & 31), okey = kt0 + orow, oh = own >> 5;
+    const long krow = (long)a.k_start[seq] + min(okey, k_cap - 1);
+    const bool live = okey < k_cap;                        // rows between a recording's length and its capacity get zeros
+    if (ns == 1) {
+        store_rows<T, DP>(a.dk + krow * a.sdk.rs + (long)kvh * a.sdk.hs, live, dk, a.scale, a.D, oh);
+        store_rows<T, DP>(a.dv + krow * a.sdv.rs + (long)kvh * a.sdv.hs, live, dv, 1.f, a.D, oh);
     } else {
-        float* p = a.part + ((((long)ti * a.hkv + kvh) * a.nsplit + split) * 2 * TILE + wave * WR + r) * DP;
-        store_rows<float, DP>((char*)p, true, dk, a.scale, DP, h2);
-        store_rows<float, DP>((char*)(p + (long)TILE * DP), true, dv, 1.f, DP, h2);
+        float* p = a.part + ((((long)ti * a.hkv + kvh) * a.nsplit + split) * 2 * TILE + orow) * DP;
+        store_rows<float, DP>((char*)p, true, dk, a.scale, DP, oh);
+        store_rows<float, DP>((char*)(p + (long)TILE * DP), true, dv, 1.f, DP, oh);
     }
 }
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(PAttnArgs a) {
     const int kvh = blockIdx.x % a.hkv, ti = blockIdx.x / a.hkv, seq = a.tiles[2 * ti], kt0 = a.tiles[2 * ti + 1];
-    const int rows = min(TILE, a.k_cap[seq] - kt0);
+    const int rows = min(TILE, a.k_cap[seq] - kt0), q_len = a.q_len[seq], k_len = max(0, min(a.k_len[seq], a.k_cap[seq]));
+    const int qfirst = dkv_first(a, kt0, q_len, k_len), per = qfirst < q_len ? (q_len - qfirst + KT - 1) / KT : 0;
+    const int ns = dkv_parts(per * (a.hq / a.hkv), a.nsplit, a.chunk);
+    if (ns == 1) return;
     const float* p = a.part + ((long)ti * a.hkv + kvh) * a.nsplit * 2 * TILE * DP;
     for (int i = threadIdx.x; i < 2 * rows * (DP / 8); i += 256) {
         const int which = i >= rows * (DP / 8), j = i - which * rows * (DP / 8), row = j / (DP / 8), d = (j % (DP / 8)) * 8;
         if (d >= a.D) continue;
         float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int x = 0; x < a.nsplit; ++x) {
+        for (int x = 0; x < ns; ++x) {
             float y[8];
             load8<float>(p + ((long)(x * 2 + which) * TILE + row) * DP + d, y);
 #pragma unroll
@@ -884,24 +971,31 @@ __global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(PAttnArgs a) 
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------------------------------
-// more than 64 KB of LDS has to be asked for (on the current device)
+// more than 64 KB of LDS has to be asked for, once per kernel, device and thread
 int ask_lds(const void* kernel, int bytes) {
-    return bytes > 65536 && hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess;
+    if (bytes <= 65536) return 0;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return -1;
+    static thread_local struct { const void* kernel; int dev; } done[64];
+    static thread_local int n = 0;
+    for (int i = 0; i < n; ++i) if (done[i].kernel == kernel && done[i].dev == dev) return 0;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return -1;
+    if (n < 64) { done[n].kernel = kernel; done[n].dev = dev; ++n; }
+    return 0;
 }
 
 struct Plan {                   // the host array of pseld_hip.h
-    long seqs, rows, max_q, k_rows, max_k, q_tiles, k_tiles;
+    long seqs, rows, max_q, k_rows, max_k, q_tiles, k_tiles, k_work, k_work_causal;
     const int *q_start, *q_len, *k_start, *k_cap, *k_len, *q_tile, *q_tile_causal, *k_tile, *k_tile_causal;
 };
 Plan plan_of(const long* p) {
     Plan x;
-    x.seqs = p[0]; x.rows = p[1]; x.max_q = p[2]; x.k_rows = p[3]; x.max_k = p[4]; x.q_tiles = p[5]; x.k_tiles = p[6];
+    x.seqs = p[0]; x.rows = p[1]; x.max_q = p[2]; x.k_rows = p[3]; x.max_k = p[4]; x.q_tiles = p[5]; x.k_tiles = p[6]; x.k_work = p[7]; x.k_work_causal = p[8];
     const int** a[] = {&x.q_start, &x.q_len, &x.k_start, &x.k_cap, &x.k_len, &x.q_tile, &x.q_tile_causal, &x.k_tile, &x.k_tile_causal};
-    for (int i = 0; i < 9; ++i) *a[i] = (const int*)p[7 + i];
+    for (int i = 0; i < 9; ++i) *a[i] = (const int*)p[9 + i];
     return x;
 }
 int pad_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
-constexpr int LDS_MAX = 160 * 1024;
 constexpr int FEW_TABLE = 4096;          // table entries of one key head's group that the few-rows kernel keeps in LDS
 
 // The few-rows kernel takes the call when one key head's query rows of every recording fit its 32-row operand.
@@ -915,13 +1009,17 @@ int few_chunk(const Plan& p, int hkv) {
     return (int)(c < 256 ? 256 : c > 8192 ? 8192 : c);
 }
 int few_splits(const Plan& p, int hkv) { const int c = few_chunk(p, hkv); return p.max_k > c ? (int)((p.max_k + c - 1) / c) : 1; }
-// workgroups that share a key tile's stream of queries: enough for two workgroups per CU, no more than the longest stream has tiles
-int dkv_splits(const Plan& p, int hq, int hkv) {
-    const long wgs = p.k_tiles * hkv, longest = (p.max_q + KT - 1) / KT * (hq / hkv);
-    if (wgs == 0 || wgs >= 512) return 1;
-    long n = (512 + wgs - 1) / wgs;
-    if (n > longest / 2) n = longest / 2;
-    return n < 1 ? 1 : n > 32 ? 32 : (int)n;
+// Query tiles per workgroup of the dk/dv kernel: two workgroups fit a CU, so the whole work is cut into about 400 equal parts (a few of the
+// 512 places stay free for the tiles' odd ends) where the key tiles alone would not fill the chip or end unevenly; below 4 tiles a part
+// would spend longer on its f32 partials than on its tiles.
+int dkv_chunk(const Plan& p, int hq, int hkv, int causal) {
+    const long work = (causal ? p.k_work_causal : p.k_work) * hq;
+    const long c = (work + 399) / 400;
+    return (int)(c < 4 ? 4 : c > (1 << 20) ? 1 << 20 : c);
+}
+int dkv_splits(const Plan& p, int hq, int hkv, int causal) {
+    const long longest = (p.max_q + KT - 1) / KT * (hq / hkv), c = dkv_chunk(p, hq, hkv, causal);
+    return longest > c ? (int)((longest + c - 1) / c) : 1;
 }
 bool delta_pass(int dtype, bool table_grad) { return table_grad && dtype == PSELD_BF16; }
 
@@ -988,7 +1086,7 @@ int run_bwd(PAttnArgs& a, const Plan& p, float* dtable, int accumulate, hipStrea
     if constexpr (BIAS) {
         if (dtable) {
             float* part = a.part;
-            PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ_TABLE>), p.q_tiles * a.hq, 256, (dq_buffers<T, DP, DQ_TABLE>()) * 2 * TB + 9 * nd + 64, a);
+            PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ_TABLE>), p.q_tiles * a.hq, 256, (dq_buffers<T, DP, DQ_TABLE>()) * 2 * TB + 5 * nd + 64 + 4 * DIAG * 4, a);
             PA_LAUNCH(packed_attn_table_kernel, (long)a.hq * ((a.buckets + 15) / 16), 256, 0, part, dtable, (int)p.q_tiles, a.hq, a.buckets, accumulate);
             a.part += p.q_tiles * a.hq * a.buckets;
             a.part = (float*)(((uintptr_t)a.part + 15) & ~(uintptr_t)15);
@@ -997,7 +1095,8 @@ int run_bwd(PAttnArgs& a, const Plan& p, float* dtable, int accumulate, hipStrea
     }
     if (!table_done) PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ>), p.q_tiles * a.hq, 256, 4 * TB + nd, a);
     a.tiles = a.causal ? p.k_tile_causal : p.k_tile;
-    a.nsplit = dkv_splits(p, a.hq, a.hkv);
+    a.nsplit = dkv_splits(p, a.hq, a.hkv, a.causal);
+    a.chunk = dkv_chunk(p, a.hq, a.hkv, a.causal);
     PA_LAUNCH((packed_attn_dkv_kernel<T, DP, BIAS>), p.k_tiles * a.hkv * a.nsplit, 256, 4 * TB + 4 * KT * 4 + nd, a);
     if (a.nsplit > 1) PA_LAUNCH((packed_attn_dkv_join_kernel<T, DP>), p.k_tiles * a.hkv, 256, 0, a);
     return PSELD_OK;
@@ -1052,10 +1151,10 @@ extern "C" int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, co
     return PSELD_OK;
 }
 
-extern "C" long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int buckets) {
+extern "C" long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int causal, int buckets) {
     if (!plan || hkv <= 0 || hq < hkv || hq % hkv) return 0;
     const Plan p = plan_of(plan);
-    const long n = dkv_splits(p, hq, hkv);
+    const long n = dkv_splits(p, hq, hkv, causal);
     return ((p.rows * hq + 3) / 4 * 4 + p.q_tiles * hq * buckets + 4 + (n > 1 ? p.k_tiles * hkv * n * 2 * TILE * pad_of(D) : 0)) * (long)sizeof(float);
 }
 
@@ -1079,7 +1178,7 @@ extern "C" int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q,
     PA_TRY(check_operand(n, "dk", dtype, dk, strides + 12, a.sdk, keys));
     PA_TRY(check_operand(n, "dv", dtype, dv, strides + 14, a.sdv, keys));
     PSELD_CHECK_ARG(!rows || lse, "packed_attn_bwd: null pointer (lse)");
-    const long need = pseld_packed_attn_bwd_workspace(plan, hq, hkv, D, dtable ? buckets : 0);
+    const long need = pseld_packed_attn_bwd_workspace(plan, hq, hkv, D, causal, dtable ? buckets : 0);
     PSELD_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, "packed_attn_bwd: workspace too small");
     a.dout = (const char*)dout; a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (const char*)out; a.lse = const_cast<float*>(lse);
     a.dq = (char*)dq; a.dk = (char*)dk; a.dv = (char*)dv;

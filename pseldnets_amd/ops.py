@@ -1577,7 +1577,6 @@ class PackedPlan:
 
     def __init__(self, q_lens, k_lens, k_cap, device):
         q_lens = [int(n) for n in q_lens]
-        own_keys = k_lens is not None or k_cap is not None
         k_lens = q_lens if k_lens is None else [int(n) for n in k_lens]
         caps = k_lens if k_cap is None else [int(n) for n in (k_cap if hasattr(k_cap, '__iter__') else [k_cap] * len(q_lens))]
         if not q_lens:
@@ -1593,7 +1592,8 @@ class PackedPlan:
             raise _lib.PseldError("packed_plan: the plan must live on the MI355X (no CPU fallback)")
         if self.device.index is None:
             self.device = torch.device('cuda', torch.cuda.current_device())
-        self.q_lens, self.k_caps, self.self_keys = q_lens, caps, not own_keys
+        self._index = self.device.index
+        self.q_lens, self.k_caps = q_lens, caps
         self.seqs, self.rows, self.max_q = len(q_lens), sum(q_lens), max(q_lens)
         self.k_rows, self.max_k = sum(caps), max(caps)
         T = _PACKED_TILE
@@ -1625,7 +1625,8 @@ class PackedPlan:
         self._ptr = {k: self._ints.data_ptr() + 4 * v for k, v in at.items()}
         self.k_len = self._ints[at['k_len']:at['k_len'] + self.seqs]
         names = ('q_start', 'q_len', 'k_start', 'k_cap', 'k_len', 'q_tile', 'q_tile_causal', 'k_tile', 'k_tile_causal')
-        self._desc = (ctypes.c_long * 16)(self.seqs, self.rows, self.max_q, self.k_rows, self.max_k, self.q_tiles, self.k_tiles,
+        work = [sum((-w + 63) // 64 for w, _, _ in tiles if w < 0) for tiles in (kf, kc)]       # 64-query tiles that a key tile meets, summed
+        self._desc = (ctypes.c_long * 18)(self.seqs, self.rows, self.max_q, self.k_rows, self.max_k, self.q_tiles, self.k_tiles, *work,
                                           *(self._ptr[k] for k in names))
 
 
@@ -1639,25 +1640,29 @@ def packed_plan(q_lens, k_lens=None, k_cap=None, device='cuda'):
     return PackedPlan(q_lens, k_lens, k_cap, device)
 
 
-def _rows_ok(what, plan, dtype, *ts):
-    """2-D row operands of the plan: on its device, of one type, unit column stride, one row per frame."""
-    if plan.device.index != torch.cuda.current_device():
+def _on_plan(what, plan):
+    """The plan's device must be the current one; returns the current stream's handle (a frame of a running stream takes a few
+    microseconds on the device: the checks of these operators are written to stay below that on the host)."""
+    index = plan._index
+    if torch._C._cuda_getDevice() != index:
         raise _lib.PseldError(f"{what}: the plan lives on {plan.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _rows_ok(what, plan, shape, dtype, *ts):
+    """2-D row operands of the plan: on its device, of one type and shape, unit column stride, one row per frame."""
+    index = plan._index
+    if len(shape) != 2 or shape[0] != plan.rows:
+        raise _lib.PseldError(f"{what}: operands must be [rows of the plan = {plan.rows}, C], one is {tuple(shape)}")
     for t in ts:
-        if t is None:
-            continue
-        if t.device != plan.device:
-            raise _lib.PseldError(f"{what}: operands must live on the plan's device {plan.device}, one is on {t.device}")
-        if t.dtype != dtype:
-            raise _lib.PseldError(f"{what}: operands must share one dtype ({dtype} and {t.dtype})")
-        if t.dim() != 2 or t.shape[0] != plan.rows or t.shape != ts[0].shape or t.stride(1) != 1:
-            raise _lib.PseldError(f"{what}: operands must be [rows of the plan = {plan.rows}, C] with unit stride along their columns, one is "
-                                  f"{tuple(t.shape)} with strides {t.stride()}")
+        if t is not None and (t.get_device() != index or t.dtype is not dtype or t.shape != shape or t.stride(1) != 1):
+            raise _lib.PseldError(f"{what}: operands must be {dtype} {tuple(shape)} on {plan.device} with unit stride along their columns, one is "
+                                  f"{t.dtype} {tuple(t.shape)} on {t.device} with strides {t.stride()}")
 
 
 def _state_ok(what, plan, C, *ts):
     for t in ts:
-        if t is not None and (t.device != plan.device or t.dtype != torch.float32 or tuple(t.shape) != (plan.seqs, C) or not t.is_contiguous()):
+        if t is not None and (t.get_device() != plan._index or t.dtype is not torch.float32 or t.shape != (plan.seqs, C) or not t.is_contiguous()):
             raise _lib.PseldError(f"{what}: states must be contiguous float32 [recordings = {plan.seqs}, C = {C}] on {plan.device}")
 
 
@@ -1671,17 +1676,18 @@ def linrec_fwd(g, n, plan, h0=None, reverse=False, need_saved=True, out=None):
     """z = sigmoid(g), h_t = z_t h_{t-1} + (1 - z_t) n_t over every recording of the plan (from its last frame to its first when
     reverse). g, n [rows, C] (row-strided views allowed), h0 f32 [recordings, C] or None (zeros).
     Returns (h [rows, C], h_last f32 [recordings, C], what linrec_bwd needs or None)."""
-    _rows_ok("linrec_fwd", plan, g.dtype, g, n, out)
+    stream = _on_plan("linrec_fwd", plan)
+    _rows_ok("linrec_fwd", plan, g.shape, g.dtype, g, n, out)
     C = g.shape[1]
     _state_ok("linrec_fwd", plan, C, h0)
     L = _lib.lib()
-    h = torch.empty((plan.rows, C), dtype=g.dtype, device=g.device) if out is None else out
-    h_last = torch.empty((plan.seqs, C), dtype=torch.float32, device=g.device)
+    h = g.new_empty((plan.rows, C)) if out is None else out
+    h_last = torch.empty((plan.seqs, C), dtype=torch.float32, device=plan.device)
     states = torch.empty((L.pseld_linrec_states(plan.rows, plan.seqs), C), dtype=torch.float32, device=g.device) if need_saved else None
     ws, nbytes = _linrec_ws(plan, C)
     rc = L.pseld_linrec_fwd(dtype_code(g), _lib.ptr(g), g.stride(0), _lib.ptr(n), n.stride(0), _lib.ptr(h0), _lib.ptr(h), h.stride(0),
                             _lib.ptr(h_last), _lib.ptr(states), plan._ptr['q_start'], plan._ptr['q_len'], plan.seqs, plan.rows, plan.max_q, C,
-                            int(bool(reverse)), _lib.ptr(ws), nbytes, _lib.stream_ptr())
+                            int(bool(reverse)), _lib.ptr(ws), nbytes, stream)
     _lib.check(rc, "pseld_linrec_fwd")
     return h, h_last, states
 
@@ -1689,19 +1695,20 @@ def linrec_fwd(g, n, plan, h0=None, reverse=False, need_saved=True, out=None):
 def linrec_bwd(dh, g, n, saved, plan, dh_last=None, h0=None, reverse=False, dg=None, dn=None):
     """Gradients of linrec_fwd for dh [rows, C] and dh_last f32 [recordings, C] (or None): (dg, dn, dh0 or None where h0 is None).
     dg, dn: optional outputs (row-strided views allowed, e.g. the halves of the gates' projection's gradient)."""
-    _rows_ok("linrec_bwd", plan, g.dtype, g, n, dh, dg, dn)
+    stream = _on_plan("linrec_bwd", plan)
+    _rows_ok("linrec_bwd", plan, g.shape, g.dtype, g, n, dh, dg, dn)
     C = g.shape[1]
     _state_ok("linrec_bwd", plan, C, h0, dh_last)
     L = _lib.lib()
     if saved is None or tuple(saved.shape) != (L.pseld_linrec_states(plan.rows, plan.seqs), C) or saved.dtype != torch.float32 or saved.device != plan.device:
         raise _lib.PseldError("linrec_bwd: saved must be what linrec_fwd(need_saved=True) returned for this plan")
-    dg = torch.empty((plan.rows, C), dtype=g.dtype, device=g.device) if dg is None else dg
-    dn = torch.empty((plan.rows, C), dtype=g.dtype, device=g.device) if dn is None else dn
+    dg = g.new_empty((plan.rows, C)) if dg is None else dg
+    dn = g.new_empty((plan.rows, C)) if dn is None else dn
     dh0 = torch.empty((plan.seqs, C), dtype=torch.float32, device=g.device) if h0 is not None else None
     ws, nbytes = _linrec_ws(plan, C)
     rc = L.pseld_linrec_bwd(dtype_code(g), _lib.ptr(dh), dh.stride(0), _lib.ptr(g), g.stride(0), _lib.ptr(n), n.stride(0), _lib.ptr(saved),
                             _lib.ptr(dh_last), _lib.ptr(dg), dg.stride(0), _lib.ptr(dn), dn.stride(0), _lib.ptr(dh0), plan._ptr['q_start'],
-                            plan._ptr['q_len'], plan.seqs, plan.rows, plan.max_q, C, int(bool(reverse)), _lib.ptr(ws), nbytes, _lib.stream_ptr())
+                            plan._ptr['q_len'], plan.seqs, plan.rows, plan.max_q, C, int(bool(reverse)), _lib.ptr(ws), nbytes, stream)
     _lib.check(rc, "pseld_linrec_bwd")
     return dg, dn, dh0
 
@@ -1749,41 +1756,35 @@ def relpos_buckets(num_buckets=32, max_distance=128, bidirectional=True, device=
     return RelposBuckets(num_buckets, max_distance, bidirectional, device)
 
 
-def _heads_ok(what, plan, dtype, named, rows):
-    """[rows, heads, D] operands on the plan's device: one type, unit stride inside a head."""
-    for name, t in named:
-        if t.device != plan.device:
-            raise _lib.PseldError(f"{what}: {name} must live on the plan's device {plan.device}, it is on {t.device}")
-        if t.dtype != dtype:
-            raise _lib.PseldError(f"{what}: operands must share one dtype ({name} is {t.dtype}, not {dtype})")
-        if t.dim() != 3 or t.shape[0] != rows or t.stride(2) != 1:
-            raise _lib.PseldError(f"{what}: {name} must be [rows = {rows}, heads, head size] with unit stride inside a head, it is {tuple(t.shape)} "
-                                  f"with strides {t.stride()}")
+def _heads_ok(what, plan, dtype, rows, heads, D, name, t):
+    """A [rows, heads, D] operand on the plan's device with unit stride inside a head."""
+    if t.get_device() != plan._index or t.dtype is not dtype or t.shape != (rows, heads, D) or t.stride(2) != 1:
+        raise _lib.PseldError(f"{what}: {name} must be {dtype} [rows = {rows}, heads = {heads}, head size = {D}] on {plan.device} with unit stride inside a "
+                              f"head, it is {t.dtype} {tuple(t.shape)} on {t.device} with strides {t.stride()}")
 
 
 def _packed_attn_args(what, plan, q, k, v, scale, bias_table, buckets):
-    if plan.device.index != torch.cuda.current_device():
-        raise _lib.PseldError(f"{what}: the plan lives on {plan.device}, the current device is cuda:{torch.cuda.current_device()}")
-    _heads_ok(what, plan, q.dtype, (('q', q),), plan.rows)
-    _heads_ok(what, plan, q.dtype, (('k', k), ('v', v)), plan.k_rows)
-    hq, D, hkv = q.shape[1], q.shape[2], k.shape[1]
-    if k.shape[2] != D or v.shape != k.shape:
-        raise _lib.PseldError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} must have one head size, k and v one shape")
+    if q.dim() != 3 or k.dim() != 3:
+        raise _lib.PseldError(f"{what}: q, k and v must be [rows, heads, head size], q is {tuple(q.shape)} and k {tuple(k.shape)}")
+    dtype, (_, hq, D), hkv = q.dtype, q.shape, k.shape[1]
+    if hkv < 1 or hq % hkv:
+        raise _lib.PseldError(f"{what}: {hq} query heads cannot share {hkv} key heads")
+    _heads_ok(what, plan, dtype, plan.rows, hq, D, 'q', q)
+    _heads_ok(what, plan, dtype, plan.k_rows, hkv, D, 'k', k)
+    _heads_ok(what, plan, dtype, plan.k_rows, hkv, D, 'v', v)
     if (bias_table is None) != (buckets is None):
         raise _lib.PseldError(f"{what}: bias_table and buckets come together")
-    if buckets is not None:
-        if buckets.device != plan.device or bias_table.device != plan.device or bias_table.dtype != torch.float32 or not bias_table.is_contiguous() or \
-                tuple(bias_table.shape) != (buckets.num_buckets, hq):
-            raise _lib.PseldError(f"{what}: bias_table must be contiguous float32 [buckets = {buckets.num_buckets}, query heads = {hq}] on {plan.device}")
-    return hq, hkv, D, float(scale) if scale is not None else D ** -0.5
+    if buckets is not None and (buckets.device != plan.device or bias_table.get_device() != plan._index or bias_table.dtype is not torch.float32 or
+                                bias_table.shape != (buckets.num_buckets, hq) or not bias_table.is_contiguous()):
+        raise _lib.PseldError(f"{what}: bias_table must be contiguous float32 [buckets = {buckets.num_buckets}, query heads = {hq}] on {plan.device}")
+    return dtype, hq, hkv, D, D ** -0.5 if scale is None else float(scale)
 
 
 def _table_args(bias_table, buckets):
     return (bias_table.data_ptr(), buckets._ints.data_ptr(), buckets.num_buckets, buckets.max_distance) if buckets is not None else (None, None, 0, 0)
 
 
-def _head_strides(*ts):
-    return (ctypes.c_long * (2 * len(ts)))(*[s for t in ts for s in t.stride()[:2]])
+_LONGS8, _LONGS16 = ctypes.c_long * 8, ctypes.c_long * 16
 
 
 def packed_attn_fwd(q, k, v, plan, causal=False, scale=None, bias_table=None, buckets=None, out=None):
@@ -1792,21 +1793,25 @@ def packed_attn_fwd(q, k, v, plan, causal=False, scale=None, bias_table=None, bu
     stands at position i + k_len - q_len; causal masks the keys behind a query's position. A row without keys gives 0 and -inf. scale: D^-1/2 where None.
     bias_table f32 [buckets, query heads] with buckets = relpos_buckets(...): bias_table[bucket(key position - query position), head]
     is added to the scaled scores. Key rows past a recording's k_len are never read."""
-    hq, hkv, D, scale = _packed_attn_args("packed_attn_fwd", plan, q, k, v, scale, bias_table, buckets)
+    stream = _on_plan("packed_attn_fwd", plan)
+    dtype, hq, hkv, D, scale = _packed_attn_args("packed_attn_fwd", plan, q, k, v, scale, bias_table, buckets)
     L = _lib.lib()
     if out is None:
-        out = torch.empty((plan.rows, hq, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((plan.rows, hq, D))
     else:
-        _heads_ok("packed_attn_fwd", plan, q.dtype, (('out', out),), plan.rows)
-        if out.shape != q.shape:
-            raise _lib.PseldError("packed_attn_fwd: out must have q's shape")
-    lse = torch.empty((plan.rows, hq), dtype=torch.float32, device=q.device)
+        _heads_ok("packed_attn_fwd", plan, dtype, plan.rows, hq, D, 'out', out)
+    lse = torch.empty((plan.rows, hq), dtype=torch.float32, device=plan.device)
     table, lut, nb, md = _table_args(bias_table, buckets)
-    nbytes = L.pseld_packed_attn_fwd_workspace(plan._desc, hq, hkv, D, nb) if hkv and hq % hkv == 0 else 0
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None      # its own per call: nothing shared between streams
-    rc = L.pseld_packed_attn_fwd(dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _head_strides(q, k, v, out),
-                                 plan._desc, hq, hkv, D, int(bool(causal)), scale, table, lut, nb, md, _lib.ptr(ws), nbytes, _lib.stream_ptr())
-    _lib.check(rc, "pseld_packed_attn_fwd")
+    nbytes = L.pseld_packed_attn_fwd_workspace(plan._desc, hq, hkv, D, nb)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=plan.device) if nbytes else None      # its own per call: nothing shared between streams
+    q0, q1, _ = q.stride()
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    o0, o1, _ = out.stride()
+    rc = L.pseld_packed_attn_fwd(dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _LONGS8(q0, q1, k0, k1, v0, v1, o0, o1),
+                                 plan._desc, hq, hkv, D, 1 if causal else 0, scale, table, lut, nb, md, None if ws is None else ws.data_ptr(), nbytes, stream)
+    if rc:
+        _lib.check(rc, "pseld_packed_attn_fwd")
     return out, lse
 
 
@@ -1814,25 +1819,28 @@ def packed_attn_bwd(dout, q, k, v, out, lse, plan, causal=False, scale=None, bia
                     dq=None, dk=None, dv=None):
     """Gradients of packed_attn_fwd (same plan, lengths and options; out and lse are what it returned): (dq, dk, dv). dbias_table f32 [buckets, query heads]:
     written (accumulate: added to) where given. dq, dk, dv: optional outputs (e.g. the parts of the projection's gradient)."""
-    hq, hkv, D, scale = _packed_attn_args("packed_attn_bwd", plan, q, k, v, scale, bias_table, buckets)
-    dq = torch.empty((plan.rows, hq, D), dtype=q.dtype, device=q.device) if dq is None else dq
-    dk = torch.empty((plan.k_rows, hkv, D), dtype=q.dtype, device=q.device) if dk is None else dk
-    dv = torch.empty((plan.k_rows, hkv, D), dtype=q.dtype, device=q.device) if dv is None else dv
-    _heads_ok("packed_attn_bwd", plan, q.dtype, (('dout', dout), ('out', out), ('dq', dq)), plan.rows)
-    _heads_ok("packed_attn_bwd", plan, q.dtype, (('dk', dk), ('dv', dv)), plan.k_rows)
-    if not (dout.shape == out.shape == dq.shape == q.shape and dk.shape == dv.shape == k.shape):
-        raise _lib.PseldError("packed_attn_bwd: dout, out and dq must have q's shape, dk and dv k's")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (plan.rows, hq) or not lse.is_contiguous() or lse.device != plan.device:
+    what = "packed_attn_bwd"
+    stream = _on_plan(what, plan)
+    dtype, hq, hkv, D, scale = _packed_attn_args(what, plan, q, k, v, scale, bias_table, buckets)
+    dq = q.new_empty((plan.rows, hq, D)) if dq is None else dq
+    dk = q.new_empty((plan.k_rows, hkv, D)) if dk is None else dk
+    dv = q.new_empty((plan.k_rows, hkv, D)) if dv is None else dv
+    for name, t in (('dout', dout), ('out', out), ('dq', dq)):
+        _heads_ok(what, plan, dtype, plan.rows, hq, D, name, t)
+    for name, t in (('dk', dk), ('dv', dv)):
+        _heads_ok(what, plan, dtype, plan.k_rows, hkv, D, name, t)
+    if lse.get_device() != plan._index or lse.dtype is not torch.float32 or lse.shape != (plan.rows, hq) or not lse.is_contiguous():
         raise _lib.PseldError("packed_attn_bwd: lse must be what packed_attn_fwd returned")
-    if dbias_table is not None and (buckets is None or dbias_table.dtype != torch.float32 or dbias_table.shape != bias_table.shape or
-                                    not dbias_table.is_contiguous() or dbias_table.device != plan.device):
+    if dbias_table is not None and (buckets is None or dbias_table.dtype is not torch.float32 or dbias_table.shape != bias_table.shape or
+                                    not dbias_table.is_contiguous() or dbias_table.get_device() != plan._index):
         raise _lib.PseldError("packed_attn_bwd: dbias_table must be contiguous float32 of bias_table's shape, beside bias_table and buckets")
     L = _lib.lib()
     table, lut, nb, md = _table_args(bias_table, buckets)
-    nbytes = L.pseld_packed_attn_bwd_workspace(plan._desc, hq, hkv, D, nb if dbias_table is not None else 0) if hkv and hq % hkv == 0 else 0
-    ws = torch.empty((nbytes + 15) // 16 * 4, dtype=torch.float32, device=q.device)
+    nbytes = L.pseld_packed_attn_bwd_workspace(plan._desc, hq, hkv, D, 1 if causal else 0, nb if dbias_table is not None else 0)
+    ws = torch.empty((nbytes + 15) // 16 * 4, dtype=torch.float32, device=plan.device)
+    strides = _LONGS16(*[n for t in (dout, q, k, v, out, dq, dk, dv) for n in t.stride()[:2]])
     rc = L.pseld_packed_attn_bwd(dtype_code(q), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(),
-                                 dk.data_ptr(), dv.data_ptr(), _head_strides(dout, q, k, v, out, dq, dk, dv), plan._desc, hq, hkv, D, int(bool(causal)),
-                                 scale, table, lut, nb, md, _lib.ptr(dbias_table), int(bool(accumulate)), _lib.ptr(ws), nbytes, _lib.stream_ptr())
+                                 dk.data_ptr(), dv.data_ptr(), strides, plan._desc, hq, hkv, D, 1 if causal else 0, scale, table, lut, nb, md,
+                                 _lib.ptr(dbias_table), int(bool(accumulate)), ws.data_ptr(), nbytes, stream)
     _lib.check(rc, "pseld_packed_attn_bwd")
     return dq, dk, dv

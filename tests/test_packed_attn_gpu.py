@@ -498,14 +498,14 @@ def test_c_entry_refuses_without_a_launch():
         pytest.skip("libpseld_hip.so not built")
     L = _lib.lib()
     A = 4096                                                 # an address that is never followed
-    plan = (ctypes.c_long * 16)(1, 40, 40, 40, 40, 1, 1, *[A] * 9)
+    plan = (ctypes.c_long * 18)(1, 40, 40, 40, 40, 1, 1, 1, 1, *[A] * 9)
     st = (ctypes.c_long * 16)(*[256, 64] * 8)
 
     def fwd(dtype=0, q=A, k=A, st=st, plan=plan, hq=4, hkv=4, D=64, scale=1.0, table=None, lut=None, nb=0, md=0):
         return L.pseld_packed_attn_fwd(dtype, q, k, A, A, A, st, plan, hq, hkv, D, 0, scale, table, lut, nb, md, None, 0, None)
     odd = (ctypes.c_long * 16)(*[257, 64] * 8)
     far = (ctypes.c_long * 16)(*[1 << 24, 64] * 8)
-    few = (ctypes.c_long * 16)(1, 1, 1, 100000, 100000, 1, 782, *[A] * 9)
+    few = (ctypes.c_long * 18)(1, 1, 1, 100000, 100000, 1, 782, 782, 782, *[A] * 9)
     for bad in (dict(dtype=3), dict(q=None), dict(k=None), dict(q=A + 8), dict(st=odd), dict(st=far), dict(st=None), dict(plan=None), dict(hq=5, hkv=2), dict(hkv=0),
                 dict(D=60), dict(D=136), dict(D=0), dict(scale=0.0), dict(scale=float('inf')), dict(table=A), dict(table=A, lut=A, nb=513, md=128),
                 dict(table=A, lut=A, nb=32, md=1025), dict(plan=few)):
