@@ -509,10 +509,10 @@ int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void* g, long l
  * buckets, and calls of few rows (the next frame of running streams), which share the keys between workgroups.
  *   S = scale q k^T + table[bucket(key position - query position), head], P = softmax over the keys that the mask leaves, out = P v,
  *   lse[row, head] = log sum exp S;  a row without keys: out 0, lse -inf. Query i of a recording stands at position i + k_len - q_len; causal: keys
- *   behind a query's position are masked. |table| is taken to be below 1e37.
+ *   behind a query's position are masked. |table| / scale is taken to be below 1e37.
  * plan: HOST array of 18 longs {seqs, rows, max_q, k_rows, max_k, q_tiles, k_tiles, the 64-query tiles that the key tiles meet, summed: full and
- * causal, then device int arrays as addresses: q_start[seqs], q_len[seqs], k_start[seqs], k_cap[seqs], k_len[seqs], q_tile[q_tiles][2], q_tile_causal, k_tile[k_tiles][2], k_tile_causal}: a tile is
- * (recording, first row) of 128 rows of queries or of capacity, heaviest first. k_len may change between calls; it is held to 0 .. k_cap.
+ * causal, then device int arrays as addresses: q_start[seqs], q_len[seqs], k_start[seqs], k_cap[seqs], k_len[seqs], q_tile[q_tiles][8], q_tile_causal, k_tile[k_tiles][8], k_tile_causal}: a tile is 128 rows
+ * of queries or of capacity, {recording s, first row, q_start[s], q_len[s], k_start[s], k_cap[s], 0, 0}, heaviest first. k_len may change between calls; it is held to 0 .. k_cap.
  * strides: HOST array of longs, {row stride, head stride} in elements of q, k, v, out (bwd: dout, q, k, v, out, dq, dk, dv), whole
  * 16-byte pieces; unit stride inside a head. table f32 [buckets, hq] or NULL; lut (device ints): the bucket of every distance
  * -max_distance .. max_distance, then [buckets][2] first and last distance of each (none: first > last).

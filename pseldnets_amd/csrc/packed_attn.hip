@@ -60,8 +60,8 @@ template <int RB> __device__ __forceinline__ int image_swizzle(int row) {
 }
 typedef __attribute__((address_space(3))) const char* lds_cptr;
 // A lane's reads of an image. The swizzle only XORs bits inside a row, so a lane keeps three offsets for the tile at hand and reaches every piece by
-// XOR with a constant and the instruction's immediate. at() hides the offsets from loop-invariant motion: hoisted, the dozens of
-// XORed addresses cost more registers than recomputing them per tile costs time (the dk/dv kernel for 128 spilled 60 registers).
+// XOR with a constant and the instruction's immediate. move<true> hides the offsets from loop-invariant motion: where the accumulators fill the
+// register file, the hoisted XORs spill (60 registers in the dk/dv kernel for 128); elsewhere hoisting them is faster (forward for 128: 10 %).
 template <typename T, int DP> struct Image {
     static constexpr int RB = DP * (int)sizeof(T);
     using M = AMma<T>;
@@ -81,16 +81,14 @@ template <typename T, int DP> struct Image {
         }
         return l;
     }
-    static __device__ __forceinline__ void move(Lane& l, unsigned by) {
+    template <bool HIDE> static __device__ __forceinline__ void move(Lane& l, unsigned by) {
         l.row += by;
         l.lo += by;
-        asm volatile("" : "+v"(l.row));
-        if constexpr (sizeof(T) == 2) {
-            l.hi += by;
-            asm volatile("" : "+v"(l.lo), "+v"(l.hi));
-        }
+        if constexpr (sizeof(T) == 2) l.hi += by;
+        if constexpr (HIDE) asm volatile("" : "+v"(l.row), "+v"(l.lo));
+        if constexpr (HIDE && sizeof(T) == 2) asm volatile("" : "+v"(l.hi));
     }
-    static __device__ __forceinline__ Lane at(Lane l, unsigned tile) { move(l, tile); return l; }
+    static __device__ __forceinline__ Lane at(Lane l, unsigned tile) { move<false>(l, tile); return l; }
     // elements 16 kk + 8 h2 .. + 7 of image row 32 t + (lane & 31); off: bytes from the tile that l stands for (a multiple of 1024)
     static __device__ __forceinline__ Frag row_frag(const Lane& l, int t, int kk, int off = 0) {
         if constexpr (sizeof(T) == 2) return *(const __attribute__((address_space(3))) bf16x8*)(lds_cptr)(uintptr_t)((l.row ^ (kk << 5)) + t * 32 * RB + off);
@@ -208,12 +206,13 @@ template <typename T, int DP, int ROWS, int NW, bool LAZY = false> struct Stream
 __device__ __forceinline__ int dist_count(int maxd) { return 2 * (maxd + NEAR_PAD) + 1; }
 __device__ __forceinline__ float bias_at(const PAttnArgs& a, int rel, int head) {
     const int r = max(-a.maxd, min(a.maxd, rel));
-    return a.table[(long)a.lut[r + a.maxd] * a.hq + head] * LOG2E;
+    return a.table[(long)a.lut[r + a.maxd] * a.hq + head];
 }
-// dist[i] = log2(e) * bias of distance i - maxd - NEAR_PAD
+// dist[i] = bias of distance i - maxd - NEAR_PAD over the scale: in units of the raw products, whose accumulators start from it
 __device__ __forceinline__ void dist_fill(float* dist, const PAttnArgs& a, int head, int threads) {
     const int n = dist_count(a.maxd);
-    for (int i = threadIdx.x; i < n; i += threads) dist[i] = bias_at(a, i - a.maxd - NEAR_PAD, head);
+    const float inv = 1.f / a.scale;
+    for (int i = threadIdx.x; i < n; i += threads) dist[i] = bias_at(a, i - a.maxd - NEAR_PAD, head) * inv;
 }
 
 // Keeps the scheduler from requesting a whole product's operands at once where the accumulators leave no registers for them
@@ -316,13 +315,16 @@ template <int DP> struct Softmax {
     }
 };
 
-// Adds the bias of a tile's own diagonal values: x = x * c + dist[key - query]; d points at the entry of (accumulator row 0, this lane's query)
-template <int NT, int SIGN> __device__ __forceinline__ void add_near_bias(f32x16 (&x)[NT], float c, const float* d) {
+// Where a tile's scores start: from their diagonals' bias; d points at the entry of (accumulator row 0, this lane's column)
+template <int NT, int SIGN> __device__ __forceinline__ void start_near(f32x16 (&x)[NT], const float* d) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] = fmaf(x[t][e], c, d[SIGN * (t * 32 + (e & 3) + 8 * (e >> 2))]);
+        for (int e = 0; e < 16; ++e) x[t][e] = d[SIGN * (t * 32 + (e & 3) + 8 * (e >> 2))];
 }
+// A tile's distances lo .. hi: all at or past -maxd / maxd (one bias for the whole tile), or near
+enum { FAR_LO = -1, NEAR = 0, FAR_HI = 1 };
+__device__ __forceinline__ int place_of(int lo, int hi, int maxd) { return hi <= -maxd ? FAR_LO : lo >= maxd ? FAR_HI : NEAR; }
 // keeps rows <= lim (rows counted from the tile's first, lim already less 4 * (lane >> 5))
 template <int NT> __device__ __forceinline__ void mask_rows(f32x16 (&x)[NT], int lim, float with) {
 #pragma unroll
@@ -342,13 +344,14 @@ __device__ __forceinline__ QTile q_tile_of(const PAttnArgs& a) {
     const int p = blockIdx.x % a.hq, ti = blockIdx.x / a.hq;
     t.kvh = p % a.hkv;
     t.head = t.kvh * (a.hq / a.hkv) + p / a.hkv;
-    t.seq = a.tiles[2 * ti];
-    t.q0 = a.tiles[2 * ti + 1];
-    t.q_len = a.q_len[t.seq];
-    t.k_len = max(0, min(a.k_len[t.seq], a.k_cap[t.seq]));
+    const int* rec = a.tiles + 8 * (long)ti;               // one load for all that is fixed: the chain to the first key row is two loads long
+    t.seq = rec[0];
+    t.q0 = rec[1];
+    t.q_row = rec[2];
+    t.q_len = rec[3];
+    t.k_row = rec[4];
+    t.k_len = max(0, min(a.k_len[t.seq], rec[5]));
     t.off = t.k_len - t.q_len;
-    t.q_row = a.q_start[t.seq];
-    t.k_row = a.k_start[t.seq];
     t.nk = a.causal ? max(0, min(t.k_len, t.q0 + TILE + t.off)) : t.k_len;
     return t;
 }
@@ -386,7 +389,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
     const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;   // every query of the wave sees keys up to here,
     const int wlim1 = w.q0 + wave * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;     // none sees one past here
     float far_lo = 0.f, far_hi = 0.f;
-    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, w.head); far_hi = bias_at(a, a.maxd, w.head); }
+    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, w.head) * LOG2E; far_hi = bias_at(a, a.maxd, w.head) * LOG2E; }
     Softmax<DP> sm;
     sm.init();
     for (int i = 0; i < nt; ++i) {
@@ -401,19 +404,18 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
         const typename I::Lane im = I::at(im0, lds0 + (i & 1) * 2 * TB);
         f32x16 st[2];
         zero_acc(st);
+        float off = 0.f;
+        if constexpr (BIAS) {
+            const int place = place_of(k0 - (qw0 + WR - 1), k0 + KT - 1 - qw0, a.maxd);
+            if (place == NEAR) start_near<2, 1>(st, dist + (k0 + 4 * h2 - qpos + a.maxd + NEAR_PAD));
+            else off = place < 0 ? far_lo : far_hi;
+        }
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
             for (int t = 0; t < 2; ++t) I::M::mma(I::row_frag(im, t, kk), fq[kk], st[t]);
-        float c = a.c, off = 0.f;
-        if constexpr (BIAS) {
-            const int lo = k0 - (qw0 + WR - 1), hi = k0 + KT - 1 - qw0;      // the tile's smallest and largest distance
-            if (hi <= -a.maxd) off = far_lo;
-            else if (lo >= a.maxd) off = far_hi;
-            else { add_near_bias<2, 1>(st, c, dist + (k0 + 4 * h2 - qpos + a.maxd + NEAR_PAD)); c = 1.f; }
-        }
         if (k0 + KT - 1 > wlim0) mask_rows<2>(st, klim - k0 - 4 * h2, -__builtin_inff());
-        sm.template step<2>(st, c, off);
+        sm.template step<2>(st, a.c, off);
         acc_product<T, DP, 2>(sm.ot, st, im, 0, lane, TB);
     }
     const float l = sm.l + __shfl_xor(sm.l, 32, 64);
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
     const int off = k_len - q_len;
     if constexpr (BIAS) {
         if (kend - 1 - off > -a.maxd) {                    // some key is near some query
-            for (int i = threadIdx.x; i < a.buckets * G; i += 64 * NW) tab[i] = a.table[(long)(i / G) * a.hq + kvh * G + i % G] * LOG2E;
+            for (int i = threadIdx.x; i < a.buckets * G; i += 64 * NW) tab[i] = a.table[(long)(i / G) * a.hq + kvh * G + i % G] / a.scale;
             for (int i = threadIdx.x; i <= 2 * a.maxd; i += 64 * NW) lut[i] = (unsigned short)a.lut[i];
         }
         __syncthreads();
@@ -460,7 +462,7 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing of the compiler's stays in flight among the counted DMAs
     const int qpos = qi + off, klim = a.causal ? min(k_len - 1, qpos) : k_len - 1;
     float far_lo = 0.f, far_hi = 0.f;
-    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, kvh * G + g); far_hi = bias_at(a, a.maxd, kvh * G + g); }
+    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, kvh * G + g) * LOG2E; far_hi = bias_at(a, a.maxd, kvh * G + g) * LOG2E; }
     const char* kb = a.k + (long)a.k_start[seq] * a.sk.rs + (long)kvh * a.sk.hs;
     const char* vb = a.v + (long)a.k_start[seq] * a.sv.rs + (long)kvh * a.sv.hs;
     Stream<T, DP, WR, 1> ks, vs;
@@ -488,25 +490,19 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
         const typename I::Lane im = I::at(im0, lds0 + par * 2 * BB);
         f32x16 st[1];
         zero_acc(st);
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) I::M::mma(I::row_frag(im, 0, kk), fq[kk], st[0]);
-        float c = a.c, o = 0.f;
+        float o = 0.f;
         if constexpr (BIAS) {
-            const int lo = k0 - (k_len - 1), hi = min(k0 + WR, kend) - 1 - off;      // over every query of the recording
-            if (hi <= -a.maxd) o = far_lo;
-            else if (lo >= a.maxd) o = far_hi;
-            else {
+            const int place = place_of(k0 - (k_len - 1), min(k0 + WR, kend) - 1 - off, a.maxd);      // over every query of the recording
+            if (place == NEAR) {
                 const int base = k0 + 4 * h2 - qpos + a.maxd;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int i = max(0, min(2 * a.maxd, base + (e & 3) + 8 * (e >> 2)));
-                    st[0][e] = fmaf(st[0][e], c, tab[lut[i] * G + g]);
-                }
-                c = 1.f;
-            }
+                for (int e = 0; e < 16; ++e) st[0][e] = tab[lut[max(0, min(2 * a.maxd, base + (e & 3) + 8 * (e >> 2)))] * G + g];
+            } else o = place < 0 ? far_lo : far_hi;
         }
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) I::M::mma(I::row_frag(im, 0, kk), fq[kk], st[0]);
         if (a.causal ? k0 + WR - 1 > min(k_len - 1, off) || k0 + WR > kend : k0 + WR > kend) mask_rows<1>(st, min(klim, kend - 1) - k0 - 4 * h2, -__builtin_inff());
-        sm.template step<1>(st, c, o);
+        sm.template step<1>(st, a.c, o);
         acc_product<T, DP, 1>(sm.ot, st, im, 0, lane, BB);
     }
     // join the waves
@@ -652,8 +648,9 @@ __device__ __forceinline__ void add_diagonals(unsigned m, unsigned h, const f32x
 // (f32 heads of 128 with the table: two buffers and the sums for 1024 distances would not fit 160 KB, so that variant has one buffer)
 template <typename T, int DP, int MODE> constexpr int dq_buffers() { return sizeof(T) == 4 && DP == 128 && MODE == DQ_TABLE ? 1 : 2; }
 // dq (and the table's gradient), tiled like the forward; DELTA: only delta = sum_j P dP
+// (and its LDS leaves room for one workgroup per CU at heads of 128 anyway: the whole register file instead of spills)
 template <typename T, int DP, bool BIAS, int MODE>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq_kernel(PAttnArgs a) {
+__global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per_simd<T, DP>())) void packed_attn_dq_kernel(PAttnArgs a) {
     using I = Image<T, DP>;
     constexpr int TB = KT * I::RB, NB = dq_buffers<T, DP, MODE>();
     constexpr bool TIGHT = DP == 128;
@@ -697,9 +694,11 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
     const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;
     const int wlim1 = w.q0 + wave * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;
     float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f;
-    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, w.head); far_hi = bias_at(a, a.maxd, w.head); }
-    f32x16 dq[DP / 32];
+    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, w.head) * LOG2E; far_hi = bias_at(a, a.maxd, w.head) * LOG2E; }
+    f32x16 dq[DP / 32], start;
     zero_acc(dq);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) start[e] = MODE == DELTA ? 0.f : -dl;
     for (int i = 0; i < nt; ++i) {
         const int k0 = i * KT;
         PA_SYNC_TILE();
@@ -717,7 +716,15 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
         const typename I::Lane im = I::at(im0, lds0 + (NB == 2 ? i & 1 : 0) * 2 * TB);
         f32x16 st[2], dp[2];
         zero_acc(st);
-        zero_acc(dp);
+        float off = 0.f;
+        int place = NEAR;
+        if constexpr (BIAS) {
+            place = place_of(k0 - (qw0 + WR - 1), k0 + KT - 1 - qw0, a.maxd);
+            if (place == NEAR) start_near<2, 1>(st, dist + (k0 + 4 * h2 - qpos + a.maxd + NEAR_PAD));
+            else off = place < 0 ? far_lo : far_hi;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) dp[t] = start;          // dP - delta: the product starts from -delta of the lane's query
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
@@ -726,27 +733,18 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
                 I::M::mma(I::row_frag(im, t, kk, TB), fo[kk], dp[t]);
                 if (t) pace<TIGHT>();
             }
-        float c = a.c, off = 0.f;
-        int where = 0;                       // of the tile's distances: -1 / 1 all at or past -maxd / maxd, 0 near
-        const int di = k0 + 4 * h2 - qpos + a.maxd + NEAR_PAD;
-        if constexpr (BIAS) {
-            const int lo = k0 - (qw0 + WR - 1), hi = k0 + KT - 1 - qw0;
-            if (hi <= -a.maxd) { off = far_lo; where = -1; }
-            else if (lo >= a.maxd) { off = far_hi; where = 1; }
-            else { add_near_bias<2, 1>(st, c, dist + di); c = 1.f; }
-        }
         if (k0 + KT - 1 > wlim0) mask_rows<2>(st, klim - k0 - 4 * h2, -__builtin_inff());
         const float sub = off - lse2;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e], c, sub));
+                const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e], a.c, sub));
                 if constexpr (MODE == DELTA) dl = fmaf(p, dp[t][e], dl);
-                else st[t][e] = p * (dp[t][e] - dl);
+                else st[t][e] = p * dp[t][e];
             }
         if constexpr (MODE == DQ_TABLE) {
-            if (where == 0) {
+            if (place == NEAR) {
                 add_diagonals(diag + wave * DIAG * 4, lds_addr(hist) + (wave * ndist + k0 - qw0 + a.maxd + NEAR_PAD) * 4, st, lane);
             } else {
                 float s = 0.f;
@@ -754,7 +752,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s += st[t][e];
-                if (where < 0) sum_lo += s; else sum_hi += s;
+                if (place < 0) sum_lo += s; else sum_hi += s;
             }
         }
         if constexpr (MODE != DELTA) acc_product<T, DP, 2, TIGHT>(dq, st, im, 0, lane, 0);
@@ -776,16 +774,17 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dq
         }
         __syncthreads();
         float* part = a.part + ((long)(blockIdx.x / a.hq) * a.hq + w.head) * a.buckets;
-        for (int b = threadIdx.x; b < a.buckets; b += 256) {
-            const int first = a.ranges[2 * b], last = a.ranges[2 * b + 1];      // distances of the bucket; none: first > last
+        for (int b = threadIdx.x >> 4; b < a.buckets; b += 16) {            // 16 lanes a bucket
+            const int first = a.ranges[2 * b], last = a.ranges[2 * b + 1], l16 = threadIdx.x & 15;      // distances of the bucket; none: first > last
             float s = 0.f;
             if (first <= last) {
                 const int i0 = first <= -a.maxd ? 0 : first + a.maxd + NEAR_PAD, i1 = last >= a.maxd ? ndist - 1 : last + a.maxd + NEAR_PAD;
-                if (first <= -a.maxd) s += far[0] + far[2] + far[4] + far[6];
-                if (last >= a.maxd) s += far[1] + far[3] + far[5] + far[7];
-                for (int i = i0; i <= i1; ++i) s += dist[i];
+                if (l16 < 4 && first <= -a.maxd) s += far[2 * l16];
+                if (l16 < 4 && last >= a.maxd) s += far[2 * l16 + 1];
+                for (int i = i0 + l16; i <= i1; i += 16) s += dist[i];
             }
-            part[b] = s;
+            s = group_sum<16>(s);
+            if (l16 == 0) part[b] = s;
         }
     }
 }
@@ -823,8 +822,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
     float* stat = (float*)(smem + 4 * TB);
     float* dist = stat + 4 * KT;
     const int kvh = blockIdx.x % a.hkv, rest = blockIdx.x / a.hkv, split = rest % a.nsplit, ti = rest / a.nsplit;
-    const int seq = a.tiles[2 * ti], kt0 = a.tiles[2 * ti + 1];
-    const int q_len = a.q_len[seq], k_cap = a.k_cap[seq], k_len = max(0, min(a.k_len[seq], k_cap)), off = k_len - q_len, G = a.hq / a.hkv;
+    const int* rec = a.tiles + 8 * (long)ti;
+    const int seq = rec[0], kt0 = rec[1], q_row = rec[2], q_len = rec[3], k_row = rec[4], k_cap = rec[5];
+    const int k_len = max(0, min(a.k_len[seq], k_cap)), off = k_len - q_len, G = a.hq / a.hkv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
     const int kw0 = kt0 + wave * WR, key = kw0 + r;
     f32x16 dk[DP / 32], dv[DP / 32];
@@ -838,7 +838,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
     if (i0 < i1) {
         typename I::Frag fk[DP / 16], fv[DP / 16];
         {
-            const long kr = (long)a.k_start[seq] + min(key, k_len - 1);
+            const long kr = (long)k_row + min(key, k_len - 1);
             const char* krp = a.k + kr * a.sk.rs + (long)kvh * a.sk.hs;
             const char* vrp = a.v + kr * a.sv.rs + (long)kvh * a.sv.hs;
 #pragma unroll
@@ -852,7 +852,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
         float reg = 0.f;                                   // threads 0..63: lse of the next tile, 64..127: -delta
         auto fetch = [&](int it, unsigned dst) {
             const int g = it / per, q0 = qfirst + (it - g * per) * KT, head = kvh * G + g;
-            const long row = (long)a.q_start[seq] + q0;
+            const long row = (long)q_row + q0;
             if (threadIdx.x < 2 * KT) {
                 const int j = threadIdx.x & (KT - 1);
                 const bool in = q0 + j < q_len;
@@ -877,12 +877,12 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
                     if (held >= 0) __syncthreads();
                     held = g;
                     dist_fill(dist, a, kvh * G + g, 256);
-                    far_lo = bias_at(a, -a.maxd, kvh * G + g);
-                    far_hi = bias_at(a, a.maxd, kvh * G + g);
+                    far_lo = bias_at(a, -a.maxd, kvh * G + g) * LOG2E;
+                    far_hi = bias_at(a, a.maxd, kvh * G + g) * LOG2E;
                 }
             }
             PA_SYNC_TILE();
-            I::move(im, par ? 2 * TB : -2 * TB);
+            I::template move<TIGHT>(im, par ? 2 * TB : -2 * TB);
             if (it + 1 < i1) fetch(it + 1, lds0 + (par ^ 1) * 2 * TB);
             const int qp0 = q0 + off;                      // position of the tile's first query
             if (kw0 >= k_len || (a.causal && qp0 + KT - 1 < kw0)) continue;
@@ -890,6 +890,13 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
             for (int t = 0; t < 2; ++t) {
                 f32x16 s[1], dp[1];
                 zero_acc(s);
+                float bo = 0.f;
+                const int qt0 = qp0 + t * 32;
+                if constexpr (BIAS) {
+                    const int place = place_of(kw0 - (qt0 + 31), kw0 + WR - 1 - qt0, a.maxd);
+                    if (place == NEAR) start_near<1, -1>(s, dist + (key - qt0 - 4 * h2 + a.maxd + NEAR_PAD));
+                    else bo = place < 0 ? far_lo : far_hi;
+                }
 #pragma unroll
                 for (int gq = 0; gq < 4; ++gq) {           // dP - delta: the product starts from -delta of the row's query
                     const f32x4 dl = *(const f32x4*)(ls + KT + t * 32 + 8 * gq + 4 * h2);
@@ -901,14 +908,6 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
                     I::M::mma(I::row_frag(im, t, kk), fk[kk], s[0]);      // rows = queries, lanes = keys
                     I::M::mma(I::row_frag(im, t, kk, TB), fv[kk], dp[0]);
                     if (kk & 1) pace<TIGHT>();
-                }
-                float c = a.c, bo = 0.f;
-                const int qt0 = qp0 + t * 32;
-                if constexpr (BIAS) {
-                    const int lo = kw0 - (qt0 + 31), hi = kw0 + WR - 1 - qt0;
-                    if (hi <= -a.maxd) bo = far_lo;
-                    else if (lo >= a.maxd) bo = far_hi;
-                    else { add_near_bias<1, -1>(s, c, dist + (key - qt0 - 4 * h2 + a.maxd + NEAR_PAD)); c = 1.f; }
                 }
                 if (kw0 + WR > k_len || (a.causal && qt0 < kw0 + WR - 1)) {            // some pair is masked: keep key < k_len and query >= key
 #pragma unroll
@@ -923,7 +922,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int e = 4 * gq + i;
-                        const float p = __builtin_amdgcn_exp2f(fmaf(s[0][e], c, bo - lv[i]));
+                        const float p = __builtin_amdgcn_exp2f(fmaf(s[0][e], a.c, bo - lv[i]));
                         s[0][e] = p;
                         dp[0][e] *= p;
                     }
@@ -936,7 +935,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
     int own = lane;                                        // found again here: nothing of the outputs' addresses lives through the loop
     asm volatile("" : "+v"(own));
     const int orow = wave * WR + (own & 31), okey = kt0 + orow, oh = own >> 5;
-    const long krow = (long)a.k_start[seq] + min(okey, k_cap - 1);
+    const long krow = (long)k_row + min(okey, k_cap - 1);
     const bool live = okey < k_cap;                        // rows between a recording's length and its capacity get zeros
     if (ns == 1) {
         store_rows<T, DP>(a.dk + krow * a.sdk.rs + (long)kvh * a.sdk.hs, live, dk, a.scale, a.D, oh);
@@ -949,8 +948,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
 }
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(PAttnArgs a) {
-    const int kvh = blockIdx.x % a.hkv, ti = blockIdx.x / a.hkv, seq = a.tiles[2 * ti], kt0 = a.tiles[2 * ti + 1];
-    const int rows = min(TILE, a.k_cap[seq] - kt0), q_len = a.q_len[seq], k_len = max(0, min(a.k_len[seq], a.k_cap[seq]));
+    const int kvh = blockIdx.x % a.hkv, ti = blockIdx.x / a.hkv;
+    const int* rec = a.tiles + 8 * (long)ti;
+    const int kt0 = rec[1], q_len = rec[3], rows = min(TILE, rec[5] - kt0), k_len = max(0, min(a.k_len[rec[0]], rec[5]));
     const int qfirst = dkv_first(a, kt0, q_len, k_len), per = qfirst < q_len ? (q_len - qfirst + KT - 1) / KT : 0;
     const int ns = dkv_parts(per * (a.hq / a.hkv), a.nsplit, a.chunk);
     if (ns == 1) return;
@@ -966,7 +966,7 @@ __global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(PAttnArgs a) 
             for (int k = 0; k < 8; ++k) s[k] += y[k];
         }
         const Strides st = which ? a.sdv : a.sdk;
-        store8<T>((T*)((which ? a.dv : a.dk) + ((long)a.k_start[seq] + kt0 + row) * st.rs + (long)kvh * st.hs) + d, s);
+        store8<T>((T*)((which ? a.dv : a.dk) + ((long)rec[4] + kt0 + row) * st.rs + (long)kvh * st.hs) + d, s);
     }
 }
 
@@ -1009,16 +1009,18 @@ int few_chunk(const Plan& p, int hkv) {
     return (int)(c < 256 ? 256 : c > 8192 ? 8192 : c);
 }
 int few_splits(const Plan& p, int hkv) { const int c = few_chunk(p, hkv); return p.max_k > c ? (int)((p.max_k + c - 1) / c) : 1; }
-// Query tiles per workgroup of the dk/dv kernel: two workgroups fit a CU, so the whole work is cut into about 400 equal parts (a few of the
-// 512 places stay free for the tiles' odd ends) where the key tiles alone would not fill the chip or end unevenly; below 4 tiles a part
-// would spend longer on its f32 partials than on its tiles.
-int dkv_chunk(const Plan& p, int hq, int hkv, int causal) {
+// Query tiles per workgroup of the dk/dv kernel: the whole work is cut into equal parts where the key tiles alone would not fill the chip or end
+// unevenly. Heads above 64: two workgroups fit a CU, 400 parts (a few of the 512 places stay free for the tiles' odd ends; 1 x 8191, 16/2
+// heads of 128, forward + backward: 256 parts 1677 us, 400 1361, 512 1660, 1024 1685). Smaller heads: three fit and a tile takes half as
+// long, 700 parts (12 x 100-1200, 16/4 heads of 64: 256 parts 254 us, 400 279, 768 256, 1536 280). Below 4 tiles a part would
+// spend longer on its f32 partials than on its tiles.
+int dkv_chunk(const Plan& p, int hq, int D, int causal) {
     const long work = (causal ? p.k_work_causal : p.k_work) * hq;
-    const long c = (work + 399) / 400;
+    const long parts = D > 64 ? 400 : 700, c = (work + parts - 1) / parts;
     return (int)(c < 4 ? 4 : c > (1 << 20) ? 1 << 20 : c);
 }
-int dkv_splits(const Plan& p, int hq, int hkv, int causal) {
-    const long longest = (p.max_q + KT - 1) / KT * (hq / hkv), c = dkv_chunk(p, hq, hkv, causal);
+int dkv_splits(const Plan& p, int hq, int hkv, int D, int causal) {
+    const long longest = (p.max_q + KT - 1) / KT * (hq / hkv), c = dkv_chunk(p, hq, D, causal);
     return longest > c ? (int)((longest + c - 1) / c) : 1;
 }
 bool delta_pass(int dtype, bool table_grad) { return table_grad && dtype == PSELD_BF16; }
@@ -1095,8 +1097,8 @@ int run_bwd(PAttnArgs& a, const Plan& p, float* dtable, int accumulate, hipStrea
     }
     if (!table_done) PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ>), p.q_tiles * a.hq, 256, 4 * TB + nd, a);
     a.tiles = a.causal ? p.k_tile_causal : p.k_tile;
-    a.nsplit = dkv_splits(p, a.hq, a.hkv, a.causal);
-    a.chunk = dkv_chunk(p, a.hq, a.hkv, a.causal);
+    a.nsplit = dkv_splits(p, a.hq, a.hkv, a.D, a.causal);
+    a.chunk = dkv_chunk(p, a.hq, a.D, a.causal);
     PA_LAUNCH((packed_attn_dkv_kernel<T, DP, BIAS>), p.k_tiles * a.hkv * a.nsplit, 256, 4 * TB + 4 * KT * 4 + nd, a);
     if (a.nsplit > 1) PA_LAUNCH((packed_attn_dkv_join_kernel<T, DP>), p.k_tiles * a.hkv, 256, 0, a);
     return PSELD_OK;
@@ -1154,7 +1156,7 @@ extern "C" int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, co
 extern "C" long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int causal, int buckets) {
     if (!plan || hkv <= 0 || hq < hkv || hq % hkv) return 0;
     const Plan p = plan_of(plan);
-    const long n = dkv_splits(p, hq, hkv, causal);
+    const long n = dkv_splits(p, hq, hkv, D, causal);
     return ((p.rows * hq + 3) / 4 * 4 + p.q_tiles * hq * buckets + 4 + (n > 1 ? p.k_tiles * hkv * n * 2 * TILE * pad_of(D) : 0)) * (long)sizeof(float);
 }
 

@@ -1608,7 +1608,7 @@ class PackedPlan:
         host, at = [], {}
 
         def put(name, values):
-            host.extend([0] * (-len(host) % 4))
+            host.extend([0] * (-len(host) % 8))
             at[name] = len(host)
             host.extend(values)
 
@@ -1618,9 +1618,10 @@ class PackedPlan:
                 out.append(n)
                 n += x
             return out
-        put('q_start', starts(q_lens)); put('q_len', q_lens); put('k_start', starts(caps)); put('k_cap', caps); put('k_len', k_lens)
+        qs, ks = starts(q_lens), starts(caps)
+        put('q_start', qs); put('q_len', q_lens); put('k_start', ks); put('k_cap', caps); put('k_len', k_lens)
         for name, tiles in (('q_tile', qf), ('q_tile_causal', qc), ('k_tile', kf), ('k_tile_causal', kc)):
-            put(name, [x for _, s, r in sorted(tiles) for x in (s, r)])
+            put(name, [x for _, s, r in sorted(tiles) for x in (s, r, qs[s], q_lens[s], ks[s], caps[s], 0, 0)])
         self._ints = torch.tensor(host, dtype=torch.int32).to(self.device)
         self._ptr = {k: self._ints.data_ptr() + 4 * v for k, v in at.items()}
         self.k_len = self._ints[at['k_len']:at['k_len'] + self.seqs]
