@@ -490,7 +490,7 @@ int pseld_gru_gate_bwd(int dtype, const void* dh, long dh_stride, const void* ca
  * z = sigmoid(g), h_t = z_t h_{t-1} + (1 - z_t) n_t per channel: nn.GRU's update rule (model_utilities.py:249-252) without the recurrent
  * product, so the frames of a recording compose in parallel. Recordings lie back to back: recording s is rows start[s] .. start[s] + len[s]
  * (device int arrays, seqs of each; rows = the sum of the lengths, max_len the longest, both host values). g, n, h rows at strides ldg, ldn, ldh
- * (multiples of 4 elements, addresses on 4-element boundaries), C a multiple of 8. reverse: every recording runs from its last row to its first.
+ * (multiples of 4 elements below 2^23, addresses on 4-element boundaries), C a multiple of 8. reverse: every recording runs from its last row to its first.
  * h0 [seqs, C] (NULL: zeros) -> h and h_last [seqs, C] (= h0 for an empty recording). states: f32 [pseld_linrec_states(rows, seqs), C], what the
  * backward needs besides g and n (NULL: not wanted). bwd: dh, dh_last (NULL: zeros) -> dg, dn, dh0 (NULL: not wanted). All state
  * arrays are f32. workspace: pseld_linrec_workspace bytes (0: none needed). Deterministic. */

@@ -18,11 +18,12 @@
 // segment length is the shortest that still gives about SEG_WGS workgroups, and one segment (one launch) where the batch fills the chip.
 // States, sums and compositions are f32; h, dg, dn are rounded once to the operands' type on their way out.
 #include "common.h"
+#include <stdlib.h>
 
 namespace {
 
-constexpr int TILE = 128;        // frames per tile: 16 thread groups x 8 frames
-constexpr int R = 8;             // frames per thread
+constexpr int TILE = 64;         // frames per tile: 16 thread groups x 4 frames
+constexpr int R = 4;             // frames per thread
 constexpr int SLAB = 64;         // channels per workgroup: 16 lanes x 4
 constexpr int SEG_WGS = 1024;    // four workgroups per CU
 
@@ -38,6 +39,7 @@ struct LinrecArgs {
     float* agg;               // [rows / seg_len + seqs + 1, 2, C]
     const int* start; const int* len;
     int seqs, C, slabs, nseg, seg_len, reverse;
+    int descending;           // workgroups take the segments last to first
 };
 
 template <typename T> struct Quad;
@@ -49,24 +51,20 @@ template <> struct Quad<float> {
     f32x4 v;
     __device__ __forceinline__ float get(int i) const { return v[i]; }
 };
-template <typename T> __device__ __forceinline__ Quad<T> zero_quad() {
-    Quad<T> q;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = (T)0.f;
-    return q;
-}
 template <typename T> __device__ __forceinline__ void put_quad(T* p, const float (&x)[4]) {
     Quad<T> q;
 #pragma unroll
     for (int i = 0; i < 4; ++i) q.v[i] = (T)x[i];
     *(decltype(q.v)*)p = q.v;
 }
-// z = sigmoid(g) and 1 - z, neither by cancellation: e = exp(-|g|), 1 / (1 + e) and e / (1 + e)
+// z = sigmoid(g) = 1 / (1 + e) and 1 - z = e / (1 + e) with e = exp(-g): neither by cancellation. e is held below 2^115, so that e / (1 + e) stays 1
+// where exp(-g) would overflow (a NaN stays one)
 __device__ __forceinline__ void gate_of(float g, float& z, float& y) {
-    const float e = __expf(-fabsf(g));
-    const float big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;
-    z = g >= 0.f ? big : small;
-    y = g >= 0.f ? small : big;
+    float x = g * -1.4426950408889634f;
+    x = x > 115.f ? 115.f : x;
+    const float e = __builtin_amdgcn_exp2f(x);
+    z = __builtin_amdgcn_rcpf(1.f + e);
+    y = e * z;
 }
 
 struct Place {       // which recording, segment and channels a workgroup owns, and which frames and channels a thread does
@@ -76,7 +74,7 @@ struct Place {       // which recording, segment and channels a workgroup owns, 
 };
 __device__ __forceinline__ Place place_of(const LinrecArgs& a) {
     Place p;
-    const int slab = blockIdx.x % a.slabs, rest = blockIdx.x / a.slabs;
+    const int slab = blockIdx.x % a.slabs, at = blockIdx.x / a.slabs, rest = a.descending ? a.seqs * a.nseg - 1 - at : at;
     p.seg = rest % a.nseg;
     p.seq = rest / a.nseg;
     p.len = a.len[p.seq];
@@ -91,17 +89,37 @@ __device__ __forceinline__ Place place_of(const LinrecArgs& a) {
     p.live = p.c < a.C;
     return p;
 }
-__device__ __forceinline__ long row_of(const LinrecArgs& a, const Place& p, int t) { return p.row0 + (a.reverse ? p.len - 1 - t : t); }
-
-// the thread's 8 frames t .. t + 7 of one operand; frames past the segment and channels past C are never addressed
-template <typename T>
-__device__ __forceinline__ void fetch(Quad<T> (&q)[R], const void* base, long ld, const LinrecArgs& a, const Place& p, int t) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        if (p.live && t + i < p.t_end) q[i].v = *(const decltype(q[i].v)*)((const T*)base + row_of(a, p, t + i) * ld + p.c);
-        else q[i] = zero_quad<T>();
+// An operand's rows of one tile: a uniform base (the tile's lowest row in memory) and 32-bit offsets per lane that are the same for every tile. Rows
+// step up with time, down when reverse. Loads are unconditional - rows past the segment repeat its last one, channels past C the last four, and
+// the values are dropped later - so that nothing has to merge behind a request and wait for it.
+template <typename T> struct Rows {
+    char* base;                // row0 of the recording
+    long ld;                   // bytes per row
+    unsigned first, chan;      // bytes from a tile's lowest row to the thread's first frame; of its channels
+    int step;                  // bytes from one frame's row to the next
+    __device__ __forceinline__ Rows(const void* p0, long ld_, const LinrecArgs& a, const Place& p) {
+        ld = ld_ * (long)sizeof(T);
+        base = (char*)p0 + p.row0 * ld;
+        first = (a.reverse ? TILE - 1 - p.tg * R : p.tg * R) * (unsigned)ld;
+        chan = min(p.c, a.C - 4) * (unsigned)sizeof(T);
+        step = a.reverse ? -(int)ld : (int)ld;
     }
-}
+    __device__ __forceinline__ char* tile(const LinrecArgs& a, const Place& p, int t0) const {
+        return base + (long)(a.reverse ? p.len - t0 - TILE : t0) * ld;
+    }
+    __device__ __forceinline__ char* row(char* tile_base, int i) const { return tile_base + (first + (unsigned)(i * step) + chan); }
+    __device__ __forceinline__ void fetch(Quad<T> (&q)[R], const LinrecArgs& a, const Place& p, int t0) const {
+        char* b = tile(a, p, t0);
+        const int live = min(TILE, p.t_end - t0);          // frames of the tile that exist
+        const unsigned lo = a.reverse ? (unsigned)(TILE - live) * (unsigned)ld : 0u, hi = a.reverse ? (TILE - 1) * (unsigned)ld : (unsigned)(live - 1) * (unsigned)ld;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const unsigned o = max(lo, min(hi, first + (unsigned)(i * step)));
+            q[i].v = *(const decltype(q[i].v)*)(b + (o + chan));
+        }
+    }
+};
+
 // lanes `from` lanes below / above hold the neighbouring thread groups of the same channels
 __device__ __forceinline__ float from_lane(float v, int lane) { return __shfl(v, lane, 64); }
 
@@ -133,12 +151,15 @@ __global__ __launch_bounds__(256) void linrec_fwd_kernel(LinrecArgs a) {
             for (int i = 0; i < 4; ++i) carry[i] = fmaf(A[i], carry[i], B[i]);
         }
     }
+    const Rows<T> rg(a.g, a.ldg, a, p), rn(a.n, a.ldn, a, p), rh(a.h, a.ldh, a, p);
     Quad<T> qg[R], qn[R];
-    fetch<T>(qg, a.g, a.ldg, a, p, p.t0 + p.tg * R);
-    fetch<T>(qn, a.n, a.ldn, a, p, p.t0 + p.tg * R);
+    rg.fetch(qg, a, p, p.t0);
+    rn.fetch(qn, a, p, p.t0);
+    const int last = p.t0 + (p.t_end - 1 - p.t0) / TILE * TILE;
     int par = 0;
     for (int t0 = p.t0; t0 < p.t_end; t0 += TILE, par ^= 1) {
         const int t = t0 + p.tg * R;
+        const bool whole = t0 + TILE <= p.t_end;
         float z[R][4], b[R][4], A[4], B[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) { A[c] = 1.f; B[c] = 0.f; }
@@ -149,12 +170,22 @@ __global__ __launch_bounds__(256) void linrec_fwd_kernel(LinrecArgs a) {
                 float y;
                 gate_of(qg[i].get(c), z[i][c], y);
                 b[i][c] = y * qn[i].get(c);
-                if (t + i >= p.t_end) { z[i][c] = 1.f; b[i][c] = 0.f; }
+            }
+        if (!whole)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (t + i >= p.t_end)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) { z[i][c] = 1.f; b[i][c] = 0.f; }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
                 A[c] *= z[i][c];
                 B[c] = fmaf(z[i][c], B[c], b[i][c]);
             }
-        fetch<T>(qg, a.g, a.ldg, a, p, t + TILE);
-        fetch<T>(qn, a.n, a.ldn, a, p, t + TILE);
+        rg.fetch(qg, a, p, min(t0 + TILE, last));
+        rn.fetch(qn, a, p, min(t0 + TILE, last));
         // inclusive composition over the wave's four thread groups
 #pragma unroll
         for (int o = 16; o <= 32; o <<= 1)
@@ -185,15 +216,15 @@ __global__ __launch_bounds__(256) void linrec_fwd_kernel(LinrecArgs a) {
                 const float ea = from_lane(A[c], lane - 16), eb = from_lane(B[c], lane - 16);
                 x[c] = p.tgl ? fmaf(ea, in[c], eb) : in[c];
             }
+            char* hb = rh.tile(a, p, t0);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) x[c] = fmaf(z[i][c], x[c], b[i][c]);
-                if (p.live && t + i < p.t_end) {
-                    put_quad<T>((T*)a.h + row_of(a, p, t + i) * a.ldh + p.c, x);
-                    if (t + i == p.len - 1) *(f32x4*)(a.h_last + (long)p.seq * a.C + p.c) = f32x4{x[0], x[1], x[2], x[3]};
-                }
+                if (p.live && (whole || t + i < p.t_end)) put_quad<T>((T*)rh.row(hb, i), x);
             }
+            // frames past the end leave the state alone: the last thread's is the recording's
+            if (t0 + TILE >= p.len && p.live && p.tg == 15) *(f32x4*)(a.h_last + (long)p.seq * a.C + p.c) = f32x4{x[0], x[1], x[2], x[3]};
         }
     }
     if (AGG && p.tg == 0 && p.live) {
@@ -234,15 +265,19 @@ __global__ __launch_bounds__(256) void linrec_bwd_kernel(LinrecArgs a) {
     }
     Quad<T> qg[R], qn[R], qd[R];
     const int last = p.t0 + (p.t_end - 1 - p.t0) / TILE * TILE;
-    fetch<T>(qg, a.g, a.ldg, a, p, last + p.tg * R);
-    if constexpr (!AGG) fetch<T>(qn, a.n, a.ldn, a, p, last + p.tg * R);
-    fetch<T>(qd, a.dh, a.lddh, a, p, last + p.tg * R);
+    const Rows<T> rg(a.g, a.ldg, a, p), rn(a.n, a.ldn, a, p), rd(a.dh, a.lddh, a, p), og(a.dg, a.lddg, a, p), on(a.dn, a.lddn, a, p);
+    rg.fetch(qg, a, p, last);
+    if constexpr (!AGG) rn.fetch(qn, a, p, last);
+    rd.fetch(qd, a, p, last);
+    const float* states = AGG ? nullptr : a.states + (p.row0 / TILE + p.seq) * a.C + min(p.c, a.C - 4);
+    f32x4 nst = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (!AGG) nst = *(const f32x4*)(states + (long)(last / TILE) * a.C);
     int par = 0;
     for (int t0 = last; t0 >= p.t0; t0 -= TILE, par ^= 1) {
         const int t = t0 + p.tg * R;
+        const bool whole = t0 + TILE <= p.t_end;
         float z[R][4], y[R][4], n[R][4], d[R][4], A[4], B[4], M[4];
-        f32x4 st = {0.f, 0.f, 0.f, 0.f};
-        if (!AGG && p.live) st = *(const f32x4*)(a.states + (p.row0 / TILE + p.seq + t0 / TILE) * a.C + p.c);
+        const f32x4 st = nst;                             // the state before the tile
 #pragma unroll
         for (int c = 0; c < 4; ++c) { A[c] = 1.f; B[c] = 0.f; M[c] = 0.f; }
 #pragma unroll
@@ -250,9 +285,19 @@ __global__ __launch_bounds__(256) void linrec_bwd_kernel(LinrecArgs a) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 gate_of(qg[i].get(c), z[i][c], y[i][c]);
-                d[i][c] = qd[i].get(c);                  // zero past the segment
+                d[i][c] = qd[i].get(c);
                 if constexpr (!AGG) n[i][c] = qn[i].get(c);
-                if (t + i >= p.t_end) { z[i][c] = 1.f; y[i][c] = 0.f; }
+            }
+        if (!whole)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (t + i >= p.t_end)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) { z[i][c] = 1.f; y[i][c] = 0.f; d[i][c] = 0.f; }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
                 A[c] *= z[i][c];
                 if constexpr (!AGG) B[c] = fmaf(z[i][c], B[c], y[i][c] * n[i][c]);
             }
@@ -260,11 +305,11 @@ __global__ __launch_bounds__(256) void linrec_bwd_kernel(LinrecArgs a) {
         for (int i = R - 1; i >= 0; --i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) M[c] = z[i][c] * (d[i][c] + M[c]);
-        if (t0 > p.t0) {
-            fetch<T>(qg, a.g, a.ldg, a, p, t - TILE);
-            if constexpr (!AGG) fetch<T>(qn, a.n, a.ldn, a, p, t - TILE);
-            fetch<T>(qd, a.dh, a.lddh, a, p, t - TILE);
-        }
+        const int next = max(t0 - TILE, p.t0);
+        rg.fetch(qg, a, p, next);
+        if constexpr (!AGG) rn.fetch(qn, a, p, next);
+        rd.fetch(qd, a, p, next);
+        if constexpr (!AGG) nst = *(const f32x4*)(states + (long)(next / TILE) * a.C);
         // inclusive compositions over the wave's thread groups: the states from the first group on, mu from the last group back
         float S[4] = {A[0], A[1], A[2], A[3]};           // product from this group to the wave's last
 #pragma unroll
@@ -313,20 +358,20 @@ __global__ __launch_bounds__(256) void linrec_bwd_kernel(LinrecArgs a) {
             for (int i = 0; i < R; ++i)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) { hp[i][c] = x[c]; x[c] = fmaf(z[i][c], x[c], y[i][c] * n[i][c]); }
+            char *gb = og.tile(a, p, t0), *nb = on.tile(a, p, t0);
 #pragma unroll
             for (int i = R - 1; i >= 0; --i) {
-                float og[4], on[4];
+                float vg[4], vn[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const float lam = d[i][c] + m[c];
-                    on[c] = lam * y[i][c];
-                    og[c] = on[c] * z[i][c] * (hp[i][c] - n[i][c]);
+                    vn[c] = lam * y[i][c];
+                    vg[c] = vn[c] * z[i][c] * (hp[i][c] - n[i][c]);
                     m[c] = z[i][c] * lam;
                 }
-                if (p.live && t + i < p.t_end) {
-                    const long row = row_of(a, p, t + i);
-                    put_quad<T>((T*)a.dg + row * a.lddg + p.c, og);
-                    put_quad<T>((T*)a.dn + row * a.lddn + p.c, on);
+                if (p.live && (whole || t + i < p.t_end)) {
+                    put_quad<T>((T*)og.row(gb, i), vg);
+                    put_quad<T>((T*)on.row(nb, i), vn);
                 }
             }
         }
@@ -342,15 +387,16 @@ __global__ __launch_bounds__(256) void linrec_bwd_kernel(LinrecArgs a) {
     }
 }
 
-// frames per segment: whole tiles, at least two (a segment of one tile would spend as long on its neighbours as on its own frames),
-// and the whole recording where the batch gives SEG_WGS workgroups without cutting
+// Frames per segment. Cutting costs a second read of the operands, so a batch whose longest recording is at most twice an even share of the rows over
+// two workgroups per CU stays whole (32 x 200-1000 x 1024 bf16, forward + backward: whole 103 us, cut 158); otherwise about SEG_WGS segments
+// of at least four tiles.
 int seg_len_of(long rows, int max_len, int C) {
-    const long slabs = (C + SLAB - 1) / SLAB;
-    const long want = (rows * slabs + SEG_WGS - 1) / SEG_WGS;
-    const long s = (want + TILE - 1) / TILE * TILE;
-    const long whole = ((long)max_len + TILE - 1) / TILE * TILE;
-    const long got = s < 2 * TILE ? 2 * TILE : s;
-    return (int)(got > whole ? (whole > 0 ? whole : TILE) : got);
+    const long slabs = (C + SLAB - 1) / SLAB, whole = max_len > 0 ? ((long)max_len + TILE - 1) / TILE * TILE : TILE;
+    if (max_len <= 2 * (rows * slabs) / 512) return (int)whole;
+    static const long SW = getenv("LR_SEG") ? atol(getenv("LR_SEG")) : SEG_WGS;
+    long s = ((rows * slabs + SW - 1) / SW + TILE - 1) / TILE * TILE;
+    if (s < 4 * TILE) s = 4 * TILE;
+    return (int)(s < whole ? s : whole);
 }
 long agg_bytes_of(long rows, int seqs, int max_len, int C) {
     const int s = seg_len_of(rows, max_len, C);
@@ -362,9 +408,11 @@ void launch(LinrecArgs a, int backward, hipStream_t s) {
     const dim3 grid((unsigned)((long)a.slabs * a.nseg * a.seqs));
     if (!backward) {
         if (a.nseg > 1) hipLaunchKernelGGL((linrec_fwd_kernel<T, true>), grid, dim3(256), 0, s, a);
+        a.descending = a.nseg > 1;                         // what the first launch read last is still in the caches
         hipLaunchKernelGGL((linrec_fwd_kernel<T, false>), grid, dim3(256), 0, s, a);
     } else {
         if (a.nseg > 1) hipLaunchKernelGGL((linrec_bwd_kernel<T, true>), grid, dim3(256), 0, s, a);
+        a.descending = a.nseg > 1;
         hipLaunchKernelGGL((linrec_bwd_kernel<T, false>), grid, dim3(256), 0, s, a);
     }
 }
@@ -384,7 +432,7 @@ int go(const char* name, int dtype, LinrecArgs& a, long rows, int max_len, const
     PSELD_LAUNCH_CHECK(name);
     return PSELD_OK;
 }
-bool quads(const void* p, long ld, int dtype) { return ((uintptr_t)p & (dtype == PSELD_BF16 ? 7 : 15)) == 0 && (ld & 3) == 0; }
+bool quads(const void* p, long ld, int dtype) { return ((uintptr_t)p & (dtype == PSELD_BF16 ? 7 : 15)) == 0 && (ld & 3) == 0 && ld >= 0 && ld < (1l << 23); }
 
 }  // namespace
 
@@ -397,7 +445,7 @@ extern "C" int pseld_linrec_fwd(int dtype, const void* g, long ldg, const void* 
                                 float* states, const int* start, const int* len, int seqs, long rows, int max_len, int C, int reverse,
                                 float* workspace, long workspace_bytes, void* stream) {
     PSELD_CHECK_ARG(h_last && (rows == 0 || (g && n && h)), "linrec_fwd: null pointer");
-    PSELD_CHECK_ARG(quads(g, ldg, dtype) && quads(n, ldn, dtype) && quads(h, ldh, dtype), "linrec_fwd: rows must start on 4-element boundaries");
+    PSELD_CHECK_ARG(quads(g, ldg, dtype) && quads(n, ldn, dtype) && quads(h, ldh, dtype), "linrec_fwd: rows must start on 4-element boundaries, less than 2^23 elements apart");
     LinrecArgs a{};
     a.g = g; a.ldg = ldg; a.n = n; a.ldn = ldn; a.h0 = h0; a.h = h; a.ldh = ldh; a.h_last = h_last; a.states = states; a.agg = workspace;
     a.start = start; a.len = len; a.seqs = seqs; a.C = C; a.reverse = reverse;
@@ -409,7 +457,7 @@ extern "C" int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void
                                 int seqs, long rows, int max_len, int C, int reverse, float* workspace, long workspace_bytes, void* stream) {
     PSELD_CHECK_ARG(rows == 0 || (dh && g && n && dg && dn && states), "linrec_bwd: null pointer");
     PSELD_CHECK_ARG(quads(dh, lddh, dtype) && quads(g, ldg, dtype) && quads(n, ldn, dtype) && quads(dg, lddg, dtype) && quads(dn, lddn, dtype),
-                    "linrec_bwd: rows must start on 4-element boundaries");
+                    "linrec_bwd: rows must start on 4-element boundaries, less than 2^23 elements apart");
     LinrecArgs a{};
     a.dh = dh; a.lddh = lddh; a.g = g; a.ldg = ldg; a.n = n; a.ldn = ldn; a.states = const_cast<float*>(states); a.dlast = dh_last;
     a.dg = dg; a.lddg = lddg; a.dn = dn; a.lddn = lddn; a.dh0 = dh0; a.agg = workspace;

@@ -53,10 +53,13 @@ struct PAttnArgs {
 template <typename T, int DP> constexpr int waves_per_simd() { return sizeof(T) == 2 || DP == 32 ? 2 : 1; }
 
 // ---- LDS images: rows of DP elements, lane-linear, 16-byte pieces swizzled inside the row ------------------------------------------
-template <int RB> __device__ __forceinline__ int image_swizzle(int row) {
-    if constexpr (RB == 64) return (row >> 2) & 3;
-    else if constexpr (RB == 128) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
-    else return (row & 7) << 1;
+// What the XOR has to do (64 banks of 4 bytes): 16 rows that are read one 16-byte piece each (row_frag) must hit all 64 banks once, and so must 4 rows
+// that are read 64 bytes each (half a wave of col_frag). With only 8 rows and 32 bytes apart every read took half as long again.
+template <int RB, int E> __device__ __forceinline__ int image_swizzle(int row) {
+    if constexpr (RB == 64) return (row >> 2) & 3;                                             // four rows span the banks
+    else if constexpr (RB == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);           // two
+    else if constexpr (E == 2) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else return (((row >> 2) & 1) << 3) | ((row & 3) << 1) | ((row >> 3) & 1);                 // f32 columns: rows 4 apart, 128 bytes each
 }
 typedef __attribute__((address_space(3))) const char* lds_cptr;
 // A lane's reads of an image. The swizzle only XORs bits inside a row, so a lane keeps three offsets for the tile at hand and reaches every piece by
@@ -72,11 +75,11 @@ template <typename T, int DP> struct Image {
         Lane l;
         if constexpr (sizeof(T) == 2) {
             const int ra = 4 * h2 + ((lane & 15) >> 2), rb = ra + 8, p = lane & 3, ch = 2 * ((lane >> 4) & 1) + (p >> 1);
-            l.row = r * RB + ((h2 ^ image_swizzle<RB>(r)) << 4);
-            l.lo = ra * RB + ((ch ^ image_swizzle<RB>(ra)) << 4) + (p & 1) * 8;
-            l.hi = rb * RB + ((ch ^ image_swizzle<RB>(rb)) << 4) + (p & 1) * 8;
+            l.row = r * RB + ((h2 ^ image_swizzle<RB, (int)sizeof(T)>(r)) << 4);
+            l.lo = ra * RB + ((ch ^ image_swizzle<RB, (int)sizeof(T)>(ra)) << 4) + (p & 1) * 8;
+            l.hi = rb * RB + ((ch ^ image_swizzle<RB, (int)sizeof(T)>(rb)) << 4) + (p & 1) * 8;
         } else {
-            l.row = r * RB + (((2 * h2) ^ image_swizzle<RB>(r)) << 4);
+            l.row = r * RB + (((2 * h2) ^ image_swizzle<RB, (int)sizeof(T)>(r)) << 4);
             l.lo = l.hi = 0;
         }
         return l;
@@ -116,7 +119,7 @@ template <typename T, int DP> struct Image {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int row = row0 + 8 * (j >> 2) + 4 * h2 + (j & 3);
-                x.v[j] = *(const __attribute__((address_space(3))) float*)(lds_cptr)(uintptr_t)(l.lo + row * RB + (((col >> 2) ^ image_swizzle<RB>(row)) << 4) + (col & 3) * 4 + off);
+                x.v[j] = *(const __attribute__((address_space(3))) float*)(lds_cptr)(uintptr_t)(l.lo + row * RB + (((col >> 2) ^ image_swizzle<RB, (int)sizeof(T)>(row)) << 4) + (col & 3) * 4 + off);
             }
             return x;
         }
@@ -170,14 +173,14 @@ template <typename T, int DP, int ROWS, int NW, bool LAZY = false> struct Stream
     static constexpr int RB = DP * (int)sizeof(T);
     static constexpr int NI = ROWS * RB / 1024 / NW;       // wave-instructions per wave
     static constexpr int RPI = 1024 / RB;                  // rows per instruction
-    static constexpr int NP = RB == 64 ? 1 : RB == 512 ? 4 : 2;
+    static constexpr int NP = 16 / RPI;                    // the swizzle repeats after 16 rows
     static_assert(NI >= NP && NI % NP == 0 && NI * NW * 1024 == ROWS * RB, "whole swizzle periods per wave");
     unsigned voff[LAZY ? 1 : NP];
     unsigned rs;
     int wave, pieces;
     __device__ __forceinline__ unsigned offset(int lane, int row0, int limit) const {
         const int row = row0 + lane * 16 / RB;
-        return (unsigned)min(row, limit) * rs + (unsigned)min(((lane * 16 % RB) >> 4) ^ image_swizzle<RB>(row), pieces - 1) * 16;
+        return (unsigned)min(row, limit) * rs + (unsigned)min(((lane * 16 % RB) >> 4) ^ image_swizzle<RB, (int)sizeof(T)>(row), pieces - 1) * 16;
     }
     __device__ __forceinline__ void init(long row_bytes, int D, int w) {
         wave = w; rs = (unsigned)row_bytes; pieces = D * (int)sizeof(T) / 16;
@@ -414,6 +417,14 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
             for (int t = 0; t < 2; ++t) I::M::mma(I::row_frag(im, t, kk), fq[kk], st[t]);
+        if constexpr (DP == 128 && sizeof(T) == 2) {       // four reads ahead of the products: two waves per SIMD do not cover an LDS read (668 -> 601 us)
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int kk = 0; kk < DP / 8; ++kk) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        }
         if (k0 + KT - 1 > wlim0) mask_rows<2>(st, klim - k0 - 4 * h2, -__builtin_inff());
         sm.template step<2>(st, a.c, off);
         acc_product<T, DP, 2>(sm.ot, st, im, 0, lane, TB);
