@@ -157,6 +157,10 @@ __device__ __forceinline__ const char* uniform_ptr(const char* p) {
 }
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char*)p; }
 
+// Every ordinary load has landed, as a wait that the compiler's own bookkeeping sees (gfx9 encoding: vmcnt 0, expcnt 7, lgkmcnt 15). In front of each loop
+// that keeps DMAs in flight: without it the compiler waits for the operands loaded before the loop INSIDE it, at every turn, and drains the next
+// tile's DMA right after its request (1 x 12289 forward, 16/2 heads of 128: see the loop's figures).
+#define PA_LOADS_DONE() __builtin_amdgcn_s_waitcnt(0x0F70)
 #define PA_SYNC_TILE()                                                  \
     do {                                                                \
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");     \
@@ -395,6 +399,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
     if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, w.head) * LOG2E; far_hi = bias_at(a, a.maxd, w.head) * LOG2E; }
     Softmax<DP> sm;
     sm.init();
+    PA_LOADS_DONE();
     for (int i = 0; i < nt; ++i) {
         const int k0 = i * KT;
         PA_SYNC_TILE();
@@ -454,6 +459,16 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
     float* all = ml + NW * 64;                             // the waves' joined (m, l)
     float* tab = all + 64;
     unsigned short* lut = (unsigned short*)(tab + a.buckets * G);
+    const char* kb = a.k + (long)a.k_start[seq] * a.sk.rs + (long)kvh * a.sk.hs;
+    const char* vb = a.v + (long)a.k_start[seq] * a.sv.rs + (long)kvh * a.sv.hs;
+    Stream<T, DP, WR, 1> ks, vs;
+    ks.init(a.sk.rs, a.D, 0);
+    vs.init(a.sv.rs, a.D, 0);
+    char* mine = smem + wave * 4 * BB;
+    const unsigned lds0 = lds_addr(mine);
+    const typename I::Lane im0 = I::lane_offsets(lane);
+    const int first = kbeg + wave * WR;                    // the first block is on its way before anything else is read
+    if (first < kend) { ks.load(kb + (long)first * a.sk.rs, k_len - first, lds0); vs.load(vb + (long)first * a.sv.rs, k_len - first, lds0 + BB); }
     const int off = k_len - q_len;
     if constexpr (BIAS) {
         if (kend - 1 - off > -a.maxd) {                    // some key is near some query
@@ -470,23 +485,12 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) fq[kk] = global_frag<T, DP>(row, kk, h2, a.D);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing of the compiler's stays in flight among the counted DMAs
     const int qpos = qi + off, klim = a.causal ? min(k_len - 1, qpos) : k_len - 1;
     float far_lo = 0.f, far_hi = 0.f;
     if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, kvh * G + g) * LOG2E; far_hi = bias_at(a, a.maxd, kvh * G + g) * LOG2E; }
-    const char* kb = a.k + (long)a.k_start[seq] * a.sk.rs + (long)kvh * a.sk.hs;
-    const char* vb = a.v + (long)a.k_start[seq] * a.sv.rs + (long)kvh * a.sv.hs;
-    Stream<T, DP, WR, 1> ks, vs;
-    ks.init(a.sk.rs, a.D, 0);
-    vs.init(a.sv.rs, a.D, 0);
-    char* mine = smem + wave * 4 * BB;
-    const unsigned lds0 = lds_addr(mine);
-    const typename I::Lane im0 = I::lane_offsets(lane);
     Softmax<DP> sm;
     sm.init();
-    const int first = kbeg + wave * WR;
-    if (BIAS) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (first < kend) { ks.load(kb + (long)first * a.sk.rs, k_len - first, lds0); vs.load(vb + (long)first * a.sv.rs, k_len - first, lds0 + BB); }
+    PA_LOADS_DONE();
     int par = 0;
     for (int k0 = first; k0 < kend; k0 += NW * WR, par ^= 1) {
         const int nx = k0 + NW * WR;
@@ -495,7 +499,7 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
             const unsigned dst = lds0 + (par ^ 1) * 2 * BB;
             ks.load(kb + (long)nx * a.sk.rs, k_len - nx, dst);
             vs.load(vb + (long)nx * a.sv.rs, k_len - nx, dst + BB);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Stream<T, DP, WR, 1>::NI) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Stream<T, DP, WR, 1>::NI) : "memory");      // all but the block just requested
         } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
         const typename I::Lane im = I::at(im0, lds0 + par * 2 * BB);
@@ -710,6 +714,7 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
     zero_acc(dq);
 #pragma unroll
     for (int e = 0; e < 16; ++e) start[e] = MODE == DELTA ? 0.f : -dl;
+    PA_LOADS_DONE();
     for (int i = 0; i < nt; ++i) {
         const int k0 = i * KT;
         PA_SYNC_TILE();
@@ -860,18 +865,13 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
         os.init(a.sdo.rs, a.D, wave);
         const unsigned lds0 = lds_addr(smem);
         typename I::Lane im = I::at(I::lane_offsets(lane), lds0 + 2 * TB);      // moved to the other buffer at every tile
-        float reg = 0.f;                                   // threads 0..63: lse of the next tile, 64..127: -delta
+        float reg = 0.f;                                   // threads 0..63: lse of the next tile, 64..127: delta
         auto fetch = [&](int it, unsigned dst) {
             const int g = it / per, q0 = qfirst + (it - g * per) * KT, head = kvh * G + g;
             const long row = (long)q_row + q0;
             if (threadIdx.x < 2 * KT) {
-                const int j = threadIdx.x & (KT - 1);
-                const bool in = q0 + j < q_len;
-                const long s = (row + min(j, q_len - 1 - q0)) * a.hq + head;
-                if (threadIdx.x < KT) {
-                    const float x = a.lse[s];
-                    reg = in && x > -__builtin_inff() ? x * LOG2E : __builtin_inff();
-                } else reg = in ? -a.delta[s] : 0.f;
+                const long s = (row + min((int)threadIdx.x & (KT - 1), q_len - 1 - q0)) * a.hq + head;
+                reg = (threadIdx.x < KT ? a.lse : a.delta)[s];
             }
             qs.load(a.q + row * a.sq.rs + (long)head * a.sq.hs, q_len - q0, dst);
             os.load(a.dout + row * a.sdo.rs + (long)head * a.sdo.hs, q_len - q0, dst + TB);
@@ -882,7 +882,10 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
         for (int it = i0; it < i1; ++it) {
             const int par = (it - i0) & 1, g = it / per, q0 = qfirst + (it - g * per) * KT;
             float* ls = stat + par * 2 * KT;
-            if (threadIdx.x < 2 * KT) ls[threadIdx.x] = reg;
+            if (threadIdx.x < 2 * KT) {                    // rows past the end and rows without keys: probabilities 0
+                const bool in = q0 + ((int)threadIdx.x & (KT - 1)) < q_len;
+                ls[threadIdx.x] = threadIdx.x < KT ? (in && reg > -__builtin_inff() ? reg * LOG2E : __builtin_inff()) : in ? -reg : 0.f;
+            }
             if constexpr (BIAS) {
                 if (g != held) {                           // uniform; the last tile's readers are past the barrier below before anything is overwritten
                     if (held >= 0) __syncthreads();
@@ -892,6 +895,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
                     far_hi = bias_at(a, a.maxd, kvh * G + g) * LOG2E;
                 }
             }
+            PA_LOADS_DONE();
             PA_SYNC_TILE();
             I::template move<TIGHT>(im, par ? 2 * TB : -2 * TB);
             if (it + 1 < i1) fetch(it + 1, lds0 + (par ^ 1) * 2 * TB);
@@ -1011,11 +1015,12 @@ constexpr int FEW_TABLE = 4096;          // table entries of one key head's grou
 
 // The few-rows kernel takes the call when one key head's query rows of every recording fit its 32-row operand.
 bool few_rows(const Plan& p, int hq, int hkv, int buckets) { return p.max_q * (hq / hkv) <= WR && (long)buckets * (hq / hkv) <= FEW_TABLE; }
-// keys per workgroup: about four workgroups per CU, whole rounds of the four waves' blocks; a recording of up to 512 keys stays whole (one
-// launch instead of two)
+// keys per workgroup: two workgroups per CU by the capacities, whole rounds of the four waves' blocks (3 streams of 60-131 k keys, 16/4 heads of
+// 64: 2048 workgroups 73 us, 1024 72, 512 68; 48 of 100-4096, 16/2 heads of 128: 48, 34, 33); a recording of up to 512 keys stays
+// whole (one launch instead of two)
 int few_chunk(const Plan& p, int hkv) {
     if (p.max_k <= 512) return 512;
-    const long want = (p.k_rows * hkv + 1023) / 1024;
+    const long want = (p.k_rows * hkv + 511) / 512;
     const long c = (want + 127) / 128 * 128;
     return (int)(c < 256 ? 256 : c > 8192 ? 8192 : c);
 }

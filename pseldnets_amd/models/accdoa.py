@@ -9,6 +9,7 @@ from .components.passt import FcTanhHead, PasstEncoder
 from .components.crnn import ConvEncoder
 from .components.conformer import ConformerDecoder
 from .components.gru import GRUDecoder
+from .components.stream import StreamDecoder
 from .components.transformer import TransformerDecoder
 from .. import ops
 from .components.seld_net import HTSATNetBase
@@ -248,6 +249,8 @@ def make_decoder(arena, prefix, decoder, num_feats, n_layers):
         return GRUDecoder(arena, prefix, num_feats, n_layers)
     if decoder == 'transformer':
         return TransformerDecoder(arena, prefix, num_feats, n_layers)
+    if decoder == 'stream':                                             # not in the reference: looks back only, see components/stream.py
+        return StreamDecoder(arena, prefix, num_feats, n_layers)
     if decoder is None:
         return None
     raise NotImplementedError(f"{decoder} is not implemented")          # model_utilities.py:262-263
@@ -278,7 +281,7 @@ class CRNN(StaticBufferMixin, HTSATNetBase):
     """models/accdoa.py:12-95: scalar BatchNorms -> CNN8 / CNN12 (the PANNs CNN14 conv stack) -> frequency mean ->
     decoder -> 'repeat' x8 interpolation + 10-frame mean -> Linear -> tanh. Built on the MI355X path with
     `cfg.model.decoder` = 'conformer' (configs/model/crnn.yaml:5; ConformerBlocks, model_utilities.py:254-255) or None
-    (nn.Identity, :260-261), 'gru' or 'transformer'."""
+    (nn.Identity, :260-261), 'gru', 'transformer' or 'stream' (causal: components/stream.py)."""
     out_key = 'accdoa'
     tracks_axes = 3
     decoder_prefix = 'decoder.decoder.'          # Decoder(...).decoder = ConformerBlocks
@@ -290,7 +293,7 @@ class CRNN(StaticBufferMixin, HTSATNetBase):
         decoder, n_layers = decoder_config(cfg)
         if self.forced_decoder_layers is not None:
             decoder, n_layers = 'conformer', self.forced_decoder_layers
-        if decoder not in (None, 'conformer', 'gru', 'transformer'):
+        if decoder not in (None, 'conformer', 'gru', 'transformer', 'stream'):
             raise NotImplementedError(f"{decoder} is not implemented")          # model_utilities.py:262-263
         self.num_classes = num_classes
         self.interpolate_time_ratio = 2 ** 3
