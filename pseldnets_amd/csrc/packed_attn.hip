@@ -215,6 +215,10 @@ __device__ __forceinline__ float bias_at(const PAttnArgs& a, int rel, int head) 
     const int r = max(-a.maxd, min(a.maxd, rel));
     return a.table[(long)a.lut[r + a.maxd] * a.hq + head];
 }
+// the same, log2 units, for a head that is the workgroup's: in a scalar register
+__device__ __forceinline__ float far_bias(const PAttnArgs& a, int rel, int head) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, bias_at(a, rel, head) * LOG2E)));
+}
 // dist[i] = bias of distance i - maxd - NEAR_PAD over the scale: in units of the raw products, whose accumulators start from it
 __device__ __forceinline__ void dist_fill(float* dist, const PAttnArgs& a, int head, int threads) {
     const int n = dist_count(a.maxd);
@@ -396,7 +400,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
     const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;   // every query of the wave sees keys up to here,
     const int wlim1 = w.q0 + wave * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;     // none sees one past here
     float far_lo = 0.f, far_hi = 0.f;
-    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, w.head) * LOG2E; far_hi = bias_at(a, a.maxd, w.head) * LOG2E; }
+    if constexpr (BIAS) { far_lo = far_bias(a, -a.maxd, w.head); far_hi = far_bias(a, a.maxd, w.head); }
     Softmax<DP> sm;
     sm.init();
     PA_LOADS_DONE();
@@ -709,7 +713,7 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
     const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;
     const int wlim1 = w.q0 + wave * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;
     float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f;
-    if constexpr (BIAS) { far_lo = bias_at(a, -a.maxd, w.head) * LOG2E; far_hi = bias_at(a, a.maxd, w.head) * LOG2E; }
+    if constexpr (BIAS) { far_lo = far_bias(a, -a.maxd, w.head); far_hi = far_bias(a, a.maxd, w.head); }
     f32x16 dq[DP / 32], start;
     zero_acc(dq);
 #pragma unroll
@@ -829,6 +833,9 @@ __device__ __forceinline__ int dkv_parts(int total, int most, int chunk) { retur
 
 // dk, dv: 128 keys of one (recording, key head), a wave 32 (lanes = keys); the query heads of the group and the 64-query tiles stream by.
 // A stream of more than `chunk` tiles is shared between up to nsplit workgroups: f32 partials, added in order by packed_attn_dkv_join_kernel.
+// (heads of 128 in bf16: a few of v's operands are read from LDS at every tile; held in registers with the rest they spill, and a spill's reload
+// waits for the next tile's DMA. Two workgroups still fit a CU's LDS.)
+template <typename T, int DP, bool BIAS> constexpr int dkv_lds_frags() { return sizeof(T) == 2 && DP == 128 ? (BIAS ? 3 : 2) : 0; }
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dkv_kernel(PAttnArgs a) {
     using I = Image<T, DP>;
@@ -836,7 +843,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
     constexpr bool TIGHT = DP == 128;
     extern __shared__ __attribute__((aligned(1024))) char smem[];      // 2 x (Q | dO) | 2 x (lse | -delta) x 64 | bias by distance
     float* stat = (float*)(smem + 4 * TB);
-    float* dist = stat + 4 * KT;
+    constexpr int LV = dkv_lds_frags<T, DP, BIAS>(), RV = DP / 16 - LV;      // operands of v kept in LDS / in registers
+    char* kept = (char*)(stat + 4 * KT) + (threadIdx.x >> 6) * LV * 1024 + (threadIdx.x & 63) * 16;
+    float* dist = stat + 4 * KT + LV * 1024;
     const int kvh = blockIdx.x % a.hkv, rest = blockIdx.x / a.hkv, split = rest % a.nsplit, ti = rest / a.nsplit;
     const int* rec = a.tiles + 8 * (long)ti;
     const int seq = rec[0], kt0 = rec[1], q_row = rec[2], q_len = rec[3], k_row = rec[4], k_cap = rec[5];
@@ -852,13 +861,16 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
     if (split >= ns) return;
     const int i0 = (int)((long)total * split / ns), i1 = (int)((long)total * (split + 1) / ns);
     if (i0 < i1) {
-        typename I::Frag fk[DP / 16], fv[DP / 16];
+        typename I::Frag fk[DP / 16], fv[RV];
         {
             const long kr = (long)k_row + min(key, k_len - 1);
             const char* krp = a.k + kr * a.sk.rs + (long)kvh * a.sk.hs;
             const char* vrp = a.v + kr * a.sv.rs + (long)kvh * a.sv.hs;
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) { fk[kk] = global_frag<T, DP>(krp, kk, h2, a.D); fv[kk] = global_frag<T, DP>(vrp, kk, h2, a.D); }
+            for (int kk = 0; kk < DP / 16; ++kk) { fk[kk] = global_frag<T, DP>(krp, kk, h2, a.D); if (kk < RV) fv[kk < RV ? kk : 0] = global_frag<T, DP>(vrp, kk, h2, a.D); }
+            if constexpr (sizeof(T) == 2)
+#pragma unroll
+                for (int x = 0; x < LV; ++x) *(typename I::Frag*)(kept + x * 1024) = global_frag<T, DP>(vrp, RV + x, h2, a.D);
         }
         Stream<T, DP, KT, 4, TIGHT> qs, os;
         qs.init(a.sq.rs, a.D, wave);
@@ -891,8 +903,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
                     if (held >= 0) __syncthreads();
                     held = g;
                     dist_fill(dist, a, kvh * G + g, 256);
-                    far_lo = bias_at(a, -a.maxd, kvh * G + g) * LOG2E;
-                    far_hi = bias_at(a, a.maxd, kvh * G + g) * LOG2E;
+                    far_lo = far_bias(a, -a.maxd, kvh * G + g);
+                    far_hi = far_bias(a, a.maxd, kvh * G + g);
                 }
             }
             PA_LOADS_DONE();
@@ -921,7 +933,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
                     I::M::mma(I::row_frag(im, t, kk), fk[kk], s[0]);      // rows = queries, lanes = keys
-                    I::M::mma(I::row_frag(im, t, kk, TB), fv[kk], dp[0]);
+                    if (kk < RV) I::M::mma(I::row_frag(im, t, kk, TB), fv[kk < RV ? kk : 0], dp[0]);
+                    else if constexpr (sizeof(T) == 2) I::M::mma(I::row_frag(im, t, kk, TB), *(const typename I::Frag*)(kept + (kk - RV) * 1024), dp[0]);
                     if (kk & 1) pace<TIGHT>();
                 }
                 if (kw0 + WR > k_len || (a.causal && qt0 < kw0 + WR - 1)) {            // some pair is masked: keep key < k_len and query >= key
@@ -1115,7 +1128,7 @@ int run_bwd(PAttnArgs& a, const Plan& p, float* dtable, int accumulate, hipStrea
     a.tiles = a.causal ? p.k_tile_causal : p.k_tile;
     a.nsplit = dkv_splits(p, a.hq, a.hkv, a.D, a.causal);
     a.chunk = dkv_chunk(p, a.hq, a.D, a.causal);
-    PA_LAUNCH((packed_attn_dkv_kernel<T, DP, BIAS>), p.k_tiles * a.hkv * a.nsplit, 256, 4 * TB + 4 * KT * 4 + nd, a);
+    PA_LAUNCH((packed_attn_dkv_kernel<T, DP, BIAS>), p.k_tiles * a.hkv * a.nsplit, 256, 4 * TB + 4 * KT * 4 + 4096 * (dkv_lds_frags<T, DP, BIAS>()) + nd, a);
     if (a.nsplit > 1) PA_LAUNCH((packed_attn_dkv_join_kernel<T, DP>), p.k_tiles * a.hkv, 256, 0, a);
     return PSELD_OK;
 }
