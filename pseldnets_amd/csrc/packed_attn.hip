@@ -46,6 +46,7 @@ struct PAttnArgs {
     int buckets, maxd;
     float* part;                // dtable: [tiles, hq, buckets]; split dk/dv: [tiles, hkv, nsplit, 2, TILE, DP]; few rows: see there
     int max_rows;               // few rows: rows reserved per key head
+    int bias_heads;             // dk, dv: heads whose bias LDS has room for
 };
 
 // Two waves per SIMD where 256 registers hold a wave's accumulators and operands: the compiler then keeps the accumulators in vector registers
@@ -346,24 +347,28 @@ template <int NT> __device__ __forceinline__ void mask_rows(f32x16 (&x)[NT], int
 
 // which recording, rows and head a workgroup of the query-tiled kernels owns. Heads fastest, the query heads of one key head a multiple of
 // hkv apart: with hkv a multiple of the eight XCDs every key head's tiles stay on one XCD's L2
+// f32 (the parity mode): an f32 matrix instruction takes 64 cycles and short recordings leave few waves, so the four waves are two groups of 32
+// rows x two halves of every key tile, joined through LDS at the end: half the rows per workgroup, half the time per tile (6 recordings of 30-600,
+// 8 heads of 64: forward 63 -> 40 us)
+template <typename T> constexpr int key_split() { return sizeof(T) == 4 ? 2 : 1; }
 struct QTile {
     int seq, q0, q_len, k_len, off, head, kvh, nk;
     long q_row, k_row;
 };
-__device__ __forceinline__ QTile q_tile_of(const PAttnArgs& a) {
+template <int KS> __device__ __forceinline__ QTile q_tile_of(const PAttnArgs& a) {
     QTile t;
-    const int p = blockIdx.x % a.hq, ti = blockIdx.x / a.hq;
+    const int p = blockIdx.x % a.hq, ti = blockIdx.x / a.hq / KS;
     t.kvh = p % a.hkv;
     t.head = t.kvh * (a.hq / a.hkv) + p / a.hkv;
     const int* rec = a.tiles + 8 * (long)ti;               // one load for all that is fixed: the chain to the first key row is two loads long
     t.seq = rec[0];
-    t.q0 = rec[1];
+    t.q0 = rec[1] + blockIdx.x / a.hq % KS * (TILE / KS);
     t.q_row = rec[2];
     t.q_len = rec[3];
     t.k_row = rec[4];
     t.k_len = max(0, min(a.k_len[t.seq], rec[5]));
     t.off = t.k_len - t.q_len;
-    t.nk = a.causal ? max(0, min(t.k_len, t.q0 + TILE + t.off)) : t.k_len;
+    t.nk = t.q0 >= t.q_len ? 0 : a.causal ? max(0, min(t.k_len, t.q0 + TILE / KS + t.off)) : t.k_len;
     return t;
 }
 
@@ -371,12 +376,13 @@ __device__ __forceinline__ QTile q_tile_of(const PAttnArgs& a) {
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fwd_kernel(PAttnArgs a) {
     using I = Image<T, DP>;
-    constexpr int TB = KT * I::RB;
+    constexpr int TB = KT * I::RB, KS = key_split<T>(), KW = KT / KS, NT = 2 / KS;
     extern __shared__ __attribute__((aligned(1024))) char smem[];      // 2 x (K tile | V tile) | bias by distance
     float* dist = (float*)(smem + 4 * TB);
-    const QTile w = q_tile_of(a);
+    const QTile w = q_tile_of<KS>(a);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
-    const int qi = w.q0 + wave * WR + r;
+    const int rg = wave % (4 / KS), kh = wave / (4 / KS);       // the wave's rows and its part of every key tile
+    const int qi = w.q0 + rg * WR + r;
     const bool live = qi < w.q_len;
     const long qrow = w.q_row + min(qi, w.q_len - 1);
     const char* kb = a.k + w.k_row * a.sk.rs + (long)w.kvh * a.sk.hs;
@@ -395,10 +401,10 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) fq[kk] = global_frag<T, DP>(row, kk, h2, a.D);
     }
-    const int qpos = qi + w.off, qw0 = w.q0 + wave * WR + w.off;        // the lane's and the wave's first query position
+    const int qpos = qi + w.off, qw0 = w.q0 + rg * WR + w.off;        // the lane's and the wave's first query position
     const int klim = a.causal ? min(w.k_len - 1, qpos) : w.k_len - 1;
     const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;   // every query of the wave sees keys up to here,
-    const int wlim1 = w.q0 + wave * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;     // none sees one past here
+    const int wlim1 = w.q0 + rg * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;     // none sees one past here
     float far_lo = 0.f, far_hi = 0.f;
     if constexpr (BIAS) { far_lo = far_bias(a, -a.maxd, w.head); far_hi = far_bias(a, a.maxd, w.head); }
     Softmax<DP> sm;
@@ -412,20 +418,21 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
             ks.load(kb + (long)(k0 + KT) * a.sk.rs, w.k_len - k0 - KT, dst);
             vs.load(vb + (long)(k0 + KT) * a.sv.rs, w.k_len - k0 - KT, dst + TB);
         }
-        if (k0 > wlim1) continue;
-        const typename I::Lane im = I::at(im0, lds0 + (i & 1) * 2 * TB);
-        f32x16 st[2];
+        const int kt0 = k0 + kh * KW;                      // the wave's first key of the tile
+        if (kt0 > wlim1) continue;
+        const typename I::Lane im = I::at(im0, lds0 + kh * KW * I::RB + (i & 1) * 2 * TB);
+        f32x16 st[NT];
         zero_acc(st);
         float off = 0.f;
         if constexpr (BIAS) {
-            const int place = place_of(k0 - (qw0 + WR - 1), k0 + KT - 1 - qw0, a.maxd);
-            if (place == NEAR) start_near<2, 1>(st, dist + (k0 + 4 * h2 - qpos + a.maxd + NEAR_PAD));
+            const int place = place_of(kt0 - (qw0 + WR - 1), kt0 + KW - 1 - qw0, a.maxd);
+            if (place == NEAR) start_near<NT, 1>(st, dist + (kt0 + 4 * h2 - qpos + a.maxd + NEAR_PAD));
             else off = place < 0 ? far_lo : far_hi;
         }
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) I::M::mma(I::row_frag(im, t, kk), fq[kk], st[t]);
+            for (int t = 0; t < NT; ++t) I::M::mma(I::row_frag(im, t, kk), fq[kk], st[t]);
         if constexpr (DP == 128 && sizeof(T) == 2) {       // four reads ahead of the products: two waves per SIMD do not cover an LDS read (668 -> 601 us)
             __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
@@ -434,9 +441,27 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
         }
-        if (k0 + KT - 1 > wlim0) mask_rows<2>(st, klim - k0 - 4 * h2, -__builtin_inff());
-        sm.template step<2>(st, a.c, off);
-        acc_product<T, DP, 2>(sm.ot, st, im, 0, lane, TB);
+        if (kt0 + KW - 1 > wlim0) mask_rows<NT>(st, klim - kt0 - 4 * h2, -__builtin_inff());
+        sm.template step<NT>(st, a.c, off);
+        acc_product<T, DP, NT>(sm.ot, st, im, 0, lane, TB);
+    }
+    if constexpr (KS > 1) {                                // the second half's waves hand over their maxima, sums and outputs, a register per row of 64 lanes
+        float* x = (float*)smem + rg * (DP / 2 + 2) * 64 + lane;
+        __syncthreads();
+        if (kh) {
+#pragma unroll
+            for (int e = 0; e < DP / 2; ++e) x[e * 64] = sm.ot[e >> 4][e & 15];
+            x[DP / 2 * 64] = sm.m;
+            x[(DP / 2 + 1) * 64] = sm.l;
+        }
+        __syncthreads();
+        if (kh) return;
+        const float m2 = x[DP / 2 * 64], mn = fmaxf(sm.m, m2);
+        const float f1 = sm.m == mn ? 1.f : __builtin_amdgcn_exp2f(sm.m - mn), f2 = m2 == mn ? 1.f : __builtin_amdgcn_exp2f(m2 - mn);
+#pragma unroll
+        for (int e = 0; e < DP / 2; ++e) sm.ot[e >> 4][e & 15] = fmaf(sm.ot[e >> 4][e & 15], f1, x[e * 64] * f2);
+        sm.l = sm.l * f1 + x[(DP / 2 + 1) * 64] * f2;
+        sm.m = mn;
     }
     const float l = sm.l + __shfl_xor(sm.l, 32, 64);
     store_rows<T, DP>(a.out + qrow * a.so.rs + (long)w.head * a.so.hs, live, sm.ot, l > 0.f ? 1.f / l : 0.f, a.D, h2);
@@ -641,13 +666,18 @@ enum { DQ = 0, DQ_TABLE = 1, DELTA = 2 };
 constexpr int DIAG_PITCH = 68, DIAG = 32 * DIAG_PITCH;      // floats; 16-byte pieces of eight rows fall in different banks
 typedef __attribute__((address_space(3))) float* lds_fptr;
 typedef __attribute__((address_space(3))) f32x4* lds_f4ptr;
-__device__ __forceinline__ void add_diagonals(unsigned m, unsigned h, const f32x16 (&x)[2], int lane) {
+template <int NT> __device__ __forceinline__ void add_diagonals(unsigned m, unsigned h, const f32x16 (&x)[NT], int lane) {
     const int r = lane & 31, h2 = lane >> 5;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-            *(lds_f4ptr)(uintptr_t)(m + (r * DIAG_PITCH + 4 * h2) * 4 + (t * 32 + 8 * g) * 4) = f32x4{x[t][4 * g], x[t][4 * g + 1], x[t][4 * g + 2], x[t][4 * g + 3]};
+        for (int g = 0; g < 4; ++g) {
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};                // (32 keys only: the other half is zeros)
+            if (t < NT)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = x[t < NT ? t : 0][4 * g + i];
+            *(lds_f4ptr)(uintptr_t)(m + (r * DIAG_PITCH + 4 * h2) * 4 + (t * 32 + 8 * g) * 4) = v;
+        }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // a wave's LDS operations run in order; this keeps the compiler's order too
     float all = 0.f, before = 0.f;
 #pragma unroll
@@ -671,7 +701,7 @@ template <typename T, int DP, int MODE> constexpr int dq_buffers() { return size
 template <typename T, int DP, bool BIAS, int MODE>
 __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per_simd<T, DP>())) void packed_attn_dq_kernel(PAttnArgs a) {
     using I = Image<T, DP>;
-    constexpr int TB = KT * I::RB, NB = dq_buffers<T, DP, MODE>();
+    constexpr int TB = KT * I::RB, NB = dq_buffers<T, DP, MODE>(), KS = key_split<T>(), KW = KT / KS, NT = 2 / KS;
     constexpr bool TIGHT = DP == 128;
     extern __shared__ __attribute__((aligned(1024))) char smem[];      // NB x (K | V) | bias by distance | then (DQ_TABLE) sums by distance, a copy per wave | 8 floats | 4 x DIAG
     float* dist = (float*)(smem + NB * 2 * TB);
@@ -679,9 +709,10 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
     float* hist = dist + ndist;
     float* far = hist + 4 * ndist;
     const unsigned diag = (lds_addr(far + 8) + 15) & ~15u;
-    const QTile w = q_tile_of(a);
+    const QTile w = q_tile_of<KS>(a);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
-    const int qi = w.q0 + wave * WR + r;
+    const int rg = wave % (4 / KS), kh = wave / (4 / KS);       // the wave's rows and its part of every key tile
+    const int qi = w.q0 + rg * WR + r;
     const bool live = qi < w.q_len;
     const long qrow = w.q_row + min(qi, w.q_len - 1);
     const char* kb = a.k + w.k_row * a.sk.rs + (long)w.kvh * a.sk.hs;
@@ -708,10 +739,10 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
     const float lse2 = live && lse > -__builtin_inff() ? lse * LOG2E : __builtin_inff();      // +inf: every probability of the row is 0
     float dl = 0.f;
     if constexpr (MODE != DELTA) dl = a.delta[si];
-    const int qpos = qi + w.off, qw0 = w.q0 + wave * WR + w.off;
+    const int qpos = qi + w.off, qw0 = w.q0 + rg * WR + w.off;
     const int klim = a.causal ? min(w.k_len - 1, qpos) : w.k_len - 1;
     const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;
-    const int wlim1 = w.q0 + wave * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;
+    const int wlim1 = w.q0 + rg * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;
     float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f;
     if constexpr (BIAS) { far_lo = far_bias(a, -a.maxd, w.head); far_hi = far_bias(a, a.maxd, w.head); }
     f32x16 dq[DP / 32], start;
@@ -732,31 +763,32 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
             ks.load(kb + (long)(k0 + KT) * a.sk.rs, w.k_len - k0 - KT, dst);
             vs.load(vb + (long)(k0 + KT) * a.sv.rs, w.k_len - k0 - KT, dst + TB);
         }
-        if (k0 > wlim1) continue;
-        const typename I::Lane im = I::at(im0, lds0 + (NB == 2 ? i & 1 : 0) * 2 * TB);
-        f32x16 st[2], dp[2];
+        const int kt0 = k0 + kh * KW;                      // the wave's first key of the tile
+        if (kt0 > wlim1) continue;
+        const typename I::Lane im = I::at(im0, lds0 + kh * KW * I::RB + (NB == 2 ? i & 1 : 0) * 2 * TB);
+        f32x16 st[NT], dp[NT];
         zero_acc(st);
         float off = 0.f;
         int place = NEAR;
         if constexpr (BIAS) {
-            place = place_of(k0 - (qw0 + WR - 1), k0 + KT - 1 - qw0, a.maxd);
-            if (place == NEAR) start_near<2, 1>(st, dist + (k0 + 4 * h2 - qpos + a.maxd + NEAR_PAD));
+            place = place_of(kt0 - (qw0 + WR - 1), kt0 + KW - 1 - qw0, a.maxd);
+            if (place == NEAR) start_near<NT, 1>(st, dist + (kt0 + 4 * h2 - qpos + a.maxd + NEAR_PAD));
             else off = place < 0 ? far_lo : far_hi;
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) dp[t] = start;          // dP - delta: the product starts from -delta of the lane's query
+        for (int t = 0; t < NT; ++t) dp[t] = start;          // dP - delta: the product starts from -delta of the lane's query
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < NT; ++t) {
                 I::M::mma(I::row_frag(im, t, kk), fq[kk], st[t]);
                 I::M::mma(I::row_frag(im, t, kk, TB), fo[kk], dp[t]);
-                if (t) pace<TIGHT>();
+                if (t == NT - 1) pace<TIGHT>();
             }
-        if (k0 + KT - 1 > wlim0) mask_rows<2>(st, klim - k0 - 4 * h2, -__builtin_inff());
+        if (kt0 + KW - 1 > wlim0) mask_rows<NT>(st, klim - kt0 - 4 * h2, -__builtin_inff());
         const float sub = off - lse2;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e], a.c, sub));
@@ -765,22 +797,33 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
             }
         if constexpr (MODE == DQ_TABLE) {
             if (place == NEAR) {
-                add_diagonals(diag + wave * DIAG * 4, lds_addr(hist) + (wave * ndist + k0 - qw0 + a.maxd + NEAR_PAD) * 4, st, lane);
+                add_diagonals<NT>(diag + wave * DIAG * 4, lds_addr(hist) + (wave * ndist + kt0 - qw0 + a.maxd + NEAR_PAD) * 4, st, lane);
             } else {
                 float s = 0.f;
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s += st[t][e];
                 if (place < 0) sum_lo += s; else sum_hi += s;
             }
         }
-        if constexpr (MODE != DELTA) acc_product<T, DP, 2, TIGHT>(dq, st, im, 0, lane, 0);
+        if constexpr (MODE != DELTA) acc_product<T, DP, NT, TIGHT>(dq, st, im, 0, lane, 0);
+    }
+    if constexpr (KS > 1) {                                // the second half's waves hand over their sums
+        float* x = (float*)smem + rg * (DP / 2) * 64 + lane;
+        __syncthreads();
+        if (kh)
+#pragma unroll
+            for (int e = 0; e < DP / 2; ++e) x[e * 64] = dq[e >> 4][e & 15];
+        __syncthreads();
+        if (!kh)
+#pragma unroll
+            for (int e = 0; e < DP / 2; ++e) dq[e >> 4][e & 15] += x[e * 64];
     }
     if constexpr (MODE == DELTA) {
         dl += __shfl_xor(dl, 32, 64);
         if (live && h2 == 0) a.delta[si] = dl;
-    } else store_rows<T, DP>(a.dq + qrow * a.sdq.rs + (long)w.head * a.sdq.hs, live, dq, a.scale, a.D, h2);
+    } else store_rows<T, DP>(a.dq + qrow * a.sdq.rs + (long)w.head * a.sdq.hs, live && kh == 0, dq, a.scale, a.D, h2);
     if constexpr (MODE == DQ_TABLE) {
         sum_lo = wave_sum(sum_lo);
         sum_hi = wave_sum(sum_hi);
@@ -889,8 +932,13 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
             os.load(a.dout + row * a.sdo.rs + (long)head * a.sdo.hs, q_len - q0, dst + TB);
         };
         fetch(i0, lds0);
-        int held = -1;                                     // the head whose bias LDS holds
-        float far_lo = 0.f, far_hi = 0.f;
+        // the bias of all the part's heads at once where LDS has room, otherwise of one head at a time
+        const int g0 = i0 / per, ndist = BIAS ? dist_count(a.maxd) : 0;
+        const bool all = BIAS && (i1 - 1) / per - g0 < a.bias_heads;
+        if constexpr (BIAS)
+            if (all)
+                for (int g = g0; g <= (i1 - 1) / per; ++g) dist_fill(dist + (g - g0) * ndist, a, kvh * G + g, 256);
+        int held = -1;                                     // the head that LDS holds
         for (int it = i0; it < i1; ++it) {
             const int par = (it - i0) & 1, g = it / per, q0 = qfirst + (it - g * per) * KT;
             float* ls = stat + par * 2 * KT;
@@ -899,12 +947,10 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
                 ls[threadIdx.x] = threadIdx.x < KT ? (in && reg > -__builtin_inff() ? reg * LOG2E : __builtin_inff()) : in ? -reg : 0.f;
             }
             if constexpr (BIAS) {
-                if (g != held) {                           // uniform; the last tile's readers are past the barrier below before anything is overwritten
+                if (!all && g != held) {                   // uniform; the last tile's readers are past the barrier below before anything is overwritten
                     if (held >= 0) __syncthreads();
                     held = g;
                     dist_fill(dist, a, kvh * G + g, 256);
-                    far_lo = far_bias(a, -a.maxd, kvh * G + g);
-                    far_hi = far_bias(a, a.maxd, kvh * G + g);
                 }
             }
             PA_LOADS_DONE();
@@ -912,6 +958,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
             I::template move<TIGHT>(im, par ? 2 * TB : -2 * TB);
             if (it + 1 < i1) fetch(it + 1, lds0 + (par ^ 1) * 2 * TB);
             const int qp0 = q0 + off;                      // position of the tile's first query
+            const float* near = dist + (all ? (g - g0) * ndist : 0);
             if (kw0 >= k_len || (a.causal && qp0 + KT - 1 < kw0)) continue;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -921,8 +968,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
                 const int qt0 = qp0 + t * 32;
                 if constexpr (BIAS) {
                     const int place = place_of(kw0 - (qt0 + 31), kw0 + WR - 1 - qt0, a.maxd);
-                    if (place == NEAR) start_near<1, -1>(s, dist + (key - qt0 - 4 * h2 + a.maxd + NEAR_PAD));
-                    else bo = place < 0 ? far_lo : far_hi;
+                    if (place == NEAR) start_near<1, -1>(s, near + (key - qt0 - 4 * h2 + a.maxd + NEAR_PAD));
+                    else bo = near[place < 0 ? 0 : ndist - 1] * a.c;
                 }
 #pragma unroll
                 for (int gq = 0; gq < 4; ++gq) {           // dP - delta: the product starts from -delta of the row's query
@@ -974,28 +1021,28 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dk
         store_rows<float, DP>((char*)(p + (long)TILE * DP), true, dv, 1.f, DP, oh);
     }
 }
+// adds the parts of a key tile, 256 pieces of 8 elements a workgroup
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(PAttnArgs a) {
-    const int kvh = blockIdx.x % a.hkv, ti = blockIdx.x / a.hkv;
+    constexpr int PIECES = 2 * TILE * DP / 8 / 256;
+    const int at = blockIdx.x % PIECES, kvh = blockIdx.x / PIECES % a.hkv, ti = blockIdx.x / PIECES / a.hkv;
     const int* rec = a.tiles + 8 * (long)ti;
     const int kt0 = rec[1], q_len = rec[3], rows = min(TILE, rec[5] - kt0), k_len = max(0, min(a.k_len[rec[0]], rec[5]));
     const int qfirst = dkv_first(a, kt0, q_len, k_len), per = qfirst < q_len ? (q_len - qfirst + KT - 1) / KT : 0;
     const int ns = dkv_parts(per * (a.hq / a.hkv), a.nsplit, a.chunk);
-    if (ns == 1) return;
-    const float* p = a.part + ((long)ti * a.hkv + kvh) * a.nsplit * 2 * TILE * DP;
-    for (int i = threadIdx.x; i < 2 * rows * (DP / 8); i += 256) {
-        const int which = i >= rows * (DP / 8), j = i - which * rows * (DP / 8), row = j / (DP / 8), d = (j % (DP / 8)) * 8;
-        if (d >= a.D) continue;
-        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int x = 0; x < ns; ++x) {
-            float y[8];
-            load8<float>(p + ((long)(x * 2 + which) * TILE + row) * DP + d, y);
+    const int i = at * 256 + threadIdx.x, which = i / (TILE * DP / 8), row = i / (DP / 8) % TILE, d = i % (DP / 8) * 8;
+    if (ns == 1 || row >= rows || d >= a.D) return;
+    const float* p = a.part + (((long)ti * a.hkv + kvh) * a.nsplit * 2 + which) * TILE * DP + row * DP + d;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int x = 0; x < ns; ++x) {
+        float y[8];
+        load8<float>(p + (long)x * 2 * TILE * DP, y);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s[k] += y[k];
-        }
-        const Strides st = which ? a.sdv : a.sdk;
-        store8<T>((T*)((which ? a.dv : a.dk) + ((long)rec[4] + kt0 + row) * st.rs + (long)kvh * st.hs) + d, s);
+        for (int k = 0; k < 8; ++k) s[k] += y[k];
     }
+    const Strides st = which ? a.sdv : a.sdk;
+    store8<T>((T*)((which ? a.dv : a.dk) + ((long)rec[4] + kt0 + row) * st.rs + (long)kvh * st.hs) + d, s);
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------------------------------
@@ -1042,14 +1089,15 @@ int few_splits(const Plan& p, int hkv) { const int c = few_chunk(p, hkv); return
 // unevenly. Heads above 64: two workgroups fit a CU, 400 parts (a few of the 512 places stay free for the tiles' odd ends; 1 x 8191, 16/2
 // heads of 128, forward + backward: 256 parts 1677 us, 400 1361, 512 1660, 1024 1685). Smaller heads: three fit and a tile takes half as
 // long, 700 parts (12 x 100-1200, 16/4 heads of 64: 256 parts 254 us, 400 279, 768 256, 1536 280). Below 4 tiles a part would
-// spend longer on its f32 partials than on its tiles.
-int dkv_chunk(const Plan& p, int hq, int D, int causal) {
+// spend longer on its f32 partials than on its tiles. f32 tiles take longer: parts of any length (6 x 30-600, 8 heads of 64: 240 parts 232 us,
+// 700 210).
+int dkv_chunk(const Plan& p, int hq, int D, int causal, int dtype) {
     const long work = (causal ? p.k_work_causal : p.k_work) * hq;
-    const long parts = D > 64 ? 400 : 700, c = (work + parts - 1) / parts;
-    return (int)(c < 4 ? 4 : c > (1 << 20) ? 1 << 20 : c);
+    const long parts = dtype == PSELD_BF16 && D > 64 ? 400 : 700, c = (work + parts - 1) / parts, least = dtype == PSELD_F32 ? 1 : 4;
+    return (int)(c < least ? least : c > (1 << 20) ? 1 << 20 : c);
 }
-int dkv_splits(const Plan& p, int hq, int hkv, int D, int causal) {
-    const long longest = (p.max_q + KT - 1) / KT * (hq / hkv), c = dkv_chunk(p, hq, D, causal);
+int dkv_splits(const Plan& p, int hq, int hkv, int D, int causal, int dtype) {
+    const long longest = (p.max_q + KT - 1) / KT * (hq / hkv), c = dkv_chunk(p, hq, D, causal, dtype);
     return longest > c ? (int)((longest + c - 1) / c) : 1;
 }
 bool delta_pass(int dtype, bool table_grad) { return table_grad && dtype == PSELD_BF16; }
@@ -1101,35 +1149,38 @@ int run_fwd(PAttnArgs& a, const Plan& p, hipStream_t s) {
         return PSELD_OK;
     }
     a.tiles = a.causal ? p.q_tile_causal : p.q_tile;
-    PA_LAUNCH((packed_attn_fwd_kernel<T, DP, BIAS>), p.q_tiles * a.hq, 256, 4 * TB + dist_bytes(a), a);
+    PA_LAUNCH((packed_attn_fwd_kernel<T, DP, BIAS>), p.q_tiles * key_split<T>() * a.hq, 256, 4 * TB + dist_bytes(a), a);
     return PSELD_OK;
 }
 template <typename T, int DP, bool BIAS>
 int run_bwd(PAttnArgs& a, const Plan& p, float* dtable, int accumulate, hipStream_t s) {
     constexpr int TB = KT * DP * (int)sizeof(T);
     const int nd = dist_bytes(a);
+    const long q_tiles = p.q_tiles * key_split<T>();
+    constexpr int dtype = sizeof(T) == 2 ? PSELD_BF16 : PSELD_F32;
     a.tiles = a.causal ? p.q_tile_causal : p.q_tile;
     if constexpr (BIAS && sizeof(T) == 2) {
-        if (dtable) PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DELTA>), p.q_tiles * a.hq, 256, 4 * TB + nd, a);
+        if (dtable) PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DELTA>), q_tiles * a.hq, 256, 4 * TB + nd, a);
     }
-    if (!delta_pass(sizeof(T) == 2 ? PSELD_BF16 : PSELD_F32, BIAS && dtable)) PA_LAUNCH((packed_attn_delta_kernel<T>), (p.rows * a.hq + 15) / 16, 256, 0, a, p.rows * a.hq);
+    if (!delta_pass(dtype, BIAS && dtable)) PA_LAUNCH((packed_attn_delta_kernel<T>), (p.rows * a.hq + 15) / 16, 256, 0, a, p.rows * a.hq);
     bool table_done = false;
     if constexpr (BIAS) {
         if (dtable) {
             float* part = a.part;
-            PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ_TABLE>), p.q_tiles * a.hq, 256, (dq_buffers<T, DP, DQ_TABLE>()) * 2 * TB + 5 * nd + 64 + 4 * DIAG * 4, a);
-            PA_LAUNCH(packed_attn_table_kernel, (long)a.hq * ((a.buckets + 15) / 16), 256, 0, part, dtable, (int)p.q_tiles, a.hq, a.buckets, accumulate);
-            a.part += p.q_tiles * a.hq * a.buckets;
+            PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ_TABLE>), q_tiles * a.hq, 256, (dq_buffers<T, DP, DQ_TABLE>()) * 2 * TB + 5 * nd + 64 + 4 * DIAG * 4, a);
+            PA_LAUNCH(packed_attn_table_kernel, (long)a.hq * ((a.buckets + 15) / 16), 256, 0, part, dtable, (int)q_tiles, a.hq, a.buckets, accumulate);
+            a.part += q_tiles * a.hq * a.buckets;
             a.part = (float*)(((uintptr_t)a.part + 15) & ~(uintptr_t)15);
             table_done = true;
         }
     }
-    if (!table_done) PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ>), p.q_tiles * a.hq, 256, 4 * TB + nd, a);
+    if (!table_done) PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ>), q_tiles * a.hq, 256, 4 * TB + nd, a);
     a.tiles = a.causal ? p.k_tile_causal : p.k_tile;
-    a.nsplit = dkv_splits(p, a.hq, a.hkv, a.D, a.causal);
-    a.chunk = dkv_chunk(p, a.hq, a.D, a.causal);
-    PA_LAUNCH((packed_attn_dkv_kernel<T, DP, BIAS>), p.k_tiles * a.hkv * a.nsplit, 256, 4 * TB + 4 * KT * 4 + 4096 * (dkv_lds_frags<T, DP, BIAS>()) + nd, a);
-    if (a.nsplit > 1) PA_LAUNCH((packed_attn_dkv_join_kernel<T, DP>), p.k_tiles * a.hkv, 256, 0, a);
+    a.bias_heads = BIAS ? (DP == 128 || 2 * nd > 12288 ? 1 : min(a.hq / a.hkv, 12288 / nd)) : 0;      // (two workgroups per CU stay possible)
+    a.nsplit = dkv_splits(p, a.hq, a.hkv, a.D, a.causal, dtype);
+    a.chunk = dkv_chunk(p, a.hq, a.D, a.causal, dtype);
+    PA_LAUNCH((packed_attn_dkv_kernel<T, DP, BIAS>), p.k_tiles * a.hkv * a.nsplit, 256, 4 * TB + 4 * KT * 4 + 4096 * (dkv_lds_frags<T, DP, BIAS>()) + a.bias_heads * nd, a);
+    if (a.nsplit > 1) PA_LAUNCH((packed_attn_dkv_join_kernel<T, DP>), p.k_tiles * a.hkv * (TILE * DP / 1024), 256, 0, a);
     return PSELD_OK;
 }
 template <typename T, typename F> int by_head_size(int D, bool bias, F&& f) {
@@ -1185,8 +1236,10 @@ extern "C" int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, co
 extern "C" long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int causal, int buckets) {
     if (!plan || hkv <= 0 || hq < hkv || hq % hkv) return 0;
     const Plan p = plan_of(plan);
-    const long n = dkv_splits(p, hq, hkv, D, causal);
-    return ((p.rows * hq + 3) / 4 * 4 + p.q_tiles * hq * buckets + 4 + (n > 1 ? p.k_tiles * hkv * n * 2 * TILE * pad_of(D) : 0)) * (long)sizeof(float);
+    long n = dkv_splits(p, hq, hkv, D, causal, PSELD_BF16);
+    const long n4 = dkv_splits(p, hq, hkv, D, causal, PSELD_F32);
+    if (n4 > n) n = n4;
+    return ((p.rows * hq + 3) / 4 * 4 + 2 * p.q_tiles * hq * buckets + 4 + (n > 1 ? p.k_tiles * hkv * n * 2 * TILE * pad_of(D) : 0)) * (long)sizeof(float);
 }
 
 extern "C" int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
