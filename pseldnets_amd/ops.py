@@ -2,7 +2,9 @@
 checks shapes/dtypes, allocates outputs with torch's caching allocator and enqueues one or two HIP kernels on
 torch's current stream. CUDA tensors only — there is no CPU path."""
 import ctypes
+import functools
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -1576,16 +1578,21 @@ class PackedPlan:
     hold it to 0 .. capacity. Everything else is fixed when the plan is made."""
 
     def __init__(self, q_lens, k_lens, k_cap, device):
-        q_lens = [int(n) for n in q_lens]
-        k_lens = q_lens if k_lens is None else [int(n) for n in k_lens]
-        caps = k_lens if k_cap is None else [int(n) for n in (k_cap if hasattr(k_cap, '__iter__') else [k_cap] * len(q_lens))]
-        if not q_lens:
+        q = np.array([int(n) for n in q_lens], dtype=np.int64)
+        seqs = len(q)
+        k = q if k_lens is None else np.array([int(n) for n in k_lens], dtype=np.int64)
+        cap = k if k_cap is None else np.array([int(n) for n in (k_cap if hasattr(k_cap, '__iter__') else [k_cap] * seqs)], dtype=np.int64)
+        if not seqs:
             raise _lib.PseldError("packed_plan: no recordings")
-        if len(k_lens) != len(q_lens) or len(caps) != len(q_lens):
+        if len(k) != seqs or len(cap) != seqs:
             raise _lib.PseldError("packed_plan: q_lens, k_lens and k_cap must name the same recordings")
-        if min(q_lens) < 0 or min(k_lens) < 0 or any(n > c for n, c in zip(k_lens, caps)):
+        if q.min() < 0 or k.min() < 0 or (k > cap).any():
             raise _lib.PseldError("packed_plan: lengths must be >= 0 and at most the capacity")
-        if sum(q_lens) >= 1 << 31 or sum(caps) >= 1 << 31 or len(q_lens) > 1 << 20:
+        if q.max() >= 1 << 31 or cap.max() >= 1 << 31 or seqs > 1 << 20:       # (so that no sum below wraps)
+            raise _lib.PseldError("packed_plan: at most 2^31 - 1 rows and 2^20 recordings")
+        self.seqs, self.rows, self.max_q = seqs, int(q.sum()), int(q.max())
+        self.k_rows, self.max_k = int(cap.sum()), int(cap.max())
+        if self.rows >= 1 << 31 or self.k_rows >= 1 << 31:
             raise _lib.PseldError("packed_plan: at most 2^31 - 1 rows and 2^20 recordings")
         self.device = torch.device(device)
         if self.device.type != 'cuda':
@@ -1593,42 +1600,32 @@ class PackedPlan:
         if self.device.index is None:
             self.device = torch.device('cuda', torch.cuda.current_device())
         self._index = self.device.index
-        self.q_lens, self.k_caps = q_lens, caps
-        self.seqs, self.rows, self.max_q = len(q_lens), sum(q_lens), max(q_lens)
-        self.k_rows, self.max_k = sum(caps), max(caps)
-        T = _PACKED_TILE
-        # work lists, heaviest tile first: (recording, first row) of every 128-row tile of queries and of keys, ordered for
-        # full attention (by the other side's length) and for causal attention (by how much of the other side the mask leaves)
-        pairs = list(enumerate(zip(q_lens, caps)))
-        qf = [(-k, s, q0) for s, (q, k) in pairs for q0 in range(0, q, T)]
-        qc = [(-(k - q + q0), s, q0) for s, (q, k) in pairs for q0 in range(0, q, T)]
-        kf = [(-q, s, k0) for s, (q, k) in pairs for k0 in range(0, k, T)]
-        kc = [(-min(q, k - k0), s, k0) for s, (q, k) in pairs for k0 in range(0, k, T)]
+        q_start, k_start = np.cumsum(q) - q, np.cumsum(cap) - cap
+        # work lists, heaviest tile first: every 128-row tile of queries and of keys, ordered for full attention (by the other side's length)
+        # and for causal attention (by how much of the other side the mask leaves)
+        per = np.stack([q_start, q, k_start, cap, np.zeros_like(q), np.zeros_like(q)], 1)
+
+        def tiles(lens, full, causal):
+            n = -(-lens // _PACKED_TILE)
+            s = np.repeat(np.arange(seqs), n)
+            first = (np.arange(len(s)) - np.repeat(np.cumsum(n) - n, n)) * _PACKED_TILE
+            rec = np.concatenate([s[:, None], first[:, None], per[s]], 1)
+            weights = full(s), causal(s, first)
+            return [rec[np.argsort(-w, kind='stable')] for w in weights], weights
+        (qf, qc), _ = tiles(q, lambda s: cap[s], lambda s, first: cap[s] - q[s] + first)
+        (kf, kc), weights = tiles(cap, lambda s: q[s], lambda s, first: np.minimum(q[s], cap[s] - first))
         self.q_tiles, self.k_tiles = len(qf), len(kf)
-        host, at = [], {}
-
-        def put(name, values):
-            host.extend([0] * (-len(host) % 8))
-            at[name] = len(host)
-            host.extend(values)
-
-        def starts(lens):
-            out, n = [], 0
-            for x in lens:
-                out.append(n)
-                n += x
-            return out
-        qs, ks = starts(q_lens), starts(caps)
-        put('q_start', qs); put('q_len', q_lens); put('k_start', ks); put('k_cap', caps); put('k_len', k_lens)
-        for name, tiles in (('q_tile', qf), ('q_tile_causal', qc), ('k_tile', kf), ('k_tile_causal', kc)):
-            put(name, [x for _, s, r in sorted(tiles) for x in (s, r, qs[s], q_lens[s], ks[s], caps[s], 0, 0)])
-        self._ints = torch.tensor(host, dtype=torch.int32).to(self.device)
-        self._ptr = {k: self._ints.data_ptr() + 4 * v for k, v in at.items()}
-        self.k_len = self._ints[at['k_len']:at['k_len'] + self.seqs]
-        names = ('q_start', 'q_len', 'k_start', 'k_cap', 'k_len', 'q_tile', 'q_tile_causal', 'k_tile', 'k_tile_causal')
-        work = [sum((-w + 63) // 64 for w, _, _ in tiles if w < 0) for tiles in (kf, kc)]       # 64-query tiles that a key tile meets, summed
-        self._desc = (ctypes.c_long * 18)(self.seqs, self.rows, self.max_q, self.k_rows, self.max_k, self.q_tiles, self.k_tiles, *work,
-                                          *(self._ptr[k] for k in names))
+        work = [int((-(-np.maximum(w, 0) // 64)).sum()) for w in weights]      # 64-query tiles that a key tile meets, summed
+        host, at, end = [], {}, 0
+        for name, values in (('q_start', q_start), ('q_len', q), ('k_start', k_start), ('k_cap', cap), ('k_len', k), ('q_tile', qf),
+                             ('q_tile_causal', qc), ('k_tile', kf), ('k_tile_causal', kc)):
+            at[name] = end
+            host += [values.reshape(-1), np.zeros(-values.size % 8, dtype=np.int64)]
+            end += values.size + -values.size % 8
+        self._ints = torch.from_numpy(np.concatenate(host).astype(np.int32)).to(self.device)
+        self._ptr = {name: self._ints.data_ptr() + 4 * v for name, v in at.items()}
+        self.k_len = self._ints[at['k_len']:at['k_len'] + seqs]
+        self._desc = (ctypes.c_long * 18)(seqs, self.rows, self.max_q, self.k_rows, self.max_k, self.q_tiles, self.k_tiles, *work, *self._ptr.values())
 
 
 _PACKED_TILE = 128
@@ -1714,6 +1711,28 @@ def linrec_bwd(dh, g, n, saved, plan, dh_last=None, h0=None, reverse=False, dg=N
     return dg, dn, dh0
 
 
+@functools.lru_cache(maxsize=64)
+def _bucket_table(num_buckets, max_distance, bidirectional):
+    """(bucket of every distance -max_distance .. max_distance, first and last distance of every bucket), from the formula in whole numbers."""
+    side = num_buckets // 2 if bidirectional else num_buckets
+    e = side // 2
+    K = side - e
+    of_dist, k = [], 0
+    for n in range(max_distance + 1):
+        if n < e:
+            of_dist.append(n)
+            continue
+        while k + 1 < K and n ** K * e ** (k + 1) >= max_distance ** (k + 1) * e ** K:
+            k += 1
+        of_dist.append(e + k)
+    lut = [of_dist[-r] if r <= 0 else side + of_dist[r] if bidirectional else 0 for r in range(-max_distance, max_distance + 1)]
+    first, last = {}, {}
+    for r, b in zip(range(-max_distance, max_distance + 1), lut):
+        first.setdefault(b, r)
+        last[b] = r
+    return tuple(lut), tuple(x for b in range(num_buckets) for x in (first.get(b, 1), last.get(b, 0)))
+
+
 class RelposBuckets:
     """Buckets of relative positions (key - query) for a learned bias table [num_buckets, heads]. Bidirectional: half the buckets for keys behind
     the query and the query itself, half for keys ahead; otherwise all of them for keys behind and bucket 0 for every key ahead. The first
@@ -1728,23 +1747,9 @@ class RelposBuckets:
             raise _lib.PseldError("relpos_buckets: 2 to 512 buckets, an even number (at least 4) for both directions")
         if not e < max_distance <= 1024:
             raise _lib.PseldError(f"relpos_buckets: max_distance must lie above the {e} one-distance buckets of a side and be at most 1024")
-        K = side - e
-        of_dist, k = [], 0
-        for n in range(max_distance + 1):
-            if n < e:
-                of_dist.append(n)
-                continue
-            while k + 1 < K and n ** K * e ** (k + 1) >= max_distance ** (k + 1) * e ** K:
-                k += 1
-            of_dist.append(e + k)
-        lut = [of_dist[-r] if r <= 0 else side + of_dist[r] if bidirectional else 0 for r in range(-max_distance, max_distance + 1)]
-        first, last = {}, {}
-        for r, b in zip(range(-max_distance, max_distance + 1), lut):
-            first.setdefault(b, r)
-            last[b] = r
-        ranges = [x for b in range(num_buckets) for x in (first.get(b, 1), last.get(b, 0))]
+        lut, ranges = _bucket_table(int(num_buckets), int(max_distance), bool(bidirectional))
         self.num_buckets, self.max_distance, self.bidirectional = num_buckets, max_distance, bidirectional
-        self.host_lut = lut
+        self.host_lut = list(lut)
         self.device = torch.device(device)
         if self.device.type == 'cuda':
             if self.device.index is None:
