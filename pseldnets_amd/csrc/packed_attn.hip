@@ -160,7 +160,7 @@ __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(
 
 // Every ordinary load has landed, as a wait that the compiler's own bookkeeping sees (gfx9 encoding: vmcnt 0, expcnt 7, lgkmcnt 15). In front of each loop
 // that keeps DMAs in flight: without it the compiler waits for the operands loaded before the loop INSIDE it, at every turn, and drains the next
-// tile's DMA right after its request (1 x 12289 forward, 16/2 heads of 128: see the loop's figures).
+// tile's DMA right after its request.
 #define PA_LOADS_DONE() __builtin_amdgcn_s_waitcnt(0x0F70)
 #define PA_SYNC_TILE()                                                  \
     do {                                                                \
@@ -349,7 +349,7 @@ template <int NT> __device__ __forceinline__ void mask_rows(f32x16 (&x)[NT], int
 // hkv apart: with hkv a multiple of the eight XCDs every key head's tiles stay on one XCD's L2
 // f32 (the parity mode): an f32 matrix instruction takes 64 cycles and short recordings leave few waves, so the four waves are two groups of 32
 // rows x two halves of every key tile, joined through LDS at the end: half the rows per workgroup, half the time per tile (6 recordings of 30-600,
-// 8 heads of 64: forward 63 -> 40 us)
+// 8 heads of 64: forward 63 -> 46 us)
 template <typename T> constexpr int key_split() { return sizeof(T) == 4 ? 2 : 1; }
 struct QTile {
     int seq, q0, q_len, k_len, off, head, kvh, nk;
@@ -662,7 +662,7 @@ enum { DQ = 0, DQ_TABLE = 1, DELTA = 2 };
 // Adds a wave's 32 x 64 dS (lanes = queries) to its sums by distance; h points at the entry of distance (tile's first key - wave's first query). The
 // tile goes through LDS as [query][key]; in step q lane l reads key (q + l - 31) mod 64 of query q: over the 32 steps every element is read once, and what
 // a lane sees is one diagonal key - query = l - 31 while q + l >= 31 and one diagonal l + 33 before. (One LDS float atomic per element
-// instead took 67 cycles each: 200 us of the dq kernel for 12 recordings of 100-1200 frames, 16 heads of 64, where this takes 85.)
+// instead took 67 cycles each: 200 us of the dq kernel for 12 recordings of 100-1200 frames, 16 heads of 64; with this the kernel takes 71.)
 constexpr int DIAG_PITCH = 68, DIAG = 32 * DIAG_PITCH;      // floats; 16-byte pieces of eight rows fall in different banks
 typedef __attribute__((address_space(3))) float* lds_fptr;
 typedef __attribute__((address_space(3))) f32x4* lds_f4ptr;
@@ -880,7 +880,7 @@ __device__ __forceinline__ int dkv_parts(int total, int most, int chunk) { retur
 // waits for the next tile's DMA. Two workgroups still fit a CU's LDS.)
 template <typename T, int DP, bool BIAS> constexpr int dkv_lds_frags() { return sizeof(T) == 2 && DP == 128 ? (BIAS ? 3 : 2) : 0; }
 template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_dkv_kernel(PAttnArgs a) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && DP == 64 ? 3 : waves_per_simd<T, DP>())) void packed_attn_dkv_kernel(PAttnArgs a) {
     using I = Image<T, DP>;
     constexpr int TB = KT * I::RB;
     constexpr bool TIGHT = DP == 128;
@@ -1086,14 +1086,13 @@ int few_chunk(const Plan& p, int hkv) {
 }
 int few_splits(const Plan& p, int hkv) { const int c = few_chunk(p, hkv); return p.max_k > c ? (int)((p.max_k + c - 1) / c) : 1; }
 // Query tiles per workgroup of the dk/dv kernel: the whole work is cut into equal parts where the key tiles alone would not fill the chip or end
-// unevenly. Heads above 64: two workgroups fit a CU, 400 parts (a few of the 512 places stay free for the tiles' odd ends; 1 x 8191, 16/2
-// heads of 128, forward + backward: 256 parts 1677 us, 400 1361, 512 1660, 1024 1685). Smaller heads: three fit and a tile takes half as
-// long, 700 parts (12 x 100-1200, 16/4 heads of 64: 256 parts 254 us, 400 279, 768 256, 1536 280). Below 4 tiles a part would
-// spend longer on its f32 partials than on its tiles. f32 tiles take longer: parts of any length (6 x 30-600, 8 heads of 64: 240 parts 232 us,
-// 700 210).
+// unevenly: as many as about four fifths of the places (the tiles' odd ends take the rest), so that all run at once. Two workgroups fit a CU at heads
+// above 64 (1 x 8191, 16/2 heads of 128, forward + backward: 256 parts 1677 us, 400 1361, 512 1660, 1024 1685), three below (12 x 100-1200, 16/4
+// heads of 64: 500 parts 233 us, 600 206, 700 221, 1400 218). Below 4 tiles a part would spend longer on its f32 partials than on its tiles. f32
+// tiles take longer: parts of any length (6 x 30-600, 8 heads of 64: 240 parts 232 us, 700 210).
 int dkv_chunk(const Plan& p, int hq, int D, int causal, int dtype) {
     const long work = (causal ? p.k_work_causal : p.k_work) * hq;
-    const long parts = dtype == PSELD_BF16 && D > 64 ? 400 : 700, c = (work + parts - 1) / parts, least = dtype == PSELD_F32 ? 1 : 4;
+    const long parts = dtype == PSELD_F32 ? 700 : D > 64 ? 400 : 600, c = (work + parts - 1) / parts, least = dtype == PSELD_F32 ? 1 : 4;
     return (int)(c < least ? least : c > (1 << 20) ? 1 << 20 : c);
 }
 int dkv_splits(const Plan& p, int hq, int hkv, int D, int causal, int dtype) {
