@@ -327,6 +327,10 @@ template <int DP> struct Softmax {
     }
 };
 
+// A row's sum is 0 only where it has no keys (or -inf scores alone); a NaN goes on into out and lse
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -__builtin_inff() : (m + __log2f(l)) * LN2; }
+
 // Where a tile's scores start: from their diagonals' bias; d points at the entry of (accumulator row 0, this lane's column)
 template <int NT, int SIGN> __device__ __forceinline__ void start_near(f32x16 (&x)[NT], const float* d) {
 #pragma unroll
@@ -464,8 +468,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
         sm.m = mn;
     }
     const float l = sm.l + __shfl_xor(sm.l, 32, 64);
-    store_rows<T, DP>(a.out + qrow * a.so.rs + (long)w.head * a.so.hs, live, sm.ot, l > 0.f ? 1.f / l : 0.f, a.D, h2);
-    if (live && h2 == 0) a.lse[qrow * a.hq + w.head] = l > 0.f ? (sm.m + __log2f(l)) * LN2 : -__builtin_inff();
+    store_rows<T, DP>(a.out + qrow * a.so.rs + (long)w.head * a.so.hs, live, sm.ot, inverse(l), a.D, h2);
+    if (live && h2 == 0) a.lse[qrow * a.hq + w.head] = lse_of(sm.m, l);
 }
 
 // ---- few rows: a step of running streams ------------------------------------------------------------------------------------------------
@@ -557,7 +561,7 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
 #pragma unroll
     for (int x = 0; x < NW; ++x) mt = fmaxf(mt, ml[x * 64 + r]);
 #pragma unroll
-    for (int x = 0; x < NW; ++x) { const float mx = ml[x * 64 + r]; lt += mx == -__builtin_inff() ? 0.f : ml[x * 64 + 32 + r] * __builtin_amdgcn_exp2f(mx - mt); }
+    for (int x = 0; x < NW; ++x) { const float mx = ml[x * 64 + r]; lt += ml[x * 64 + 32 + r] * (mx == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mx - mt)); }
     const float f = sm.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sm.m - mt);
     constexpr int PITCH = DP + 4;                          // floats per row of a wave's output image: 32 rows of 4-float pieces fall in different banks
     static_assert(32 * PITCH * 4 <= 4 * BB, "the output image fits the wave's buffers");
@@ -583,9 +587,9 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
         } else {
             const int qj = row / G, head = kvh * G + row - qj * G;
             const long qr = (long)a.q_start[seq] + qj;
-            const float inv = lr > 0.f ? 1.f / lr : 0.f;
+            const float inv = inverse(lr);
             store4<T>(a.out + qr * a.so.rs + (long)head * a.so.hs + d * (int)sizeof(T), s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
-            if (d == 0) a.lse[qr * a.hq + head] = lr > 0.f ? (m + __log2f(lr)) * LN2 : -__builtin_inff();
+            if (d == 0) a.lse[qr * a.hq + head] = lse_of(m, lr);
         }
     }
 }
@@ -611,7 +615,7 @@ __global__ __launch_bounds__(64) void packed_attn_join_kernel(PAttnArgs a) {
     }
     l = wave_sum(l);
     __syncthreads();
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = inverse(l);
     const int qj = row / G, head = kvh * G + row - qj * G;
     const long qr = (long)a.q_start[seq] + qj;
     // 16-lane groups take the chunks in turn, 8 elements a lane; the four groups' sums meet by shuffles
@@ -634,7 +638,7 @@ __global__ __launch_bounds__(64) void packed_attn_join_kernel(PAttnArgs a) {
         s[j] *= inv;
     }
     if (grp == 0 && dl < a.D) store8<T>((T*)(a.out + qr * a.so.rs + (long)head * a.so.hs) + dl, s);
-    if (lane == 0) a.lse[qr * a.hq + head] = l > 0.f ? (m + __log2f(l)) * LN2 : -__builtin_inff();
+    if (lane == 0) a.lse[qr * a.hq + head] = lse_of(m, l);
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------------------
@@ -736,7 +740,7 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
     }
     const long si = qrow * a.hq + w.head;
     const float lse = a.lse[si];
-    const float lse2 = live && lse > -__builtin_inff() ? lse * LOG2E : __builtin_inff();      // +inf: every probability of the row is 0
+    const float lse2 = live && lse != -__builtin_inff() ? lse * LOG2E : __builtin_inff();      // +inf: every probability of the row is 0 (a NaN stays one)
     float dl = 0.f;
     if constexpr (MODE != DELTA) dl = a.delta[si];
     const int qpos = qi + w.off, qw0 = w.q0 + rg * WR + w.off;
@@ -944,7 +948,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP == 64 ? 3 : waves_per_si
             float* ls = stat + par * 2 * KT;
             if (threadIdx.x < 2 * KT) {                    // rows past the end and rows without keys: probabilities 0
                 const bool in = q0 + ((int)threadIdx.x & (KT - 1)) < q_len;
-                ls[threadIdx.x] = threadIdx.x < KT ? (in && reg > -__builtin_inff() ? reg * LOG2E : __builtin_inff()) : in ? -reg : 0.f;
+                ls[threadIdx.x] = threadIdx.x < KT ? (in && reg != -__builtin_inff() ? reg * LOG2E : __builtin_inff()) : in ? -reg : 0.f;
             }
             if constexpr (BIAS) {
                 if (!all && g != held) {                   // uniform; the last tile's readers are past the barrier below before anything is overwritten

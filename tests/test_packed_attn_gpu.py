@@ -513,3 +513,22 @@ def test_c_entry_refuses_without_a_launch():
     assert b"workspace" in L.pseld_last_error()
     assert L.pseld_packed_attn_bwd(0, A, A, A, A, A, A, A, A, A, st, plan, 4, 4, 64, 0, 1.0, None, None, 0, 0, A, 0, A, 1 << 30, None) == -1
     assert L.pseld_packed_attn_bwd(0, A, A, A, A, A, A, A, A, A, st, plan, 4, 4, 64, 0, 1.0, None, None, 0, 0, None, 0, A, 16, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("q_lens,k_lens,row", [([70, 200], None, 130), ([1, 1, 1], [9, 600, 300], 1), ([1, 1], [4000, 90], 0)])
+def test_a_nan_query_shows_in_its_own_row_alone(dev, dtype, q_lens, k_lens, row):
+    """Whole recordings, few rows in one chunk and in many: out, lse and dq of the (row, head) are NaN, every other row's are not."""
+    from pseldnets_amd import ops
+    plan = ops.packed_plan(q_lens, k_lens, device=dev)
+    q, dout = rnd((plan.rows, 4, 64), 1, dtype, dev), rnd((plan.rows, 4, 64), 2, dtype, dev)
+    k, v = rnd((plan.k_rows, 2, 64), 3, dtype, dev), rnd((plan.k_rows, 2, 64), 4, dtype, dev)
+    q[row, 1, 5] = float('nan')
+    out, lse = ops.packed_attn_fwd(q, k, v, plan, causal=True)
+    dq, _, _ = ops.packed_attn_bwd(dout, q, k, v, out, lse, plan, causal=True)
+    want = torch.zeros(plan.rows, 4, dtype=torch.bool, device=dev)
+    want[row, 1] = True
+    assert torch.equal(torch.isnan(lse), want) and not torch.isinf(lse).any()
+    for t in (out, dq):
+        assert torch.equal(torch.isnan(t).all(-1), want) and torch.equal(torch.isnan(t).any(-1), want)
