@@ -490,7 +490,8 @@ int pseld_gru_gate_bwd(int dtype, const void* dh, long dh_stride, const void* ca
  * z = sigmoid(g), h_t = z_t h_{t-1} + (1 - z_t) n_t per channel: nn.GRU's update rule (model_utilities.py:249-252) without the recurrent
  * product, so the frames of a recording compose in parallel. Recordings lie back to back: recording s is rows start[s] .. start[s] + len[s]
  * (device int arrays, seqs of each; rows = the sum of the lengths, max_len the longest, both host values). g, n, h rows at strides ldg, ldn, ldh
- * (multiples of 4 elements below 2^23, addresses on 4-element boundaries), C a multiple of 8. reverse: every recording runs from its last row to its first.
+ * (multiples of 4 elements below 2^23, addresses on 4-element boundaries), C a multiple of 8; at most 2^30 rows. Results must
+ * not overlap operands. reverse: every recording runs from its last row to its first.
  * h0 [seqs, C] (NULL: zeros) -> h and h_last [seqs, C] (= h0 for an empty recording). states: f32 [pseld_linrec_states(rows, seqs), C], what the
  * backward needs besides g and n (NULL: not wanted). bwd: dh, dh_last (NULL: zeros) -> dg, dn, dh0 (NULL: not wanted). All state
  * arrays are f32. workspace: pseld_linrec_workspace bytes (0: none needed). Deterministic. */
@@ -514,7 +515,7 @@ int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void* g, long l
  * causal, then device int arrays as addresses: q_start[seqs], q_len[seqs], k_start[seqs], k_cap[seqs], k_len[seqs], q_tile[q_tiles][8], q_tile_causal, k_tile[k_tiles][8], k_tile_causal}: a tile is 128 rows
  * of queries or of capacity, {recording s, first row, q_start[s], q_len[s], k_start[s], k_cap[s], 0, 0}, heaviest first. k_len may change between calls; it is held to 0 .. k_cap.
  * strides: HOST array of longs, {row stride, head stride} in elements of q, k, v, out (bwd: dout, q, k, v, out, dq, dk, dv), whole
- * 16-byte pieces; unit stride inside a head. table f32 [buckets, hq] or NULL; lut (device ints): the bucket of every distance
+ * 16-byte pieces; unit stride inside a head. At most 2^30 rows and key rows; results must not overlap operands. table f32 [buckets, hq] or NULL; lut (device ints): the bucket of every distance
  * -max_distance .. max_distance, then [buckets][2] first and last distance of each (none: first > last).
  * bwd: dq, dk, dv (rows between k_len and k_cap get zeros) and, where dtable is not NULL, dtable (f32, accumulate: added to). With bf16 operands and a
  * table gradient the sums that enter it are formed from f32 probabilities. Deterministic (no floating atomics between lanes).

@@ -417,10 +417,13 @@ void launch(LinrecArgs a, int backward, hipStream_t s) {
 
 int go(const char* name, int dtype, LinrecArgs& a, long rows, int max_len, const float* ws, long ws_bytes, int backward, void* stream) {
     PSELD_CHECK_ARG(dtype == PSELD_F32 || dtype == PSELD_BF16, "%s: unknown dtype", name);
-    PSELD_CHECK_ARG(a.start && a.len && a.seqs > 0 && rows >= 0 && max_len >= 0 && max_len <= rows, "%s: bad recordings", name);
+    PSELD_CHECK_ARG(a.start && a.len && a.seqs > 0 && rows >= 0 && rows <= (1l << 30) && max_len >= 0 && max_len <= rows, "%s: bad recordings", name);
     PSELD_CHECK_ARG(a.C > 0 && a.C % 8 == 0, "%s: channels must be a positive multiple of 8", name);
     const long need = agg_bytes_of(rows, a.seqs, max_len, a.C);
     PSELD_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "%s: workspace too small", name);
+    const void* const results[] = {a.h, a.dg, a.dn};
+    for (const void* r : results) PSELD_CHECK_ARG(!r || (r != a.g && r != a.n && r != a.dh), "%s: a result must not be an operand", name);
+    PSELD_CHECK_ARG(!a.dg || a.dg != a.dn, "%s: dg and dn must not be the same memory", name);
     a.slabs = (a.C + SLAB - 1) / SLAB;
     a.seg_len = seg_len_of(rows, max_len, a.C);
     a.nseg = max_len > a.seg_len ? (max_len + a.seg_len - 1) / a.seg_len : 1;
@@ -430,6 +433,8 @@ int go(const char* name, int dtype, LinrecArgs& a, long rows, int max_len, const
     PSELD_LAUNCH_CHECK(name);
     return PSELD_OK;
 }
+// rows of a result must not overlap
+bool apart(long ld, long rows, int C) { return rows <= 1 || ld >= C; }
 bool quads(const void* p, long ld, int dtype) { return ((uintptr_t)p & (dtype == PSELD_BF16 ? 7 : 15)) == 0 && (ld & 3) == 0 && ld >= 0 && ld < (1l << 23); }
 
 }  // namespace
@@ -444,6 +449,7 @@ extern "C" int pseld_linrec_fwd(int dtype, const void* g, long ldg, const void* 
                                 float* workspace, long workspace_bytes, void* stream) {
     PSELD_CHECK_ARG(h_last && (rows == 0 || (g && n && h)), "linrec_fwd: null pointer");
     PSELD_CHECK_ARG(quads(g, ldg, dtype) && quads(n, ldn, dtype) && quads(h, ldh, dtype), "linrec_fwd: rows must start on 4-element boundaries, less than 2^23 elements apart");
+    PSELD_CHECK_ARG(apart(ldh, rows, C), "linrec_fwd: the rows of h overlap");
     LinrecArgs a{};
     a.g = g; a.ldg = ldg; a.n = n; a.ldn = ldn; a.h0 = h0; a.h = h; a.ldh = ldh; a.h_last = h_last; a.states = states; a.agg = workspace;
     a.start = start; a.len = len; a.seqs = seqs; a.C = C; a.reverse = reverse;
@@ -456,6 +462,7 @@ extern "C" int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void
     PSELD_CHECK_ARG(rows == 0 || (dh && g && n && dg && dn && states), "linrec_bwd: null pointer");
     PSELD_CHECK_ARG(quads(dh, lddh, dtype) && quads(g, ldg, dtype) && quads(n, ldn, dtype) && quads(dg, lddg, dtype) && quads(dn, lddn, dtype),
                     "linrec_bwd: rows must start on 4-element boundaries, less than 2^23 elements apart");
+    PSELD_CHECK_ARG(apart(lddg, rows, C) && apart(lddn, rows, C), "linrec_bwd: the rows of dg or dn overlap");
     LinrecArgs a{};
     a.dh = dh; a.lddh = lddh; a.g = g; a.ldg = ldg; a.n = n; a.ldn = ldn; a.states = const_cast<float*>(states); a.dlast = dh_last;
     a.dg = dg; a.lddg = lddg; a.dn = dn; a.lddn = lddn; a.dh0 = dh0; a.agg = workspace;

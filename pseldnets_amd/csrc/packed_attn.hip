@@ -1081,12 +1081,12 @@ constexpr int FEW_TABLE = 4096;          // table entries of one key head's grou
 bool few_rows(const Plan& p, int hq, int hkv, int buckets) { return p.max_q * (hq / hkv) <= WR && (long)buckets * (hq / hkv) <= FEW_TABLE; }
 // keys per workgroup: two workgroups per CU by the capacities, whole rounds of the four waves' blocks (3 streams of 60-131 k keys, 16/4 heads of
 // 64: 2048 workgroups 73 us, 1024 72, 512 68; 48 of 100-4096, 16/2 heads of 128: 48, 34, 33); a recording of up to 512 keys stays
-// whole (one launch instead of two)
+// whole (one launch instead of two). At most 16384 chunks, whose weights fit the joining launch's LDS.
 int few_chunk(const Plan& p, int hkv) {
     if (p.max_k <= 512) return 512;
     const long want = (p.k_rows * hkv + 511) / 512;
-    const long c = (want + 127) / 128 * 128;
-    return (int)(c < 256 ? 256 : c > 8192 ? 8192 : c);
+    const long c = (want + 127) / 128 * 128, least = (p.max_k + 16383) / 16384 > 256 ? (p.max_k + 16383) / 16384 : 256, most = least > 8192 ? least : 8192;
+    return (int)((c < least ? least : c > most ? most : c) + 127) / 128 * 128;
 }
 int few_splits(const Plan& p, int hkv) { const int c = few_chunk(p, hkv); return p.max_k > c ? (int)((p.max_k + c - 1) / c) : 1; }
 // Query tiles per workgroup of the dk/dv kernel: the whole work is cut into equal parts where the key tiles alone would not fill the chip or end
@@ -1105,9 +1105,10 @@ int dkv_splits(const Plan& p, int hq, int hkv, int D, int causal, int dtype) {
 }
 bool delta_pass(int dtype, bool table_grad) { return table_grad && dtype == PSELD_BF16; }
 
+#define PA_TRY(x) do { const int rc__ = (x); if (rc__) return rc__; } while (0)
 int check(const char* name, int dtype, const Plan& p, int hq, int hkv, int D, float scale, const float* table, const int* lut, int buckets, int maxd) {
     PSELD_CHECK_ARG(dtype == PSELD_F32 || dtype == PSELD_BF16, "%s: unknown dtype", name);
-    PSELD_CHECK_ARG(p.seqs > 0 && p.rows >= 0 && p.k_rows >= 0 && p.max_q >= 0 && p.max_k >= 0 && p.q_start && p.q_len && p.k_start && p.k_cap && p.k_len, "%s: bad plan", name);
+    PSELD_CHECK_ARG(p.seqs > 0 && p.rows >= 0 && p.k_rows >= 0 && p.max_q >= 0 && p.max_k >= 0 && p.rows <= (1l << 30) && p.k_rows <= (1l << 30) && p.q_start && p.q_len && p.k_start && p.k_cap && p.k_len, "%s: bad plan", name);
     PSELD_CHECK_ARG(hkv > 0 && hq >= hkv && hq % hkv == 0 && hq <= 1024, "%s: query heads must be a multiple of the key heads, at most 1024", name);
     PSELD_CHECK_ARG(D > 0 && D % 8 == 0 && D <= 128, "%s: head sizes are multiples of 8 up to 128", name);
     PSELD_CHECK_ARG(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", name);
@@ -1123,8 +1124,15 @@ int check_operand(const char* name, const char* what, int dtype, const void* ptr
     out.hs = st[1] * e;
     return PSELD_OK;
 }
+// a result: its (row, head) vectors must not overlap, rows outside heads or heads outside rows
+int check_result(const char* name, const char* what, int dtype, const void* ptr, const long* st, Strides& out, long rows, int heads, int D) {
+    PA_TRY(check_operand(name, what, dtype, ptr, st, out, rows > 0));
+    const bool row_major = (rows <= 1 || st[0] >= (heads - 1) * st[1] + D) && (heads <= 1 || st[1] >= D);
+    const bool head_major = (heads <= 1 || st[1] >= (rows - 1) * st[0] + D) && (rows <= 1 || st[0] >= D);
+    PSELD_CHECK_ARG(row_major || head_major, "%s: the rows of %s overlap", name, what);
+    return PSELD_OK;
+}
 
-#define PA_TRY(x) do { const int rc__ = (x); if (rc__) return rc__; } while (0)
 #define PA_LAUNCH(kernel, grid, block, lds, ...)                                                                             \
     do {                                                                                                                     \
         const long g__ = (grid);                                                                                             \
@@ -1220,10 +1228,11 @@ extern "C" int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, co
     PA_TRY(check_operand("packed_attn_fwd", "q", dtype, q, strides, a.sq, rows));
     PA_TRY(check_operand("packed_attn_fwd", "k", dtype, k, strides + 2, a.sk, keys));
     PA_TRY(check_operand("packed_attn_fwd", "v", dtype, v, strides + 4, a.sv, keys));
-    PA_TRY(check_operand("packed_attn_fwd", "out", dtype, out, strides + 6, a.so, rows));
+    PA_TRY(check_result("packed_attn_fwd", "out", dtype, out, strides + 6, a.so, p.rows, hq, D));
     PSELD_CHECK_ARG(!rows || lse, "packed_attn_fwd: null pointer (lse)");
     const long need = pseld_packed_attn_fwd_workspace(plan, hq, hkv, D, table ? buckets : 0);
     PSELD_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "packed_attn_fwd: workspace too small");
+    PSELD_CHECK_ARG(!rows || (out != q && out != k && out != v), "packed_attn_fwd: out must not be an operand");
     if (!rows) return PSELD_OK;
     a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.out = (char*)out; a.lse = lse; a.part = workspace;
     fill(a, p, hq, hkv, D, causal, scale, table, lut, buckets, max_distance);
@@ -1261,9 +1270,14 @@ extern "C" int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q,
     PA_TRY(check_operand(n, "k", dtype, k, strides + 4, a.sk, keys));
     PA_TRY(check_operand(n, "v", dtype, v, strides + 6, a.sv, keys));
     PA_TRY(check_operand(n, "out", dtype, out, strides + 8, a.so, rows));
-    PA_TRY(check_operand(n, "dq", dtype, dq, strides + 10, a.sdq, rows));
-    PA_TRY(check_operand(n, "dk", dtype, dk, strides + 12, a.sdk, keys));
-    PA_TRY(check_operand(n, "dv", dtype, dv, strides + 14, a.sdv, keys));
+    PA_TRY(check_result(n, "dq", dtype, dq, strides + 10, a.sdq, p.rows, hq, D));
+    PA_TRY(check_result(n, "dk", dtype, dk, strides + 12, a.sdk, p.k_rows, hkv, D));
+    PA_TRY(check_result(n, "dv", dtype, dv, strides + 14, a.sdv, p.k_rows, hkv, D));
+    const void* const results[] = {dq, dk, dv};
+    for (int i = 0; i < 3; ++i) {
+        const void* const others[] = {dout, q, k, v, out, results[(i + 1) % 3]};
+        for (const void* x : others) PSELD_CHECK_ARG(!x || x != results[i], "%s: a gradient must not be an operand or another gradient", n);
+    }
     PSELD_CHECK_ARG(!rows || lse, "packed_attn_bwd: null pointer (lse)");
     const long need = pseld_packed_attn_bwd_workspace(plan, hq, hkv, D, causal, dtable ? buckets : 0);
     PSELD_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, "packed_attn_bwd: workspace too small");

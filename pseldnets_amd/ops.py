@@ -1575,7 +1575,7 @@ class PackedPlan:
     """Recordings of different lengths laid back to back: recording s holds rows q_start[s] .. q_start[s] + q_lens[s] of every [rows, ...] tensor.
     Keys and values lie the same way with their own lengths, or in slabs of a fixed capacity (a cache) of which the first k_len[s] rows
     count. k_len is a device tensor: a stream that appends a frame to its slab adds to it in place (also inside a captured graph); the kernels
-    hold it to 0 .. capacity. Everything else is fixed when the plan is made."""
+    hold it to 0 .. capacity. Everything else is fixed when the plan is made. At most 2^30 rows and key rows; a captured graph needs its plan kept alive."""
 
     def __init__(self, q_lens, k_lens, k_cap, device):
         q = np.array([int(n) for n in q_lens], dtype=np.int64)
@@ -1588,12 +1588,12 @@ class PackedPlan:
             raise _lib.PseldError("packed_plan: q_lens, k_lens and k_cap must name the same recordings")
         if q.min() < 0 or k.min() < 0 or (k > cap).any():
             raise _lib.PseldError("packed_plan: lengths must be >= 0 and at most the capacity")
-        if q.max() >= 1 << 31 or cap.max() >= 1 << 31 or seqs > 1 << 20:       # (so that no sum below wraps)
-            raise _lib.PseldError("packed_plan: at most 2^31 - 1 rows and 2^20 recordings")
+        if q.max() > 1 << 30 or cap.max() > 1 << 30 or seqs > 1 << 20:       # (so that no sum below wraps)
+            raise _lib.PseldError("packed_plan: at most 2^30 rows and 2^20 recordings")
         self.seqs, self.rows, self.max_q = seqs, int(q.sum()), int(q.max())
         self.k_rows, self.max_k = int(cap.sum()), int(cap.max())
-        if self.rows >= 1 << 31 or self.k_rows >= 1 << 31:
-            raise _lib.PseldError("packed_plan: at most 2^31 - 1 rows and 2^20 recordings")
+        if self.rows > 1 << 30 or self.k_rows > 1 << 30:
+            raise _lib.PseldError("packed_plan: at most 2^30 rows and 2^20 recordings")
         self.device = torch.device(device)
         if self.device.type != 'cuda':
             raise _lib.PseldError("packed_plan: the plan must live on the MI355X (no CPU fallback)")
@@ -1672,7 +1672,7 @@ def _linrec_ws(plan, C):
 
 def linrec_fwd(g, n, plan, h0=None, reverse=False, need_saved=True, out=None):
     """z = sigmoid(g), h_t = z_t h_{t-1} + (1 - z_t) n_t over every recording of the plan (from its last frame to its first when
-    reverse). g, n [rows, C] (row-strided views allowed), h0 f32 [recordings, C] or None (zeros).
+    reverse). g, n [rows, C] (row-strided views allowed; out must not overlap them), h0 f32 [recordings, C] or None (zeros).
     Returns (h [rows, C], h_last f32 [recordings, C], what linrec_bwd needs or None)."""
     stream = _on_plan("linrec_fwd", plan)
     _rows_ok("linrec_fwd", plan, g.shape, g.dtype, g, n, out)
@@ -1798,7 +1798,8 @@ def packed_attn_fwd(q, k, v, plan, causal=False, scale=None, bias_table=None, bu
     of a cache allowed; query heads a multiple of key heads) -> (out [rows, query heads, D], lse f32 [rows, query heads]). Query i of a recording
     stands at position i + k_len - q_len; causal masks the keys behind a query's position. A row without keys gives 0 and -inf. scale: D^-1/2 where None.
     bias_table f32 [buckets, query heads] with buckets = relpos_buckets(...): bias_table[bucket(key position - query position), head]
-    is added to the scaled scores. Key rows past a recording's k_len are never read."""
+    is added to the scaled scores (-inf masks a bucket; finite entries stay below 1e37 scale). Key rows past a recording's k_len are never read. A value that
+    is not finite reaches, times a probability of 0, also the rows of its 64-key tile whose mask hides it. out must not overlap the operands."""
     stream = _on_plan("packed_attn_fwd", plan)
     dtype, hq, hkv, D, scale = _packed_attn_args("packed_attn_fwd", plan, q, k, v, scale, bias_table, buckets)
     L = _lib.lib()
@@ -1824,7 +1825,7 @@ def packed_attn_fwd(q, k, v, plan, causal=False, scale=None, bias_table=None, bu
 def packed_attn_bwd(dout, q, k, v, out, lse, plan, causal=False, scale=None, bias_table=None, buckets=None, dbias_table=None, accumulate=False,
                     dq=None, dk=None, dv=None):
     """Gradients of packed_attn_fwd (same plan, lengths and options; out and lse are what it returned): (dq, dk, dv). dbias_table f32 [buckets, query heads]:
-    written (accumulate: added to) where given. dq, dk, dv: optional outputs (e.g. the parts of the projection's gradient)."""
+    written (accumulate: added to) where given. dq, dk, dv: optional outputs (e.g. the parts of the projection's gradient), apart from the operands."""
     what = "packed_attn_bwd"
     stream = _on_plan(what, plan)
     dtype, hq, hkv, D, scale = _packed_attn_args(what, plan, q, k, v, scale, bias_table, buckets)

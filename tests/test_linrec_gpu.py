@@ -240,6 +240,25 @@ def test_c_entry_refuses_without_a_launch():
     assert L.pseld_linrec_workspace(60000, 2, 60000, 512) > 0 and L.pseld_linrec_workspace(100, 4, 40, 64) == 0
 
 
+def test_c_entry_refuses_overlapping_results_and_too_many_rows():
+    import os
+    from pseldnets_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("libpseld_hip.so not built")
+    L = _lib.lib()
+    P, Q, R, S = (4096 * i for i in range(1, 5))            # addresses that are never followed
+
+    def fwd(h=R, ldh=8, rows=4, longest=4):
+        return L.pseld_linrec_fwd(0, P, 8, Q, 8, None, h, ldh, P, None, P, P, 1, rows, longest, 8, 0, None, 0, None)
+
+    def bwd(dg=S, lddg=8, dn=5 * 4096, lddn=8):
+        return L.pseld_linrec_bwd(0, R, 8, P, 8, Q, 8, P, None, dg, lddg, dn, lddn, None, P, P, 1, 4, 4, 8, 0, None, 0, None)
+    for bad in (dict(h=P), dict(h=Q), dict(ldh=4), dict(ldh=0), dict(rows=(1 << 30) + 1)):
+        assert fwd(**bad) == -1, bad
+    for bad in (dict(dg=P), dict(dg=Q), dict(dg=R), dict(dn=P), dict(dn=Q), dict(dn=R), dict(dn=S), dict(lddg=4), dict(lddn=0)):
+        assert bwd(**bad) == -1, bad
+
+
 def test_plan_fails_loudly_without_gpu():
     import torch as t
     from pseldnets_amd import _lib, ops

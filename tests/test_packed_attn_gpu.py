@@ -515,6 +515,45 @@ def test_c_entry_refuses_without_a_launch():
     assert L.pseld_packed_attn_bwd(0, A, A, A, A, A, A, A, A, A, st, plan, 4, 4, 64, 0, 1.0, None, None, 0, 0, None, 0, A, 16, None) == -1
 
 
+def test_c_entry_refuses_overlapping_results_and_too_many_rows():
+    import ctypes
+    import os
+    from pseldnets_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("libpseld_hip.so not built")
+    L = _lib.lib()
+    A = [4096 * i for i in range(1, 12)]                     # addresses that are never followed
+
+    def plan(rows=40, k_rows=40):
+        return (ctypes.c_long * 18)(1, rows, min(rows, 40), k_rows, min(k_rows, 40), 1, 1, 1, 1, *[4096] * 9)
+
+    def fwd(out=A[3], so=(256, 64), p=plan()):
+        return L.pseld_packed_attn_fwd(0, A[0], A[1], A[2], out, A[9], (ctypes.c_long * 8)(*[256, 64] * 3, *so), p, 4, 4, 64, 0, 1.0, None, None, 0, 0, None, 0, None)
+
+    def bwd(dq=A[5], dk=A[6], dv=A[7], sdq=(256, 64), sdk=(256, 64)):
+        return L.pseld_packed_attn_bwd(0, A[4], A[0], A[1], A[2], A[3], A[9], dq, dk, dv, (ctypes.c_long * 16)(*[256, 64] * 5, *sdq, *sdk, 256, 64), plan(), 4, 4, 64,
+                                       0, 1.0, None, None, 0, 0, None, 0, A[10], 1 << 30, None)
+    for bad in (dict(out=A[0]), dict(out=A[1]), dict(out=A[2]), dict(so=(0, 64)), dict(so=(192, 64)), dict(so=(256, 0)), dict(so=(64, 64)), dict(so=(64, 2496)),
+                dict(p=plan(rows=(1 << 30) + 1)), dict(p=plan(k_rows=(1 << 30) + 1))):
+        assert fwd(**bad) == -1, bad
+    for bad in (dict(dq=A[0]), dict(dk=A[1]), dict(dv=A[2]), dict(dq=A[4]), dict(dq=A[3]), dict(dk=A[5]), dict(dv=A[6]), dict(dv=A[5]), dict(sdq=(0, 64)), dict(sdk=(128, 32))):
+        assert bwd(**bad) == -1, bad
+
+
+def test_chunks_of_the_longest_caches_stay_joinable():
+    """The joining launch keeps one weight per chunk of a recording's keys in LDS: 64 KB at most."""
+    import ctypes
+    import os
+    from pseldnets_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("libpseld_hip.so not built")
+    for keys in (1000, 100_000, 131_072, 50_000_000, 400_000_000, 1 << 30):
+        for hkv in (1, 16):
+            plan = (ctypes.c_long * 18)(1, 1, 1, keys, keys, 1, (keys + 127) // 128, 1, 1, *[4096] * 9)
+            chunks = _lib.lib().pseld_packed_attn_fwd_workspace(plan, hkv, hkv, 64, 0) // (hkv * 68 * 4)
+            assert 1 <= chunks <= 16384
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("q_lens,k_lens,row", [([70, 200], None, 130), ([1, 1, 1], [9, 600, 300], 1), ([1, 1], [4000, 90], 0)])
