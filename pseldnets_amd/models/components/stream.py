@@ -32,7 +32,7 @@ class StreamDecoder:
         self.kv_heads = self.heads // 4 if self.heads % 4 == 0 else self.heads
         self.W = (self.heads + 2 * self.kv_heads) * self.hd
         self.num_buckets, self.max_distance = num_buckets, max_distance
-        self._buckets = self._plan = None
+        self._buckets, self._plans = {}, {}      # never dropped: a captured graph goes on reading them
         for li in range(num_layers):
             b = f'{prefix}layers.{li}.'
             arena.add(b + 'norm1.weight', (dim,)); arena.add(b + 'norm1.bias', (dim,))
@@ -47,9 +47,9 @@ class StreamDecoder:
         return {}
 
     def _relpos(self, device):
-        if self._buckets is None or self._buckets.device != device:
-            self._buckets = ops.relpos_buckets(self.num_buckets, self.max_distance, bidirectional=False, device=device)
-        return self._buckets
+        if device not in self._buckets:
+            self._buckets[device] = ops.relpos_buckets(self.num_buckets, self.max_distance, bidirectional=False, device=device)
+        return self._buckets[device]
 
     def _heads(self, qkv):
         n, hq, hk, d = qkv.shape[0], self.heads, self.kv_heads, self.hd
@@ -59,9 +59,9 @@ class StreamDecoder:
     def forward(self, x, B, T, training=None, buffers=None):
         """x [B*T, D], B chunks of T frames -> [B*T, D]."""
         key = (B, T, x.device)
-        if self._plan is None or self._plan[0] != key:
-            self._plan = (key, ops.packed_plan([T] * B, device=x.device))
-        return self.forward_packed(x, self._plan[1])
+        if key not in self._plans:
+            self._plans[key] = ops.packed_plan([T] * B, device=x.device)
+        return self.forward_packed(x, self._plans[key])
 
     def forward_packed(self, x, plan):
         """x [rows, D]: the plan's recordings back to back -> [rows, D]."""
@@ -120,6 +120,8 @@ class StreamDecoder:
         caches and states move on in place."""
         if state.frames >= state.capacity:
             raise _lib.PseldError(f"stream decoder: the streams' caches hold {state.capacity} frames and are full")
+        if x.shape != (state.plan.seqs, self.D) or x.dtype != state.keys[0].dtype or x.device != state.plan.device:
+            raise _lib.PseldError(f"stream decoder: a frame of these streams is {state.keys[0].dtype} [{state.plan.seqs}, {self.D}] on {state.plan.device}")
         state.frames += 1
         a, dt, D, plan = self.arena, x.dtype, self.D, state.plan
         buckets = self._relpos(x.device)

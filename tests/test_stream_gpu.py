@@ -145,3 +145,34 @@ def test_network_with_the_stream_decoder_trains(dev):
     b = a.clone()
     b[20:] = 0
     assert torch.equal(dec.forward(a, 1, 30)[0][:20], dec.forward(b, 1, 30)[0][:20])
+
+
+def test_a_captured_pass_survives_other_shapes(dev):
+    """The plans of chunk batches stay where a captured graph reads them, whatever shapes come between the replays."""
+    dec, _, _ = make(dev, 64, 1)
+    x = torch.randn(2 * 70, 64, generator=torch.Generator().manual_seed(4)).to(dev)
+    want = dec.forward(x, 2, 70)[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = dec.forward(x, 2, 70)[0]
+    first = dec._plans[(2, 70, x.device)]
+    for B, T in ((1, 140), (4, 35), (140, 1)):
+        dec.forward(x, B, T)
+        junk = [torch.full((n,), 1 << 30, dtype=torch.int32, device=dev) for n in (8, 64, 512, 4096)]      # what a freed plan's memory would be given to
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and len(junk) == 4
+    assert dec._plans[(2, 70, x.device)] is first
+
+
+def test_step_refuses_other_frames_and_leaves_the_streams_as_they_were(dev):
+    from pseldnets_amd import _lib
+    dec, _, _ = make(dev, 64, 1)
+    state = dec.stream_state(2, 5, dev, torch.float32)
+    x = torch.randn(2, 64, device=dev)
+    for bad in (x[:1], torch.zeros(3, 64, device=dev), torch.zeros(2, 32, device=dev), x.bfloat16(), x.cpu()):
+        with pytest.raises(_lib.PseldError):
+            dec.step(bad, state)
+    assert state.frames == 0 and state.plan.k_len.tolist() == [0, 0]
+    assert torch.equal(dec.step(x, state), dec.step(x, dec.stream_state(2, 5, dev, torch.float32)))
