@@ -1625,6 +1625,7 @@ class PackedPlan:
         self._ints = torch.from_numpy(np.concatenate(host).astype(np.int32)).to(self.device)
         self._ptr = {name: self._ints.data_ptr() + 4 * v for name, v in at.items()}
         self.k_len = self._ints[at['k_len']:at['k_len'] + seqs]
+        self._layouts = {}      # operand layouts that passed the checks (shapes, strides and types) -> what a call derives from them
         self._desc = (ctypes.c_long * 18)(seqs, self.rows, self.max_q, self.k_rows, self.max_k, self.q_tiles, self.k_tiles, *work, *self._ptr.values())
 
 
@@ -1664,9 +1665,19 @@ def _state_ok(what, plan, C, *ts):
             raise _lib.PseldError(f"{what}: states must be contiguous float32 [recordings = {plan.seqs}, C = {C}] on {plan.device}")
 
 
+def _remember(plan, key, value):
+    """The checks of a running stream's calls are made once per layout: a call whose key is known only looks at its tensors' devices."""
+    if len(plan._layouts) >= 64:
+        plan._layouts.clear()
+    plan._layouts[key] = value
+    return value
+
+
 def _linrec_ws(plan, C):
     """Scratch of its own per call (segment compositions), from the caching allocator: nothing is shared between streams or captured graphs."""
-    nbytes = _lib.lib().pseld_linrec_workspace(plan.rows, plan.seqs, plan.max_q, C)
+    nbytes = plan._layouts.get(C)
+    if nbytes is None:
+        nbytes = _remember(plan, C, _lib.lib().pseld_linrec_workspace(plan.rows, plan.seqs, plan.max_q, C))
     return (torch.empty(nbytes // 4, dtype=torch.float32, device=plan.device), nbytes) if nbytes else (None, 0)
 
 
@@ -1675,18 +1686,23 @@ def linrec_fwd(g, n, plan, h0=None, reverse=False, need_saved=True, out=None):
     reverse). g, n [rows, C] (row-strided views allowed; out must not overlap them), h0 f32 [recordings, C] or None (zeros).
     Returns (h [rows, C], h_last f32 [recordings, C], what linrec_bwd needs or None)."""
     stream = _on_plan("linrec_fwd", plan)
-    _rows_ok("linrec_fwd", plan, g.shape, g.dtype, g, n, out)
-    C = g.shape[1]
+    shape, index = g.shape, plan._index
+    key = (g.dtype, shape, g.stride(), n.dtype, n.shape, n.stride())
+    if out is not None or key not in plan._layouts or g.get_device() != index or n.get_device() != index:
+        _rows_ok("linrec_fwd", plan, shape, g.dtype, g, n, out)
+        _remember(plan, key, True)
+    C = shape[1]
     _state_ok("linrec_fwd", plan, C, h0)
     L = _lib.lib()
-    h = g.new_empty((plan.rows, C)) if out is None else out
-    h_last = torch.empty((plan.seqs, C), dtype=torch.float32, device=plan.device)
+    h = g.new_empty(shape) if out is None else out
+    h_last = torch.empty(plan.seqs, C, dtype=torch.float32, device=plan.device)
     states = torch.empty((L.pseld_linrec_states(plan.rows, plan.seqs), C), dtype=torch.float32, device=g.device) if need_saved else None
     ws, nbytes = _linrec_ws(plan, C)
-    rc = L.pseld_linrec_fwd(dtype_code(g), _lib.ptr(g), g.stride(0), _lib.ptr(n), n.stride(0), _lib.ptr(h0), _lib.ptr(h), h.stride(0),
-                            _lib.ptr(h_last), _lib.ptr(states), plan._ptr['q_start'], plan._ptr['q_len'], plan.seqs, plan.rows, plan.max_q, C,
-                            int(bool(reverse)), _lib.ptr(ws), nbytes, stream)
-    _lib.check(rc, "pseld_linrec_fwd")
+    rc = L.pseld_linrec_fwd(dtype_code(g), g.data_ptr(), key[2][0], n.data_ptr(), key[5][0], None if h0 is None else h0.data_ptr(), h.data_ptr(),
+                            C if out is None else h.stride(0), h_last.data_ptr(), _lib.ptr(states), plan._ptr['q_start'], plan._ptr['q_len'], plan.seqs, plan.rows,
+                            plan.max_q, C, 1 if reverse else 0, _lib.ptr(ws), nbytes, stream)
+    if rc:
+        _lib.check(rc, "pseld_linrec_fwd")
     return h, h_last, states
 
 
@@ -1778,12 +1794,16 @@ def _packed_attn_args(what, plan, q, k, v, scale, bias_table, buckets):
     _heads_ok(what, plan, dtype, plan.rows, hq, D, 'q', q)
     _heads_ok(what, plan, dtype, plan.k_rows, hkv, D, 'k', k)
     _heads_ok(what, plan, dtype, plan.k_rows, hkv, D, 'v', v)
+    _table_ok(what, plan, hq, bias_table, buckets)
+    return dtype, hq, hkv, D, D ** -0.5 if scale is None else float(scale)
+
+
+def _table_ok(what, plan, hq, bias_table, buckets):
     if (bias_table is None) != (buckets is None):
         raise _lib.PseldError(f"{what}: bias_table and buckets come together")
     if buckets is not None and (buckets.device != plan.device or bias_table.get_device() != plan._index or bias_table.dtype is not torch.float32 or
                                 bias_table.shape != (buckets.num_buckets, hq) or not bias_table.is_contiguous()):
         raise _lib.PseldError(f"{what}: bias_table must be contiguous float32 [buckets = {buckets.num_buckets}, query heads = {hq}] on {plan.device}")
-    return dtype, hq, hkv, D, D ** -0.5 if scale is None else float(scale)
 
 
 def _table_args(bias_table, buckets):
@@ -1800,23 +1820,27 @@ def packed_attn_fwd(q, k, v, plan, causal=False, scale=None, bias_table=None, bu
     bias_table f32 [buckets, query heads] with buckets = relpos_buckets(...): bias_table[bucket(key position - query position), head]
     is added to the scaled scores (-inf masks a bucket; finite entries stay below 1e37 scale). Key rows past a recording's k_len are never read. A value that
     is not finite reaches, times a probability of 0, also the rows of its 64-key tile whose mask hides it. out must not overlap the operands."""
-    stream = _on_plan("packed_attn_fwd", plan)
-    dtype, hq, hkv, D, scale = _packed_attn_args("packed_attn_fwd", plan, q, k, v, scale, bias_table, buckets)
-    L = _lib.lib()
+    stream, index = _on_plan("packed_attn_fwd", plan), plan._index
+    key = (q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(), None if buckets is None else buckets.num_buckets)
+    known = plan._layouts.get(key)
+    if known is None or q.get_device() != index or k.get_device() != index or v.get_device() != index:
+        _, hq, hkv, D, default_scale = _packed_attn_args("packed_attn_fwd", plan, q, k, v, None, bias_table, buckets)
+        strides = _LONGS8(*(n for t in (q, k, v) for n in t.stride()[:2]), hq * D, D)
+        nbytes = _lib.lib().pseld_packed_attn_fwd_workspace(plan._desc, hq, hkv, D, key[9] or 0)
+        known = _remember(plan, key, (dtype_code(q), hq, hkv, D, default_scale, strides, nbytes))
+    code, hq, hkv, D, default_scale, strides, nbytes = known
+    _table_ok("packed_attn_fwd", plan, hq, bias_table, buckets)
     if out is None:
-        out = q.new_empty((plan.rows, hq, D))
+        out = q.new_empty(q.shape)
     else:
-        _heads_ok("packed_attn_fwd", plan, dtype, plan.rows, hq, D, 'out', out)
-    lse = torch.empty((plan.rows, hq), dtype=torch.float32, device=plan.device)
+        _heads_ok("packed_attn_fwd", plan, q.dtype, plan.rows, hq, D, 'out', out)
+        strides = _LONGS8(*strides[:6], *out.stride()[:2])
+    lse = torch.empty(plan.rows, hq, dtype=torch.float32, device=plan.device)
     table, lut, nb, md = _table_args(bias_table, buckets)
-    nbytes = L.pseld_packed_attn_fwd_workspace(plan._desc, hq, hkv, D, nb)
     ws = torch.empty(nbytes // 4, dtype=torch.float32, device=plan.device) if nbytes else None      # its own per call: nothing shared between streams
-    q0, q1, _ = q.stride()
-    k0, k1, _ = k.stride()
-    v0, v1, _ = v.stride()
-    o0, o1, _ = out.stride()
-    rc = L.pseld_packed_attn_fwd(dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _LONGS8(q0, q1, k0, k1, v0, v1, o0, o1),
-                                 plan._desc, hq, hkv, D, 1 if causal else 0, scale, table, lut, nb, md, None if ws is None else ws.data_ptr(), nbytes, stream)
+    rc = _lib.lib().pseld_packed_attn_fwd(code, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), strides, plan._desc, hq, hkv, D,
+                                          1 if causal else 0, default_scale if scale is None else float(scale), table, lut, nb, md,
+                                          None if ws is None else ws.data_ptr(), nbytes, stream)
     if rc:
         _lib.check(rc, "pseld_packed_attn_fwd")
     return out, lse
