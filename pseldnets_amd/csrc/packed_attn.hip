@@ -51,7 +51,7 @@ struct PAttnArgs {
 
 // Two waves per SIMD where 256 registers hold a wave's accumulators and operands: the compiler then keeps the accumulators in vector registers
 // (with more, it moves them to accumulation registers and back around every softmax). f32 operands of heads above 32 take the whole file.
-template <typename T, int DP> constexpr int waves_per_simd() { return sizeof(T) == 2 || DP == 32 ? 2 : 1; }
+template <typename T, int DP> constexpr int waves_per_simd() { return sizeof(T) == 2 || DP <= 64 ? 2 : 1; }
 
 // ---- LDS images: rows of DP elements, lane-linear, 16-byte pieces swizzled inside the row ------------------------------------------
 // What the XOR has to do (64 banks of 4 bytes): 16 rows that are read one 16-byte piece each (row_frag) must hit all 64 banks once, and so must 4 rows
@@ -216,15 +216,40 @@ __device__ __forceinline__ float bias_at(const PAttnArgs& a, int rel, int head) 
     const int r = max(-a.maxd, min(a.maxd, rel));
     return a.table[(long)a.lut[r + a.maxd] * a.hq + head];
 }
-// the same, log2 units, for a head that is the workgroup's: in a scalar register
-__device__ __forceinline__ float far_bias(const PAttnArgs& a, int rel, int head) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, bias_at(a, rel, head) * LOG2E)));
-}
-// dist[i] = bias of distance i - maxd - NEAR_PAD over the scale: in units of the raw products, whose accumulators start from it
-__device__ __forceinline__ void dist_fill(float* dist, const PAttnArgs& a, int head, int threads) {
+// The bias of one head by distance, laid out in LDS: dist[i] = bias of distance i - maxd - NEAR_PAD over the scale, in units of the raw products, whose
+// accumulators start from it. ask / look / put are the three steps of a chain of dependent reads (lut, table, LDS), so that a kernel can put
+// its other requests between them: ask needs nothing but the arguments. The first 512 distances go that way, the rest in a loop.
+struct Dist {
+    int n, b[2], b_lo, b_hi;
+    float v[2], lo, hi;
+    __device__ __forceinline__ void ask(const PAttnArgs& a) {
+        n = dist_count(a.maxd);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) b[j] = a.lut[max(0, min(2 * a.maxd, (int)threadIdx.x + 256 * j - NEAR_PAD))];
+        b_lo = a.lut[0];
+        b_hi = a.lut[2 * a.maxd];
+    }
+    __device__ __forceinline__ void look(const PAttnArgs& a, int head) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) v[j] = a.table[(long)b[j] * a.hq + head];
+        lo = a.table[(long)b_lo * a.hq + head];
+        hi = a.table[(long)b_hi * a.hq + head];
+    }
+    __device__ __forceinline__ void put(float* dist, const PAttnArgs& a, int head) const {
+        const float inv = 1.f / a.scale;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) if ((int)threadIdx.x + 256 * j < n) dist[threadIdx.x + 256 * j] = v[j] * inv;
+        for (int i = threadIdx.x + 512; i < n; i += 256) dist[i] = bias_at(a, i - a.maxd - NEAR_PAD, head) * inv;
+    }
+    // the first and the last bucket's bias in log2 units, in scalar registers
+    __device__ __forceinline__ float far(float x) const { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x * LOG2E))); }
+};
+
+// the whole layout in one loop: where a head changes amid a kernel's tiles
+__device__ __forceinline__ void dist_fill(float* dist, const PAttnArgs& a, int head) {
     const int n = dist_count(a.maxd);
     const float inv = 1.f / a.scale;
-    for (int i = threadIdx.x; i < n; i += threads) dist[i] = bias_at(a, i - a.maxd - NEAR_PAD, head) * inv;
+    for (int i = threadIdx.x; i < n; i += 256) dist[i] = bias_at(a, i - a.maxd - NEAR_PAD, head) * inv;
 }
 
 // Keeps the scheduler from requesting a whole product's operands at once where the accumulators leave no registers for them
@@ -383,6 +408,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
     constexpr int TB = KT * I::RB, KS = key_split<T>(), KW = KT / KS, NT = 2 / KS;
     extern __shared__ __attribute__((aligned(1024))) char smem[];      // 2 x (K tile | V tile) | bias by distance
     float* dist = (float*)(smem + 4 * TB);
+    Dist bias;
+    if constexpr (BIAS) bias.ask(a);
     const QTile w = q_tile_of<KS>(a);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
     const int rg = wave % (4 / KS), kh = wave / (4 / KS);       // the wave's rows and its part of every key tile
@@ -397,8 +424,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
     const unsigned lds0 = lds_addr(smem);
     const typename I::Lane im0 = I::lane_offsets(lane);
     const int nt = (w.nk + KT - 1) / KT;
+    if constexpr (BIAS) bias.look(a, w.head);
     if (nt) { ks.load(kb, w.k_len, lds0); vs.load(vb, w.k_len, lds0 + TB); }
-    if constexpr (BIAS) dist_fill(dist, a, w.head, 256);
     typename I::Frag fq[DP / 16];
     {
         const char* row = a.q + qrow * a.sq.rs + (long)w.head * a.sq.hs;
@@ -410,7 +437,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
     const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;   // every query of the wave sees keys up to here,
     const int wlim1 = w.q0 + rg * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;     // none sees one past here
     float far_lo = 0.f, far_hi = 0.f;
-    if constexpr (BIAS) { far_lo = far_bias(a, -a.maxd, w.head); far_hi = far_bias(a, a.maxd, w.head); }
+    if constexpr (BIAS) { bias.put(dist, a, w.head); far_lo = bias.far(bias.lo); far_hi = bias.far(bias.hi); }
     Softmax<DP> sm;
     sm.init();
     PA_LOADS_DONE();
@@ -503,13 +530,6 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
     const int first = kbeg + wave * WR;                    // the first block is on its way before anything else is read
     if (first < kend) { ks.load(kb + (long)first * a.sk.rs, k_len - first, lds0); vs.load(vb + (long)first * a.sv.rs, k_len - first, lds0 + BB); }
     const int off = k_len - q_len;
-    if constexpr (BIAS) {
-        if (kend - 1 - off > -a.maxd) {                    // some key is near some query
-            for (int i = threadIdx.x; i < a.buckets * G; i += 64 * NW) tab[i] = a.table[(long)(i / G) * a.hq + kvh * G + i % G] / a.scale;
-            for (int i = threadIdx.x; i <= 2 * a.maxd; i += 64 * NW) lut[i] = (unsigned short)a.lut[i];
-        }
-        __syncthreads();
-    }
     const int rr = min(r, rows - 1), qi = rr / G, g = rr - qi * G;
     const long qrow = (long)a.q_start[seq] + qi;
     typename I::Frag fq[DP / 16];
@@ -517,6 +537,13 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
         const char* row = a.q + qrow * a.sq.rs + (long)(kvh * G + g) * a.sq.hs;
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) fq[kk] = global_frag<T, DP>(row, kk, h2, a.D);
+    }
+    if constexpr (BIAS) {
+        if (kend - 1 - off > -a.maxd) {                    // some key is near some query
+            for (int i = threadIdx.x; i < a.buckets * G; i += 64 * NW) tab[i] = a.table[(long)(i / G) * a.hq + kvh * G + i % G] / a.scale;
+            for (int i = threadIdx.x; i <= 2 * a.maxd; i += 64 * NW) lut[i] = (unsigned short)a.lut[i];
+        }
+        __syncthreads();
     }
     const int qpos = qi + off, klim = a.causal ? min(k_len - 1, qpos) : k_len - 1;
     float far_lo = 0.f, far_hi = 0.f;
@@ -699,7 +726,7 @@ template <int NT> __device__ __forceinline__ void add_diagonals(unsigned m, unsi
 }
 
 // (f32 heads of 128 with the table: two buffers and the sums for 1024 distances would not fit 160 KB, so that variant has one buffer)
-template <typename T, int DP, int MODE> constexpr int dq_buffers() { return sizeof(T) == 4 && DP == 128 && MODE == DQ_TABLE ? 1 : 2; }
+template <typename T, int DP, int MODE> constexpr int dq_buffers() { return sizeof(T) == 4 && DP >= 64 && MODE == DQ_TABLE ? 1 : 2; }
 // dq (and the table's gradient), tiled like the forward; DELTA: only delta = sum_j P dP
 // (and its LDS leaves room for one workgroup per CU at heads of 128 anyway: the whole register file instead of spills)
 template <typename T, int DP, bool BIAS, int MODE>
@@ -713,6 +740,8 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
     float* hist = dist + ndist;
     float* far = hist + 4 * ndist;
     const unsigned diag = (lds_addr(far + 8) + 15) & ~15u;
+    Dist bias;
+    if constexpr (BIAS) bias.ask(a);
     const QTile w = q_tile_of<KS>(a);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h2 = lane >> 5;
     const int rg = wave % (4 / KS), kh = wave / (4 / KS);       // the wave's rows and its part of every key tile
@@ -727,8 +756,8 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
     const unsigned lds0 = lds_addr(smem);
     const typename I::Lane im0 = I::lane_offsets(lane);
     const int nt = (w.nk + KT - 1) / KT;
+    if constexpr (BIAS) bias.look(a, w.head);
     if (nt) { ks.load(kb, w.k_len, lds0); vs.load(vb, w.k_len, lds0 + TB); }
-    if constexpr (BIAS) dist_fill(dist, a, w.head, 256);
     if constexpr (MODE == DQ_TABLE)
         for (int i = threadIdx.x; i < 4 * ndist; i += 256) hist[i] = 0.f;
     typename I::Frag fq[DP / 16], fo[DP / 16];
@@ -748,7 +777,7 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
     const int wlim0 = a.causal ? min(w.k_len - 1, qw0) : w.k_len - 1;
     const int wlim1 = w.q0 + rg * WR >= w.q_len ? -1 : a.causal ? min(w.k_len - 1, qw0 + WR - 1) : w.k_len - 1;
     float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f;
-    if constexpr (BIAS) { far_lo = far_bias(a, -a.maxd, w.head); far_hi = far_bias(a, a.maxd, w.head); }
+    if constexpr (BIAS) { bias.put(dist, a, w.head); far_lo = bias.far(bias.lo); far_hi = bias.far(bias.hi); }
     f32x16 dq[DP / 32], start;
     zero_acc(dq);
 #pragma unroll
@@ -893,6 +922,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP == 64 ? 3 : waves_per_si
     constexpr int LV = dkv_lds_frags<T, DP, BIAS>(), RV = DP / 16 - LV;      // operands of v kept in LDS / in registers
     char* kept = (char*)(stat + 4 * KT) + (threadIdx.x >> 6) * LV * 1024 + (threadIdx.x & 63) * 16;
     float* dist = stat + 4 * KT + LV * 1024;
+    Dist bias;
+    if constexpr (BIAS) bias.ask(a);
     const int kvh = blockIdx.x % a.hkv, rest = blockIdx.x / a.hkv, split = rest % a.nsplit, ti = rest / a.nsplit;
     const int* rec = a.tiles + 8 * (long)ti;
     const int seq = rec[0], kt0 = rec[1], q_row = rec[2], q_len = rec[3], k_row = rec[4], k_cap = rec[5];
@@ -941,7 +972,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP == 64 ? 3 : waves_per_si
         const bool all = BIAS && (i1 - 1) / per - g0 < a.bias_heads;
         if constexpr (BIAS)
             if (all)
-                for (int g = g0; g <= (i1 - 1) / per; ++g) dist_fill(dist + (g - g0) * ndist, a, kvh * G + g, 256);
+                for (int g = g0; g <= (i1 - 1) / per; ++g) { bias.look(a, kvh * G + g); bias.put(dist + (g - g0) * ndist, a, kvh * G + g); }
         int held = -1;                                     // the head that LDS holds
         for (int it = i0; it < i1; ++it) {
             const int par = (it - i0) & 1, g = it / per, q0 = qfirst + (it - g * per) * KT;
@@ -954,7 +985,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP == 64 ? 3 : waves_per_si
                 if (!all && g != held) {                   // uniform; the last tile's readers are past the barrier below before anything is overwritten
                     if (held >= 0) __syncthreads();
                     held = g;
-                    dist_fill(dist, a, kvh * G + g, 256);
+                    dist_fill(dist, a, kvh * G + g);
                 }
             }
             PA_LOADS_DONE();
