@@ -50,7 +50,7 @@ struct PAttnArgs {
 };
 
 // Two waves per SIMD where 256 registers hold a wave's accumulators and operands: the compiler then keeps the accumulators in vector registers
-// (with more, it moves them to accumulation registers and back around every softmax). f32 operands of heads above 32 take the whole file.
+// (with more, it moves them to accumulation registers and back around every softmax). f32 operands of heads above 64 take the whole file.
 template <typename T, int DP> constexpr int waves_per_simd() { return sizeof(T) == 2 || DP <= 64 ? 2 : 1; }
 
 // ---- LDS images: rows of DP elements, lane-linear, 16-byte pieces swizzled inside the row ------------------------------------------
@@ -378,7 +378,7 @@ template <int NT> __device__ __forceinline__ void mask_rows(f32x16 (&x)[NT], int
 // hkv apart: with hkv a multiple of the eight XCDs every key head's tiles stay on one XCD's L2
 // f32 (the parity mode): an f32 matrix instruction takes 64 cycles and short recordings leave few waves, so the four waves are two groups of 32
 // rows x two halves of every key tile, joined through LDS at the end: half the rows per workgroup, half the time per tile (6 recordings of 30-600,
-// 8 heads of 64: forward 63 -> 46 us)
+// 8 heads of 64: forward 63 -> 43 us). bf16 tiles are too short for it (12 x 100-1200, 16 heads of 64, causal: forward 34 -> 40 us)
 template <typename T> constexpr int key_split() { return sizeof(T) == 4 ? 2 : 1; }
 struct QTile {
     int seq, q0, q_len, k_len, off, head, kvh, nk;
@@ -690,42 +690,50 @@ __global__ __launch_bounds__(256) void packed_attn_delta_kernel(PAttnArgs a, lon
 
 enum { DQ = 0, DQ_TABLE = 1, DELTA = 2 };
 
-// Adds a wave's 32 x 64 dS (lanes = queries) to its sums by distance; h points at the entry of distance (tile's first key - wave's first query). The
-// tile goes through LDS as [query][key]; in step q lane l reads key (q + l - 31) mod 64 of query q: over the 32 steps every element is read once, and what
-// a lane sees is one diagonal key - query = l - 31 while q + l >= 31 and one diagonal l + 33 before. (One LDS float atomic per element
-// instead took 67 cycles each: 200 us of the dq kernel for 12 recordings of 100-1200 frames, 16 heads of 64; with this the kernel takes 71.)
-constexpr int DIAG_PITCH = 68, DIAG = 32 * DIAG_PITCH;      // floats; 16-byte pieces of eight rows fall in different banks
+// Adds a wave's 32 x (32 NT) dS (lanes = queries) to its sums by distance; h points at the entry of distance (tile's first key - wave's first query).
+// The tile goes through LDS as [query][key]. 64 keys: in step q lane l reads key (q + l - 31) mod 64 of query q, so over the 32 steps every element
+// is read once, and what a lane sees is one diagonal key - query = l - 31 while q + l >= 31 and one diagonal l + 33 before. 32 keys: the same
+// modulo 32 by half waves, one for queries 0..15 and one for 16..31, whose sums then meet: 16 steps. (One LDS float atomic per element
+// instead took 67 cycles each: 200 us of the dq kernel for 12 recordings of 100-1200 frames, 16 heads of 64.)
+template <int NT> constexpr int diag_pitch() { return 32 * NT + 4; }      // floats; 16-byte pieces of eight rows fall in different banks
+template <int NT> constexpr int diag_floats() { return 32 * diag_pitch<NT>(); }
 typedef __attribute__((address_space(3))) float* lds_fptr;
 typedef __attribute__((address_space(3))) f32x4* lds_f4ptr;
 template <int NT> __device__ __forceinline__ void add_diagonals(unsigned m, unsigned h, const f32x16 (&x)[NT], int lane) {
+    constexpr int P = diag_pitch<NT>(), S = 16 * NT;
     const int r = lane & 31, h2 = lane >> 5;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};                // (32 keys only: the other half is zeros)
-            if (t < NT)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = x[t < NT ? t : 0][4 * g + i];
-            *(lds_f4ptr)(uintptr_t)(m + (r * DIAG_PITCH + 4 * h2) * 4 + (t * 32 + 8 * g) * 4) = v;
-        }
+        for (int g = 0; g < 4; ++g)
+            *(lds_f4ptr)(uintptr_t)(m + (r * P + 4 * h2) * 4 + (t * 32 + 8 * g) * 4) = f32x4{x[t][4 * g], x[t][4 * g + 1], x[t][4 * g + 2], x[t][4 * g + 3]};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // a wave's LDS operations run in order; this keeps the compiler's order too
     float all = 0.f, before = 0.f;
+    const int l = NT == 2 ? lane : r, q0 = NT == 2 ? 0 : 16 * h2;
+    const unsigned mq = m + q0 * P * 4;
 #pragma unroll
-    for (int q = 0; q < 32; ++q) {
-        const float v = *(lds_fptr)(uintptr_t)(m + (((lane + q + 33) & 63) << 2) + q * DIAG_PITCH * 4);
+    for (int s = 0; s < S; ++s) {
+        const float v = *(lds_fptr)(uintptr_t)(mq + (((l + q0 + s + 32 * NT - 31) & (32 * NT - 1)) << 2) + s * P * 4);
         all += v;
-        if (q < 31) before += lane < 31 - q ? v : 0.f;
-        if ((q & 7) == 7) pace<true>();
+        if (NT == 1 || s < 31) before += l < 31 - q0 - s ? v : 0.f;
+        if ((s & 7) == 7) pace<true>();
     }
-    const unsigned a = h + (lane - 31) * 4;
-    *(lds_fptr)(uintptr_t)a = *(lds_fptr)(uintptr_t)a + (all - before);
-    asm volatile("" ::: "memory");
-    if (lane < 31) *(lds_fptr)(uintptr_t)(a + 64 * 4) = *(lds_fptr)(uintptr_t)(a + 64 * 4) + before;
+    if constexpr (NT == 2) {
+        const unsigned a = h + (lane - 31) * 4;
+        *(lds_fptr)(uintptr_t)a = *(lds_fptr)(uintptr_t)a + (all - before);
+        asm volatile("" ::: "memory");
+        if (lane < 31) *(lds_fptr)(uintptr_t)(a + 64 * 4) = *(lds_fptr)(uintptr_t)(a + 64 * 4) + before;
+    } else {
+        all += __shfl_xor(all, 32, 64);
+        before += __shfl_xor(before, 32, 64);
+        const unsigned a = h + (h2 ? l + 1 : l - 31) * 4;
+        *(lds_fptr)(uintptr_t)a = *(lds_fptr)(uintptr_t)a + (h2 ? before : all - before);      // (h2, l = 31: nothing, + 0)
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// (f32 heads of 128 with the table: two buffers and the sums for 1024 distances would not fit 160 KB, so that variant has one buffer)
+// (f32 heads above 32 with the table: one buffer. At 128 two and the sums for 1024 distances would not fit 160 KB; at 64 one lets two workgroups share
+// a CU: 6 x 30-600, 8 heads of 64, 70 -> 59 us)
 template <typename T, int DP, int MODE> constexpr int dq_buffers() { return sizeof(T) == 4 && DP >= 64 && MODE == DQ_TABLE ? 1 : 2; }
 // dq (and the table's gradient), tiled like the forward; DELTA: only delta = sum_j P dP
 // (and its LDS leaves room for one workgroup per CU at heads of 128 anyway: the whole register file instead of spills)
@@ -734,7 +742,7 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
     using I = Image<T, DP>;
     constexpr int TB = KT * I::RB, NB = dq_buffers<T, DP, MODE>(), KS = key_split<T>(), KW = KT / KS, NT = 2 / KS;
     constexpr bool TIGHT = DP == 128;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];      // NB x (K | V) | bias by distance | then (DQ_TABLE) sums by distance, a copy per wave | 8 floats | 4 x DIAG
+    extern __shared__ __attribute__((aligned(1024))) char smem[];      // NB x (K | V) | bias by distance | then (DQ_TABLE) sums by distance, a copy per wave | 8 floats | 4 x diag_floats
     float* dist = (float*)(smem + NB * 2 * TB);
     const int ndist = BIAS ? dist_count(a.maxd) : 0;
     float* hist = dist + ndist;
@@ -830,7 +838,7 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
             }
         if constexpr (MODE == DQ_TABLE) {
             if (place == NEAR) {
-                add_diagonals<NT>(diag + wave * DIAG * 4, lds_addr(hist) + (wave * ndist + kt0 - qw0 + a.maxd + NEAR_PAD) * 4, st, lane);
+                add_diagonals<NT>(diag + wave * diag_floats<NT>() * 4, lds_addr(hist) + (wave * ndist + kt0 - qw0 + a.maxd + NEAR_PAD) * 4, st, lane);
             } else {
                 float s = 0.f;
 #pragma unroll
@@ -994,13 +1002,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP == 64 ? 3 : waves_per_si
             if (it + 1 < i1) fetch(it + 1, lds0 + (par ^ 1) * 2 * TB);
             const int qp0 = q0 + off;                      // position of the tile's first query
             const float* near = dist + (all ? (g - g0) * ndist : 0);
-            if (kw0 >= k_len || (a.causal && qp0 + KT - 1 < kw0)) continue;
+            if (kw0 >= k_len) continue;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
+                const int qt0 = qp0 + t * 32;
+                if (q0 + t * 32 >= q_len || (a.causal && qt0 + 31 < kw0)) continue;      // 32 queries that do not exist or see none of the wave's keys
                 f32x16 s[1], dp[1];
                 zero_acc(s);
                 float bo = 0.f;
-                const int qt0 = qp0 + t * 32;
                 if constexpr (BIAS) {
                     const int place = place_of(kw0 - (qt0 + 31), kw0 + WR - 1 - qt0, a.maxd);
                     if (place == NEAR) start_near<1, -1>(s, near + (key - qt0 - 4 * h2 + a.maxd + NEAR_PAD));
@@ -1209,7 +1218,7 @@ int run_bwd(PAttnArgs& a, const Plan& p, float* dtable, int accumulate, hipStrea
     if constexpr (BIAS) {
         if (dtable) {
             float* part = a.part;
-            PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ_TABLE>), q_tiles * a.hq, 256, (dq_buffers<T, DP, DQ_TABLE>()) * 2 * TB + 5 * nd + 64 + 4 * DIAG * 4, a);
+            PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ_TABLE>), q_tiles * a.hq, 256, (dq_buffers<T, DP, DQ_TABLE>()) * 2 * TB + 5 * nd + 64 + 16 * (diag_floats<2 / key_split<T>()>()), a);
             PA_LAUNCH(packed_attn_table_kernel, (long)a.hq * ((a.buckets + 15) / 16), 256, 0, part, dtable, (int)q_tiles, a.hq, a.buckets, accumulate);
             a.part += q_tiles * a.hq * a.buckets;
             a.part = (float*)(((uintptr_t)a.part + 15) & ~(uintptr_t)15);
