@@ -732,15 +732,17 @@ template <int NT> __device__ __forceinline__ void add_diagonals(unsigned m, unsi
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// (f32 heads above 32 with the table: one buffer. At 128 two and the sums for 1024 distances would not fit 160 KB; at 64 one lets two workgroups share
-// a CU: 6 x 30-600, 8 heads of 64, 70 -> 59 us)
-template <typename T, int DP, int MODE> constexpr int dq_buffers() { return sizeof(T) == 4 && DP >= 64 && MODE == DQ_TABLE ? 1 : 2; }
+// Keys of a wave's step in 32s, LDS buffers and waves per SIMD. With the table's gradient LDS holds its sums too: for heads above 32 one buffer and 32 keys at
+// a time let three (64) or two (f32, 128) workgroups share a CU, whose others cover a wait for the tile (bf16, 12 x 100-1200, 16 heads of 64,
+// forward + backward: two buffers and 64 keys 197 us, one and 32 186; f32, 6 x 30-600, 8 heads of 64, this kernel alone: 70 -> 59).
+template <typename T, int DP, int MODE> constexpr int dq_step() { return sizeof(T) == 4 || MODE == DQ_TABLE || (DP <= 64 && MODE == DQ) ? 1 : 2; }
+template <typename T, int DP, int MODE> constexpr int dq_buffers() { return DP >= 64 && MODE == DQ_TABLE ? 1 : 2; }
+template <typename T, int DP, int MODE> constexpr int dq_waves() { return sizeof(T) == 2 && DP == 64 && MODE != DELTA ? 3 : waves_per_simd<T, DP>(); }
 // dq (and the table's gradient), tiled like the forward; DELTA: only delta = sum_j P dP
-// (and its LDS leaves room for one workgroup per CU at heads of 128 anyway: the whole register file instead of spills)
 template <typename T, int DP, bool BIAS, int MODE>
-__global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per_simd<T, DP>())) void packed_attn_dq_kernel(PAttnArgs a) {
+__global__ __launch_bounds__(256, (dq_waves<T, DP, MODE>())) void packed_attn_dq_kernel(PAttnArgs a) {
     using I = Image<T, DP>;
-    constexpr int TB = KT * I::RB, NB = dq_buffers<T, DP, MODE>(), KS = key_split<T>(), KW = KT / KS, NT = 2 / KS;
+    constexpr int TB = KT * I::RB, NB = dq_buffers<T, DP, MODE>(), KS = key_split<T>(), KW = KT / KS, NT = 2 / KS, N = dq_step<T, DP, MODE>();
     constexpr bool TIGHT = DP == 128;
     extern __shared__ __attribute__((aligned(1024))) char smem[];      // NB x (K | V) | bias by distance | then (DQ_TABLE) sums by distance, a copy per wave | 8 floats | 4 x diag_floats
     float* dist = (float*)(smem + NB * 2 * TB);
@@ -807,48 +809,53 @@ __global__ __launch_bounds__(256, (DP == 128 && MODE == DQ_TABLE ? 1 : waves_per
         const int kt0 = k0 + kh * KW;                      // the wave's first key of the tile
         if (kt0 > wlim1) continue;
         const typename I::Lane im = I::at(im0, lds0 + kh * KW * I::RB + (NB == 2 ? i & 1 : 0) * 2 * TB);
-        f32x16 st[NT], dp[NT];
-        zero_acc(st);
-        float off = 0.f;
-        int place = NEAR;
-        if constexpr (BIAS) {
-            place = place_of(kt0 - (qw0 + WR - 1), kt0 + KW - 1 - qw0, a.maxd);
-            if (place == NEAR) start_near<NT, 1>(st, dist + (kt0 + 4 * h2 - qpos + a.maxd + NEAR_PAD));
-            else off = place < 0 ? far_lo : far_hi;
+#pragma unroll
+        for (int t0 = 0; t0 < NT; t0 += N) {
+            const int kt = kt0 + 32 * t0;
+            if (t0 && kt > wlim1) continue;
+            f32x16 st[N], dp[N];
+            zero_acc(st);
+            float off = 0.f;
+            int place = NEAR;
+            if constexpr (BIAS) {
+                place = place_of(kt - (qw0 + WR - 1), kt + 32 * N - 1 - qw0, a.maxd);
+                if (place == NEAR) start_near<N, 1>(st, dist + (kt + 4 * h2 - qpos + a.maxd + NEAR_PAD));
+                else off = place < 0 ? far_lo : far_hi;
+            }
+#pragma unroll
+            for (int t = 0; t < N; ++t) dp[t] = start;          // dP - delta: the product starts from -delta of the lane's query
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+                for (int t = 0; t < N; ++t) {
+                    I::M::mma(I::row_frag(im, t0 + t, kk), fq[kk], st[t]);
+                    I::M::mma(I::row_frag(im, t0 + t, kk, TB), fo[kk], dp[t]);
+                    if (t == N - 1) pace<TIGHT>();
+                }
+            if (kt + 32 * N - 1 > wlim0) mask_rows<N>(st, klim - kt - 4 * h2, -__builtin_inff());
+            const float sub = off - lse2;
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e], a.c, sub));
+                    if constexpr (MODE == DELTA) dl = fmaf(p, dp[t][e], dl);
+                    else st[t][e] = p * dp[t][e];
+                }
+            if constexpr (MODE == DQ_TABLE) {
+                if (place == NEAR) {
+                    add_diagonals<N>(diag + wave * diag_floats<N>() * 4, lds_addr(hist) + (wave * ndist + kt - qw0 + a.maxd + NEAR_PAD) * 4, st, lane);
+                } else {
+                    float s = 0.f;
+#pragma unroll
+                    for (int t = 0; t < N; ++t)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s += st[t][e];
+                    if (place < 0) sum_lo += s; else sum_hi += s;
+                }
+            }
+            if constexpr (MODE != DELTA) acc_product<T, DP, N, TIGHT>(dq, st, im, t0, lane, 0);
         }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) dp[t] = start;          // dP - delta: the product starts from -delta of the lane's query
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                I::M::mma(I::row_frag(im, t, kk), fq[kk], st[t]);
-                I::M::mma(I::row_frag(im, t, kk, TB), fo[kk], dp[t]);
-                if (t == NT - 1) pace<TIGHT>();
-            }
-        if (kt0 + KW - 1 > wlim0) mask_rows<NT>(st, klim - kt0 - 4 * h2, -__builtin_inff());
-        const float sub = off - lse2;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e], a.c, sub));
-                if constexpr (MODE == DELTA) dl = fmaf(p, dp[t][e], dl);
-                else st[t][e] = p * dp[t][e];
-            }
-        if constexpr (MODE == DQ_TABLE) {
-            if (place == NEAR) {
-                add_diagonals<NT>(diag + wave * diag_floats<NT>() * 4, lds_addr(hist) + (wave * ndist + kt0 - qw0 + a.maxd + NEAR_PAD) * 4, st, lane);
-            } else {
-                float s = 0.f;
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s += st[t][e];
-                if (place < 0) sum_lo += s; else sum_hi += s;
-            }
-        }
-        if constexpr (MODE != DELTA) acc_product<T, DP, NT, TIGHT>(dq, st, im, 0, lane, 0);
     }
     if constexpr (KS > 1) {                                // the second half's waves hand over their sums
         float* x = (float*)smem + rg * (DP / 2) * 64 + lane;
@@ -1218,7 +1225,7 @@ int run_bwd(PAttnArgs& a, const Plan& p, float* dtable, int accumulate, hipStrea
     if constexpr (BIAS) {
         if (dtable) {
             float* part = a.part;
-            PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ_TABLE>), q_tiles * a.hq, 256, (dq_buffers<T, DP, DQ_TABLE>()) * 2 * TB + 5 * nd + 64 + 16 * (diag_floats<2 / key_split<T>()>()), a);
+            PA_LAUNCH((packed_attn_dq_kernel<T, DP, BIAS, DQ_TABLE>), q_tiles * a.hq, 256, (dq_buffers<T, DP, DQ_TABLE>()) * 2 * TB + 5 * nd + 64 + 16 * (diag_floats<dq_step<T, DP, DQ_TABLE>()>()), a);
             PA_LAUNCH(packed_attn_table_kernel, (long)a.hq * ((a.buckets + 15) / 16), 256, 0, part, dtable, (int)q_tiles, a.hq, a.buckets, accumulate);
             a.part += q_tiles * a.hq * a.buckets;
             a.part = (float*)(((uintptr_t)a.part + 15) & ~(uintptr_t)15);
