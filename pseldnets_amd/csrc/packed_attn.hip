@@ -1138,9 +1138,10 @@ int few_chunk(const Plan& p, int hkv) {
 int few_splits(const Plan& p, int hkv) { const int c = few_chunk(p, hkv); return p.max_k > c ? (int)((p.max_k + c - 1) / c) : 1; }
 // Query tiles per workgroup of the dk/dv kernel: the whole work is cut into equal parts where the key tiles alone would not fill the chip or end
 // unevenly: as many as about four fifths of the places (the tiles' odd ends take the rest), so that all run at once. Two workgroups fit a CU at heads
-// above 64 (1 x 8191, 16/2 heads of 128, forward + backward: 256 parts 1677 us, 400 1361, 512 1660, 1024 1685), three below (12 x 100-1200, 16/4
-// heads of 64: 500 parts 233 us, 600 206, 700 221, 1400 218). Below 4 tiles a part would spend longer on its f32 partials than on its tiles. f32
-// tiles take longer: parts of any length (6 x 30-600, 8 heads of 64: 240 parts 232 us, 700 210).
+// above 64 (1 x 8191, 16/2 heads of 128, forward + backward: 256 parts 1577 us, 330 1372, 400 1283, 460 1608), three below (12 x 100-1200, 16/4
+// heads of 64: 500 parts 208 us, 600 184, 700 199, 900 194). Below 4 tiles a part would spend longer on its f32 partials than on its tiles. f32
+// tiles take longer: parts of any length (6 x 30-600, 8 heads of 64: 350 parts 196 us, 500 208, 700 196, 1500 197; 3 x 1000 causal, 4 heads of 128,
+// backward: 170 parts 344 us, 700 312).
 int dkv_chunk(const Plan& p, int hq, int D, int causal, int dtype) {
     const long work = (causal ? p.k_work_causal : p.k_work) * hq;
     const long parts = dtype == PSELD_F32 ? 700 : D > 64 ? 400 : 600, c = (work + parts - 1) / parts, least = dtype == PSELD_F32 ? 1 : 4;
