@@ -148,7 +148,7 @@ def linear_dgrad(dy, w, rowscale=None, rows_per_scale=1, gelu_grad_of=None, resi
 
 
 # ---- weight gradients on a second stream ---------------------------------------------------------------------------
-# A weight gradient feeds nothing but the optimiser: the backward passes launch it on a second, high-priority HIP stream
+# A weight gradient feeds nothing but the optimiser: the backward passes launch it on a second HIP stream
 # beside their dependent chain (input gradients, attention / LayerNorm backward) and join before the gradients are used
 # (per stage / bucket, in front of the gradient all-reduce). Operands stay referenced until the join so that the caching
 # allocator does not hand their memory to the main stream meanwhile; scratch is per (device, stream) (workspace()).
@@ -164,8 +164,7 @@ def _env_int(name, dflt):
 # (min_chunks, round 6: with a stage's weight gradients grouped into ONE launch at <= 64 chunks there are four forks per step, not fifty, and
 #  the second stream pays from 36 chunks on - 36: 5.67 / 6.04 against 6.11 / 6.10 ms, 40: 5.94 / 5.85 against 6.28, 44: 6.19 against 6.64, 48: 6.46
 #  against 6.91, 56: 7.05 against 7.47; at 32 chunks it is a wash, 5.58-5.84 against 5.66-5.67: profiles/r06_ab_runs.txt, c<chunks>_*. It was 64.)
-_wgrad_stream = {'on': _env_int('PSELD_WGRAD_STREAM', '1') == 1, 'min_chunks': _env_int('PSELD_WGRAD_STREAM_MIN_CHUNKS', '36'),
-                 'prio': _env_int('PSELD_WGRAD_STREAM_PRIO', '-1')}
+_wgrad_stream = {'on': _env_int('PSELD_WGRAD_STREAM', '1') == 1, 'min_chunks': _env_int('PSELD_WGRAD_STREAM_MIN_CHUNKS', '36')}
 
 
 def set_wgrad_stream(on=None, min_chunks=None):
@@ -184,13 +183,18 @@ def wgrad_side_enabled(device, n_chunks):
             and not torch.cuda.is_current_stream_capturing())
 
 
-def linear_wgrad_side(dy, x, dw, **kw):
-    """linear_wgrad on the device's second stream, forked from the current stream (which produced dy)."""
-    import os
-    dev = dy.device
+def _side_stream(dev):
+    """The device's second stream and what it keeps alive. Default priority: work on streams of different priorities can hang the GPU."""
     st = _side.get(dev.index)
     if st is None:
-        st = _side[dev.index] = {'stream': torch.cuda.Stream(device=dev, priority=_wgrad_stream['prio']), 'keep': []}
+        st = _side[dev.index] = {'stream': torch.cuda.Stream(device=dev), 'keep': []}
+    return st
+
+
+def linear_wgrad_side(dy, x, dw, **kw):
+    """linear_wgrad on the device's second stream, forked from the current stream (which produced dy)."""
+    dev = dy.device
+    st = _side_stream(dev)
     side = st['stream']
     side.wait_stream(torch.cuda.current_stream(dev))
     with torch.cuda.stream(side):
@@ -268,11 +272,8 @@ def linear_wgrad_group(items):
 
 def linear_wgrad_group_side(items):
     """linear_wgrad_group on the device's second stream, forked from the current stream (which produced every dy)."""
-    import os
     dev = items[0][0].device
-    st = _side.get(dev.index)
-    if st is None:
-        st = _side[dev.index] = {'stream': torch.cuda.Stream(device=dev, priority=_wgrad_stream['prio']), 'keep': []}
+    st = _side_stream(dev)
     side = st['stream']
     side.wait_stream(torch.cuda.current_stream(dev))
     with torch.cuda.stream(side):
@@ -341,11 +342,8 @@ def mlp_bwd_dw(xh, dy, w1, b1, w2t, dw1, db1, dw2, db2, rowscale=None, rows_per_
 
 def mlp_bwd_dw_side(x, dy, *args, **kw):
     """mlp_bwd_dw on the device's second stream (see linear_wgrad_side)."""
-    import os
     dev = dy.device
-    st = _side.get(dev.index)
-    if st is None:
-        st = _side[dev.index] = {'stream': torch.cuda.Stream(device=dev, priority=_wgrad_stream['prio']), 'keep': []}
+    st = _side_stream(dev)
     side = st['stream']
     side.wait_stream(torch.cuda.current_stream(dev))
     with torch.cuda.stream(side):
