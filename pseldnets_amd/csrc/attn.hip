@@ -980,6 +980,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd24_kernel(AttnArgs a) {
                     const float ds = pt[e] * (dpt[e] - dl);
                     dpt[e] = ds;                           // dS^T
                     dsum[qt - kt + 1][e] += ds;
+                    asm volatile("" : "+v"(dsum[qt - kt + 1][e]));      // added here: sunk behind the tiles, the sums keep their operands alive and spill
                 }
                 const bf16x8 pf0 = M::from_acc(pt, 0), pf1 = M::from_acc(pt, 1), sf0 = M::from_acc(dpt, 0), sf1 = M::from_acc(dpt, 1);
                 // dQ^T[d][query] += K^T dS^T (contraction over the key rows of the accumulator)

@@ -167,7 +167,7 @@ __device__ __forceinline__ void gelu_both(float x, float& y, float& dy) {
     y = x * cdf;
     dy = cdf + x * 0.3989422804014327f * e;
 }
-// the same for two values at once: the polynomial runs on v_pk_fma_f32 / v_pk_mul_f32 (two fp32 lanes per instruction)
+// the same for two values at once
 __device__ __forceinline__ void gelu_both2(f32x2 x, f32x2& y, f32x2& dy) {
     f32x2 ax;
     ax[0] = fabsf(x[0]); ax[1] = fabsf(x[1]);

@@ -13,9 +13,9 @@
 //
 // Roofline: the HBM floor (5.634 MB algorithmic bytes per 10 s chunk: 3.84 MB in + 1.794 MB out -> 0.2 ms per 192 chunks) is NOT
 // what binds this kernel. Rounds 1-4 it was VALU-issue-bound (3 590, then 1 993 vector instructions per frame; profiles/r02_pmc_feature.json,
-// r04 / r05_pmc_feature.json). Round 5: the complex arithmetic is written in packed-fp32 instructions with operand selects (below) - the frame
-// loop's 1 455 static vector instructions became 829 - and the workgroups are persistent (tables built once per CU): 1.22 -> 0.88 ms per 192
-// chunks. What is left is latency: 2 waves per SIMD (150 KB of LDS per workgroup = one workgroup per CU) walk a chain of four LDS exchanges
+// r04 / r05_pmc_feature.json). Then the complex arithmetic was written out half by half without moves between register pairs (in packed
+// fp32 first, in scalar instructions since: the same time, 0.92 against 0.93 ms inside the step) and the workgroups became persistent (tables built
+// once per CU): 1.22 -> 0.9 ms per 192 chunks. What is left is latency: 2 waves per SIMD (150 KB of LDS per workgroup = one workgroup per CU) walk a chain of four LDS exchanges
 // per frame; neither the VALU (~0.40 ms of issue) nor the LDS pipe (~0.43 ms incl. bank conflicts) is saturated. Inside the step the kernel
 // is NOT hidden by the second stream it runs on: with the features cached the step is 0.9 ms shorter (tools/experiments/feature_cost.py).
 #include "common.h"
@@ -57,65 +57,42 @@ constexpr int WAVES2 = 8;                  // waves (= frames in flight) per wor
 constexpr int FPB2 = 64;                   // frames per work item (a persistent workgroup walks the (chunk, 64-frame block) items round-robin)
 constexpr int V2_WAVE_BYTES = 2 * FFT_LDS * 8;
 
-// Complex arithmetic on packed fp32 (round 5). A complex number is one 64-bit register pair; v_pk_add / v_pk_mul / v_pk_fma_f32 pick, per
-// result half, which half of each source they read (op_sel / op_sel_hi) and whether it is negated (neg_lo / neg_hi) - so a multiplication by
-// -i, a conjugate, a broadcast of the real part are operand modifiers, not instructions. Written as inline asm: the compiler's own packing
-// of the scalar formulation spent 466 of the frame loop's 1 455 vector instructions on v_mov (pairing unrelated scalars).
+// Complex arithmetic: a complex number is a pair of registers, and every helper is one product, sum or fused product per half, so that a
+// multiplication by -i, a conjugate, a broadcast of the real part cost nothing but the order of the operands. Scalar instructions: the packed fp32 forms with
+// operand selects, which these helpers were written in before, can give wrong results on this card. No contraction: a product
+// that feeds a sum is rounded by itself, as it was then, and the features keep their bits.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-#define PSELD_PK2(name, op, mods)                                                                                  \
-    __device__ __forceinline__ f32x2 name(f32x2 a, f32x2 b) { f32x2 d; asm(op " %0, %1, %2 " mods : "=v"(d) : "v"(a), "v"(b)); return d; }
-PSELD_PK2(cadd, "v_pk_add_f32", "")                                                          // a + b
-PSELD_PK2(csub, "v_pk_add_f32", "neg_lo:[0,1] neg_hi:[0,1]")                               // a - b
-PSELD_PK2(cadd_mi, "v_pk_add_f32", "op_sel:[0,1] op_sel_hi:[1,0] neg_hi:[0,1]")            // a + (-i) b = (a.x + b.y, a.y - b.x)
-PSELD_PK2(csub_mi, "v_pk_add_f32", "op_sel:[0,1] op_sel_hi:[1,0] neg_lo:[0,1]")            // a - (-i) b = (a.x - b.y, a.y + b.x)
-PSELD_PK2(pmul, "v_pk_mul_f32", "")                                                          // (a.x b.x, a.y b.y)
-PSELD_PK2(pmul_lo, "v_pk_mul_f32", "op_sel:[0,0] op_sel_hi:[1,0]")                          // a * b.x
-PSELD_PK2(pmul_hi, "v_pk_mul_f32", "op_sel:[0,1] op_sel_hi:[1,1]")                          // a * b.y
-#undef PSELD_PK2
-__device__ __forceinline__ f32x2 pfma(f32x2 a, f32x2 b, f32x2 c) { f32x2 d; asm("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c)); return d; }
-__device__ __forceinline__ f32x2 pfma_lo(f32x2 a, f32x2 b, f32x2 c) {      // a * b.x + c
-    f32x2 d; asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[0,0,0] op_sel_hi:[1,0,1]" : "=v"(d) : "v"(a), "v"(b), "v"(c)); return d; }
-__device__ __forceinline__ f32x2 pfma_hi(f32x2 a, f32x2 b, f32x2 c) {      // a * b.y + c
-    f32x2 d; asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[0,1,0] op_sel_hi:[1,1,1]" : "=v"(d) : "v"(a), "v"(b), "v"(c)); return d; }
-// c + r a / c - r a, r = (R, R) in scalar registers
-__device__ __forceinline__ f32x2 pfma_s(f32x2 a, f32x2 r, f32x2 c) { f32x2 d; asm("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "s"(r), "v"(c)); return d; }
-__device__ __forceinline__ f32x2 pfnma_s(f32x2 a, f32x2 r, f32x2 c) { f32x2 d; asm("v_pk_fma_f32 %0, %1, %2, %3 neg_lo:[1,0,0] neg_hi:[1,0,0]" : "=v"(d) : "v"(a), "s"(r), "v"(c)); return d; }
-// complex product v w = (v.x w.x - v.y w.y, v.x w.y + v.y w.x): two instructions; w in vector or in scalar registers
-__device__ __forceinline__ f32x2 cmul(f32x2 v, f32x2 w) {
-    f32x2 t, r;
-    asm("v_pk_mul_f32 %0, %1, %2 op_sel:[0,0] op_sel_hi:[0,1]" : "=v"(t) : "v"(v), "v"(w));
-    asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[1,1,0] op_sel_hi:[1,0,1] neg_lo:[0,1,0]" : "=v"(r) : "v"(v), "v"(w), "v"(t));
-    return r;
-}
-__device__ __forceinline__ f32x2 cmul_s(f32x2 v, f32x2 w) {
-    f32x2 t, r;
-    asm("v_pk_mul_f32 %0, %1, %2 op_sel:[0,0] op_sel_hi:[0,1]" : "=v"(t) : "v"(v), "s"(w));
-    asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[1,1,0] op_sel_hi:[1,0,1] neg_lo:[0,1,0]" : "=v"(r) : "v"(v), "s"(w), "v"(t));
-    return r;
-}
-__device__ __forceinline__ f32x2 mul_mi(f32x2 a) {                          // a * (-i) = (a.y, -a.x)
-    const f32x2 c = {1.f, -1.f};
-    f32x2 d; asm("v_pk_mul_f32 %0, %1, %2 op_sel:[1,0] op_sel_hi:[0,1]" : "=v"(d) : "v"(a), "s"(c)); return d;
-}
+#pragma clang fp contract(off)
+__device__ __forceinline__ f32x2 cadd(f32x2 a, f32x2 b) { return f32x2{a.x + b.x, a.y + b.y}; }
+__device__ __forceinline__ f32x2 csub(f32x2 a, f32x2 b) { return f32x2{a.x - b.x, a.y - b.y}; }
+__device__ __forceinline__ f32x2 cadd_mi(f32x2 a, f32x2 b) { return f32x2{a.x + b.y, a.y - b.x}; }      // a + (-i) b
+__device__ __forceinline__ f32x2 csub_mi(f32x2 a, f32x2 b) { return f32x2{a.x - b.y, a.y + b.x}; }      // a - (-i) b
+__device__ __forceinline__ f32x2 pmul(f32x2 a, f32x2 b) { return f32x2{a.x * b.x, a.y * b.y}; }
+__device__ __forceinline__ f32x2 pmul1(f32x2 a, float b) { return f32x2{a.x * b, a.y * b}; }
+__device__ __forceinline__ f32x2 pfma(f32x2 a, f32x2 b, f32x2 c) { return f32x2{fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)}; }
+__device__ __forceinline__ f32x2 pfma1(f32x2 a, float b, f32x2 c) { return f32x2{fmaf(a.x, b, c.x), fmaf(a.y, b, c.y)}; }      // c + b a
+// complex product v w = (v.x w.x - v.y w.y, v.x w.y + v.y w.x)
+__device__ __forceinline__ f32x2 cmul(f32x2 v, f32x2 w) { return f32x2{fmaf(v.y, -w.y, v.x * w.x), fmaf(v.y, w.x, v.x * w.y)}; }
+__device__ __forceinline__ f32x2 mul_mi(f32x2 a) { return f32x2{a.y, -a.x}; }                           // a * (-i)
 
-// forward 4-point DFT, in place (8 packed additions: the -i of the odd butterfly is an operand select)
+// forward 4-point DFT, in place
 __device__ __forceinline__ void dft4(f32x2& x0, f32x2& x1, f32x2& x2, f32x2& x3) {
     const f32x2 a0 = cadd(x0, x2), a1 = csub(x0, x2), a2 = cadd(x1, x3), a3 = csub(x1, x3);
     x0 = cadd(a0, a2); x2 = csub(a0, a2); x1 = cadd_mi(a1, a3); x3 = csub_mi(a1, a3);
 }
-// forward 8-point DFT: in a[0..7] (natural), out X[k] (natural) written to o[0..7] (26 packed instructions)
+// forward 8-point DFT: in a[0..7] (natural), out X[k] (natural) written to o[0..7]
 __device__ __forceinline__ void dft8(const f32x2 (&a)[8], f32x2 (&o)[8]) {
     f32x2 e0 = a[0], e1 = a[2], e2 = a[4], e3 = a[6];
     f32x2 q0 = a[1], q1 = a[3], q2 = a[5], q3 = a[7];
     dft4(e0, e1, e2, e3);
     dft4(q0, q1, q2, q3);
-    const f32x2 RR = {0.70710678118654752f, 0.70710678118654752f};
+    const float R = 0.70710678118654752f;
     const f32x2 s1 = cadd_mi(q1, q1);            // (q1.x + q1.y, q1.y - q1.x):  q1 (1 - i) / sqrt2 = R s1
     const f32x2 s3 = csub_mi(q3, q3);            // (q3.x - q3.y, q3.y + q3.x):  q3 (-1 - i) / sqrt2 = -R s3
     o[0] = cadd(e0, q0); o[4] = csub(e0, q0);
-    o[1] = pfma_s(s1, RR, e1); o[5] = pfnma_s(s1, RR, e1);
+    o[1] = pfma1(s1, R, e1); o[5] = pfma1(s1, -R, e1);
     o[2] = cadd_mi(e2, q2); o[6] = csub_mi(e2, q2);          // q2 (-i)
-    o[3] = pfnma_s(s3, RR, e3); o[7] = pfma_s(s3, RR, e3);
+    o[3] = pfma1(s3, -R, e3); o[7] = pfma1(s3, R, e3);
 }
 // exp(-2 pi i j / 32), j = n2 * k1 <= 21
 __device__ __forceinline__ constexpr float w32c(int j) {
@@ -145,7 +122,7 @@ __device__ __forceinline__ void fft32(f32x2 (&x)[32]) {
             const int j = n2 * k1;
             if (j == 0) a[n2] = v;
             else if (j == 8) a[n2] = mul_mi(v);
-            else { const f32x2 w = {w32c(j), w32s(j)}; a[n2] = cmul_s(v, w); }
+            else { const f32x2 w = {w32c(j), w32s(j)}; a[n2] = cmul(v, w); }
         }
         dft8(a, r);
 #pragma unroll
@@ -284,8 +261,8 @@ __global__ __launch_bounds__(WAVES2 * 64) void logmel_iv_kernel(FeatArgs a) {
 #pragma unroll
         for (int m2 = 0; m2 < 16; ++m2) {
             const f32x2 wn = *(const f32x2*)(wins + t * 36 + 2 * m2);      // window[t + 32 m], m = 2 m2, 2 m2 + 1
-            x[2 * m2] = pmul_lo(xr[2 * m2], wn);
-            x[2 * m2 + 1] = pmul_hi(xr[2 * m2 + 1], wn);
+            x[2 * m2] = pmul1(xr[2 * m2], wn.x);
+            x[2 * m2 + 1] = pmul1(xr[2 * m2 + 1], wn.y);
         }
         if (a.n_ch < 4) {
             const f32x2 kf = {k0f, k1f};
@@ -318,20 +295,15 @@ __global__ __launch_bounds__(WAVES2 * 64) void logmel_iv_kernel(FeatArgs a) {
         for (int j = 0; j < 9; ++j) {
             const int k = lane + 64 * j;
             // ch0 = a / 2, ch1 = b / (2i), ch2 = c / 2, ch3 = d / (2i)  with  a = z + conj(zn), b = z - conj(zn). Packed as the pairs the products
-            // below want: X = (ax, bx), Y = (ay, by), P = (cx, dy), Q = (cy, dx) - four instructions
-            f32x2 X, Y, P, Q, t, pw01, pw23;
-            asm("v_pk_add_f32 %0, %1, %2 op_sel:[0,0] op_sel_hi:[0,0] neg_hi:[0,1]" : "=v"(X) : "v"(z0[j]), "v"(zn0[j]));       // (z.x + zn.x, z.x - zn.x)
-            asm("v_pk_add_f32 %0, %1, %2 op_sel:[1,1] op_sel_hi:[1,1] neg_lo:[0,1]" : "=v"(Y) : "v"(z0[j]), "v"(zn0[j]));       // (z.y - zn.y, z.y + zn.y)
-            P = cadd(z1[j], zn1[j]);                                                                                              // (z.x + zn.x, z.y + zn.y)
-            asm("v_pk_add_f32 %0, %1, %2 op_sel:[1,1] op_sel_hi:[0,0] neg_lo:[0,1] neg_hi:[0,1]" : "=v"(Q) : "v"(z1[j]), "v"(zn1[j]));   // (z.y - zn.y, z.x - zn.x)
-            pw01 = pfma(Y, Y, pmul(X, X));                                   // 4 x power of channels 0, 1
-            pw23 = pfma(Q, Q, pmul(P, P));                                   // (cx^2 + cy^2, dy^2 + dx^2): channels 2, 3
+            // below want: X = (ax, bx), Y = (ay, by), P = (cx, dy), Q = (cy, dx)
+            const f32x2 X = {z0[j].x + zn0[j].x, z0[j].x - zn0[j].x}, Y = {z0[j].y - zn0[j].y, z0[j].y + zn0[j].y};
+            const f32x2 P = cadd(z1[j], zn1[j]), Q = {z1[j].y - zn1[j].y, z1[j].x - zn1[j].x};
+            const f32x2 pw01 = pfma(Y, Y, pmul(X, X));                                   // 4 x power of channels 0, 1
+            const f32x2 pw23 = pfma(Q, Q, pmul(P, P));                                   // (cx^2 + cy^2, dy^2 + dx^2): channels 2, 3
             f32x4 iv = {0.f, 0.f, 0.f, 0.f};
             if (a.with_iv) {
                 // 4 x intensity: i1 = ax by - ay bx, (i2, i3) = (ax cx + ay cy, ax dy - ay dx) = ax P + ay (Q.x, -Q.y)
-                f32x2 i23;
-                asm("v_pk_mul_f32 %0, %1, %2 op_sel:[0,0] op_sel_hi:[0,1]" : "=v"(t) : "v"(X), "v"(P));
-                asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[0,0,0] op_sel_hi:[0,1,1] neg_hi:[0,1,0]" : "=v"(i23) : "v"(Y), "v"(Q), "v"(t));
+                const f32x2 i23 = {fmaf(Y.x, Q.x, X.x * P.x), fmaf(Y.x, -Q.y, X.x * P.y)};
                 const float i1 = fmaf(X[0], Y[1], -Y[0] * X[1]);
                 const float inv = __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(fmaf(i1, i1, fmaf(i23[0], i23[0], i23[1] * i23[1]))) + eps4);
                 iv[0] = i1 * inv; iv[1] = i23[0] * inv; iv[2] = i23[1] * inv;
@@ -356,13 +328,13 @@ __global__ __launch_bounds__(WAVES2 * 64) void logmel_iv_kernel(FeatArgs a) {
                 f32x2 a01 = {0.f, 0.f}, a23 = a01, a45 = a01;
                 float a6 = 0.f;
 #pragma unroll
-                for (int i = 0; i < MEL_CAP; ++i) {                 // a bin's seven values times its weight: three packed FMAs + one
+                for (int i = 0; i < MEL_CAP; ++i) {                 // a bin's seven values times its weight
                     const f32x4 P = *(const f32x4*)(vp + i * 16), I = *(const f32x4*)(vp + VI_OFF + i * 16);
                     const f32x2 P01 = __builtin_shufflevector(P, P, 0, 1), P23 = __builtin_shufflevector(P, P, 2, 3);
                     const f32x2 I01 = __builtin_shufflevector(I, I, 0, 1);
                     const float I2 = I[2];
-                    if (i & 1) { a01 = pfma_hi(P01, w2[i >> 1], a01); a23 = pfma_hi(P23, w2[i >> 1], a23); a45 = pfma_hi(I01, w2[i >> 1], a45); }
-                    else { a01 = pfma_lo(P01, w2[i >> 1], a01); a23 = pfma_lo(P23, w2[i >> 1], a23); a45 = pfma_lo(I01, w2[i >> 1], a45); }
+                    if (i & 1) { a01 = pfma1(P01, w2[i >> 1].y, a01); a23 = pfma1(P23, w2[i >> 1].y, a23); a45 = pfma1(I01, w2[i >> 1].y, a45); }
+                    else { a01 = pfma1(P01, w2[i >> 1].x, a01); a23 = pfma1(P23, w2[i >> 1].x, a23); a45 = pfma1(I01, w2[i >> 1].x, a45); }
                     a6 = fmaf(I2, w2[i >> 1][i & 1], a6);
                 }
                 float acc[7] = {a01[0], a01[1], a23[0], a23[1], a45[0], a45[1], a6};
