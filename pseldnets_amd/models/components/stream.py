@@ -110,23 +110,44 @@ class StreamDecoder:
     # -- running streams -------------------------------------------------------------------------------------------------
     def stream_state(self, streams, capacity, device, dtype):
         """Empty caches for `streams` live streams of at most `capacity` frames."""
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise _lib.PseldError(f"stream decoder: streams run in float32 or bfloat16, not {dtype}")
         plan = ops.packed_plan([1] * streams, [0] * streams, k_cap=capacity, device=device)
         slab = lambda: torch.zeros((streams * capacity, self.kv_heads, self.hd), dtype=dtype, device=plan.device)      # noqa: E731
         return StreamState(plan, torch.arange(streams, device=plan.device) * capacity, [slab() for _ in range(self.L)], [slab() for _ in range(self.L)],
                            [torch.zeros((streams, self.D), dtype=torch.float32, device=plan.device) for _ in range(self.L)], capacity)
 
     def step(self, x, state):
-        """x [streams, D]: the next frame of every stream -> [streams, D], what forward_packed gives for that frame of the whole recording. The
-        caches and states move on in place."""
+        """x [streams, D]: the next frame of every stream (any row stride) -> [streams, D], what forward_packed gives for that frame of the whole
+        recording. The caches and states move on in place, or not at all where the call raises."""
+        plan, D = state.plan, self.D
+        ops._on_plan("stream decoder", plan)
+        if len(state.keys) != self.L or state.keys[0].shape[1:] != (self.kv_heads, self.hd) or state.states[0].shape[1] != D:
+            raise _lib.PseldError("stream decoder: the state was made by a decoder of another shape")
+        if x.shape != (plan.seqs, D) or x.dtype != state.keys[0].dtype or x.device != plan.device:
+            raise _lib.PseldError(f"stream decoder: a frame of these streams is {state.keys[0].dtype} [{plan.seqs}, {D}] on {plan.device}")
+        capturing = torch.cuda.is_current_stream_capturing()
         if state.frames >= state.capacity:
             raise _lib.PseldError(f"stream decoder: the streams' caches hold {state.capacity} frames and are full")
-        if x.shape != (state.plan.seqs, self.D) or x.dtype != state.keys[0].dtype or x.device != state.plan.device:
-            raise _lib.PseldError(f"stream decoder: a frame of these streams is {state.keys[0].dtype} [{state.plan.seqs}, {self.D}] on {state.plan.device}")
-        state.frames += 1
-        a, dt, D, plan = self.arena, x.dtype, self.D, state.plan
-        buckets = self._relpos(x.device)
+        x = x.contiguous()
         at = state.first + plan.k_len.clamp(max=state.capacity - 1)      # a replayed graph stays inside the slabs too
         plan.k_len.add_(1)
+        try:
+            x, states = self._step(x, state, at)
+        except BaseException:
+            if not capturing:
+                plan.k_len.sub_(1)
+            raise
+        for kept, last in zip(state.states, states):
+            kept.copy_(last)
+        state.frames += 1
+        return x
+
+    def _step(self, x, state, at):
+        """The layers of step(): writes the new keys and values at the rows `at` (past what the plan's lengths counted so far), returns the output and
+        the recurrences' new states."""
+        a, dt, D, plan, states = self.arena, x.dtype, self.D, state.plan, []
+        buckets = self._relpos(x.device)
         for li in range(self.L):
             b = f'{self.prefix}layers.{li}.'
             y1 = ops.layernorm_fwd(x, a.p(b + 'norm1.weight'), a.p(b + 'norm1.bias'))
@@ -140,6 +161,6 @@ class StreamDecoder:
             y2 = ops.layernorm_fwd(x1, a.p(b + 'norm2.weight'), a.p(b + 'norm2.bias'))
             u = ops.linear_fwd(y2, a.w(b + 'linear1.weight', dt), a.p(b + 'linear1.bias'))
             h, last, _ = ops.linrec_fwd(u[:, :D], u[:, D:], plan, h0=state.states[li], need_saved=False)
-            state.states[li].copy_(last)
+            states.append(last)
             x = ops.linear_fwd(h, a.w(b + 'linear2.weight', dt), a.p(b + 'linear2.bias'), resid=x1)
-        return x
+        return x, states

@@ -176,3 +176,60 @@ def test_step_refuses_other_frames_and_leaves_the_streams_as_they_were(dev):
             dec.step(bad, state)
     assert state.frames == 0 and state.plan.k_len.tolist() == [0, 0]
     assert torch.equal(dec.step(x, state), dec.step(x, dec.stream_state(2, 5, dev, torch.float32)))
+
+
+def test_step_takes_a_frame_out_of_a_recording(dev):
+    """x[:, t] of a [streams, T, D] tensor, whose rows lie apart: the same outputs and states as contiguous frames."""
+    S, T, D = 3, 6, 64
+    dec, _, _ = make(dev, D, 2)
+    x = torch.randn(S, T, D, generator=torch.Generator().manual_seed(6)).to(dev)
+    a, b = (dec.stream_state(S, T, dev, torch.float32) for _ in range(2))
+    for t in range(T):
+        assert torch.equal(dec.step(x[:, t], a), dec.step(x[:, t].contiguous(), b)), t
+        assert a.frames == t + 1 and a.plan.k_len.tolist() == [t + 1] * S
+    assert all(torch.equal(p, q) for p, q in zip(a.keys + a.values + a.states, b.keys + b.values + b.states))
+
+
+def test_step_refuses_states_that_are_not_its_own(dev):
+    """Another decoder's state, a type the kernels are not built for: refused before anything moves."""
+    from pseldnets_amd import _lib
+    dec, _, _ = make(dev, 64, 1)
+    deeper, _, _ = make(dev, 64, 2)
+    with pytest.raises(_lib.PseldError):
+        dec.stream_state(2, 5, dev, torch.float16)
+    x = torch.randn(2, 64, device=dev)
+    state = deeper.stream_state(2, 5, dev, torch.float32)
+    with pytest.raises(_lib.PseldError):
+        dec.step(x, state)
+    shallow = dec.stream_state(2, 5, dev, torch.float32)
+    with pytest.raises(_lib.PseldError):
+        deeper.step(x, shallow)
+    for s in (state, shallow):
+        assert s.frames == 0 and s.plan.k_len.tolist() == [0, 0]
+
+
+def test_a_step_that_fails_half_way_leaves_the_streams_as_they_were(dev, monkeypatch):
+    """An error in the second layer (memory that runs out, say): the frame can be given again."""
+    from pseldnets_amd import ops
+    S, T, D = 2, 4, 64
+    dec, _, _ = make(dev, D, 2)
+    x = torch.randn(S, T, D, generator=torch.Generator().manual_seed(7)).to(dev)
+    a, b = (dec.stream_state(S, T, dev, torch.float32) for _ in range(2))
+    real, calls = ops.linrec_fwd, []
+
+    def failing(*args, **kw):
+        calls.append(1)
+        if len(calls) == 6:                                 # the third frame's second layer
+            raise MemoryError
+        return real(*args, **kw)
+    for t in range(T):
+        frame = x[:, t].contiguous()
+        monkeypatch.setattr(ops, 'linrec_fwd', failing)
+        try:
+            y = dec.step(frame, a)
+        except MemoryError:
+            assert t == 2 and a.frames == 2 and a.plan.k_len.tolist() == [2, 2]
+            y = dec.step(frame, a)
+        monkeypatch.setattr(ops, 'linrec_fwd', real)
+        assert torch.equal(y, dec.step(frame, b)), t
+    assert len(calls) == 10 and all(torch.equal(p, q) for p, q in zip(a.states, b.states))
