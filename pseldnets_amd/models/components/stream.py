@@ -7,6 +7,8 @@ x = x + out_proj(attention(norm1(x))); x = x + linear2(recurrence(linear1(norm2(
 relative position bias by buckets (ops.packed_attn_*); linear1 gives the update gates | candidates of the gated linear recurrence
 (ops.linrec_*: nn.GRU's update rule without the recurrent product).
 """
+import math
+
 import torch
 
 from ... import _lib, ops
@@ -14,10 +16,22 @@ from ... import _lib, ops
 
 class StreamState:
     """What step() carries from frame to frame: per layer the key and value slabs [streams * capacity, key heads, head size] and the recurrence's
-    state f32 [streams, D]; plan.k_len holds the frames each stream has seen."""
+    state f32 [streams, D]; plan.k_len holds the frames each stream has seen. All streams of a state begin together. `frames` is what the host has
+    counted: step() adds one where it runs, advance() what replays of a captured step() are about to add."""
 
     def __init__(self, plan, first, keys, values, states, capacity):
         self.plan, self.first, self.keys, self.values, self.states, self.capacity, self.frames = plan, first, keys, values, states, capacity, 0
+
+    def remaining(self):
+        """Frames that the caches still have room for, by the host's count."""
+        return self.capacity - self.frames
+
+    def advance(self, n=1):
+        """To be called before n replays of a captured step(), which the host does not see otherwise: counts them, or refuses where the caches
+        would overflow. (Replays past the capacity that nobody counted answer with NaN.)"""
+        if n < 0 or n > self.remaining():
+            raise _lib.PseldError(f"stream decoder: the streams' caches hold {self.capacity} frames, {self.frames} are taken: no room for {n} more")
+        self.frames += n
 
 
 class StreamDecoder:
@@ -119,28 +133,33 @@ class StreamDecoder:
 
     def step(self, x, state):
         """x [streams, D]: the next frame of every stream (any row stride) -> [streams, D], what forward_packed gives for that frame of the whole
-        recording. The caches and states move on in place, or not at all where the call raises."""
+        recording. The caches and states move on in place, or not at all where the call raises. It can be captured into a graph (after one eager
+        step): state.advance() before a replay refuses the frame that no longer fits, as an eager call does by itself. A stream whose cache is full
+        all the same, by replays that were not counted, gets NaN: its caches and its state are no longer those of its frames."""
         plan, D = state.plan, self.D
         ops._on_plan("stream decoder", plan)
         if len(state.keys) != self.L or state.keys[0].shape[1:] != (self.kv_heads, self.hd) or state.states[0].shape[1] != D:
             raise _lib.PseldError("stream decoder: the state was made by a decoder of another shape")
         if x.shape != (plan.seqs, D) or x.dtype != state.keys[0].dtype or x.device != plan.device:
             raise _lib.PseldError(f"stream decoder: a frame of these streams is {state.keys[0].dtype} [{plan.seqs}, {D}] on {plan.device}")
-        capturing = torch.cuda.is_current_stream_capturing()
-        if state.frames >= state.capacity:
+        capturing = torch.cuda.is_current_stream_capturing()      # nothing runs then: the replays count
+        if state.remaining() < 1:
             raise _lib.PseldError(f"stream decoder: the streams' caches hold {state.capacity} frames and are full")
         x = x.contiguous()
-        at = state.first + plan.k_len.clamp(max=state.capacity - 1)      # a replayed graph stays inside the slabs too
-        plan.k_len.add_(1)
+        room = plan.k_len < state.capacity
+        at = state.first + plan.k_len.clamp(max=state.capacity - 1)      # a replay past the capacity stays inside the slabs
+        plan.k_len.add_(room)
         try:
             x, states = self._step(x, state, at)
+            x.masked_fill_(~room[:, None], math.nan)
         except BaseException:
             if not capturing:
-                plan.k_len.sub_(1)
+                plan.k_len.sub_(room.int())
             raise
         for kept, last in zip(state.states, states):
             kept.copy_(last)
-        state.frames += 1
+        if not capturing:
+            state.advance()
         return x
 
     def _step(self, x, state, at):

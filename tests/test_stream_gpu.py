@@ -233,3 +233,43 @@ def test_a_step_that_fails_half_way_leaves_the_streams_as_they_were(dev, monkeyp
         monkeypatch.setattr(ops, 'linrec_fwd', real)
         assert torch.equal(y, dec.step(frame, b)), t
     assert len(calls) == 10 and all(torch.equal(p, q) for p, q in zip(a.states, b.states))
+
+
+def test_replays_up_to_the_capacity_and_past_it(dev):
+    """Counted replays: every frame that fits is right, the next is refused by advance(). Replays that nobody counted: frames past the capacity are NaN,
+    from a replay as from an eager call, and so is every later one."""
+    from pseldnets_amd import _lib
+    S, D, cap = 2, 64, 6
+    dec, _, _ = make(dev, D, 2)
+    x = torch.randn(S, cap + 3, D, generator=torch.Generator().manual_seed(8)).to(dev)
+    eager = dec.stream_state(S, cap, dev, torch.float32)
+    want = [dec.step(x[:, t].contiguous(), eager) for t in range(cap)]
+    for counted in (True, False):
+        held = dec.stream_state(S, cap, dev, torch.float32)
+        slot = x[:, 0].contiguous()
+        assert torch.equal(dec.step(slot, held), want[0]) and held.frames == 1
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = dec.step(slot, held)
+        assert held.frames == 1 and held.remaining() == cap - 1      # the capture itself ran nothing
+        for t in range(1, cap):
+            if counted:
+                held.advance()
+            slot.copy_(x[:, t])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want[t]), t
+        assert held.plan.k_len.tolist() == [cap] * S
+        if counted:
+            assert held.remaining() == 0
+            for call in (held.advance, lambda: held.advance(2), lambda: dec.step(slot, held)):
+                with pytest.raises(_lib.PseldError):
+                    call()
+            assert held.frames == cap
+        for t in range(cap, cap + 3):
+            slot.copy_(x[:, t])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert bool(torch.isnan(y).all()) and held.plan.k_len.tolist() == [cap] * S, t
+        if not counted:
+            assert bool(torch.isnan(dec.step(slot, held)).all())
