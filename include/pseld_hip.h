@@ -513,7 +513,9 @@ int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void* g, long l
  *   behind a query's position are masked. |table| / scale is taken to be below 1e37.
  * plan: HOST array of 18 longs {seqs, rows, max_q, k_rows, max_k, q_tiles, k_tiles, the 64-query tiles that the key tiles meet, summed: full and
  * causal, then device int arrays as addresses: q_start[seqs], q_len[seqs], k_start[seqs], k_cap[seqs], k_len[seqs], q_tile[q_tiles][8], q_tile_causal, k_tile[k_tiles][8], k_tile_causal}: a tile is 128 rows
- * of queries or of capacity, {recording s, first row, q_start[s], q_len[s], k_start[s], k_cap[s], 0, 0}, heaviest first. k_len may change between calls; it is held to 0 .. k_cap.
+ * of queries or of capacity, {recording s, first row, q_start[s], q_len[s], k_start[s], k_cap[s], low, high}, heaviest first; low, high: 0 for queries, for keys the 64-query tiles
+ * that the key tiles before it in its list meet, summed, in 64 bits (key tiles stand in the order of the query tiles they meet; a key tile at row r meets those
+ * from row max(0, r - k_cap + q_len) / 64 * 64 on when causal, all otherwise). k_len may change between calls; it is held to 0 .. k_cap.
  * strides: HOST array of longs, {row stride, head stride} in elements of q, k, v, out (bwd: dout, q, k, v, out, dq, dk, dv), whole
  * 16-byte pieces; unit stride inside a head. At most 2^30 rows and key rows; results must not overlap operands. table f32 [buckets, hq] or NULL; lut (device ints): the bucket of every distance
  * -max_distance .. max_distance, then [buckets][2] first and last distance of each (none: first > last).
@@ -524,7 +526,7 @@ long pseld_packed_attn_fwd_workspace(const long* plan, int hq, int hkv, int D, i
 int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const long* strides,
                           const long* plan, int hq, int hkv, int D, int causal, float scale, const float* table, const int* lut,
                           int buckets, int max_distance, float* workspace, long workspace_bytes, void* stream);
-long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int causal, int buckets);
+long pseld_packed_attn_bwd_workspace(int dtype, const long* plan, int hq, int hkv, int D, int causal, int buckets);
 int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
                           void* dq, void* dk, void* dv, const long* strides, const long* plan, int hq, int hkv, int D, int causal, float scale,
                           const float* table, const int* lut, int buckets, int max_distance, float* dtable, int accumulate,

@@ -44,7 +44,8 @@ struct PAttnArgs {
     float scale, c;             // c = scale * log2(e)
     const float* table; const int* lut; const int* ranges;      // [buckets, hq]; bucket of distance -max .. max; [buckets, 2] first and last distance
     int buckets, maxd;
-    float* part;                // dtable: [tiles, hq, buckets]; split dk/dv: [tiles, hkv, nsplit, 2, TILE, DP]; few rows: see there
+    float* part;                // dtable: [tiles, hq, buckets]; split dk/dv: [hkv, slots, 2, TILE, DP]; few rows: see there
+    long slots;                 // dk, dv: parts reserved per key head
     int max_rows;               // few rows: rows reserved per key head
     int bias_heads;             // dk, dv: heads whose bias LDS has room for
 };
@@ -921,6 +922,13 @@ __device__ __forceinline__ int dkv_first(const PAttnArgs& a, int kt0, int q_len,
     return kt0 >= k_len ? q_len : a.causal ? max(0, kt0 - (k_len - q_len)) / KT * KT : 0;
 }
 __device__ __forceinline__ int dkv_parts(int total, int most, int chunk) { return max(1, min(most, (total + chunk - 1) / chunk)); }
+// The place of a tile's first part, so that memory follows the work and not the longest recording times the tiles: the tiles before it in the list hold `before`
+// query tiles per head (counted by the keys' capacity: at least as many as there are) and take the sum of ceil(their G / chunk) places, which
+// floor(before G / chunk) + their number is never less than.
+__device__ __forceinline__ long dkv_slot(const PAttnArgs& a, const int* rec, int ti, int kvh) {
+    const unsigned long before = (unsigned)rec[6] | (unsigned long)(unsigned)rec[7] << 32;
+    return kvh * a.slots + (long)(before * (unsigned)(a.hq / a.hkv) / (unsigned)a.chunk) + ti;
+}
 
 // dk, dv: 128 keys of one (recording, key head), a wave 32 (lanes = keys); the query heads of the group and the 64-query tiles stream by.
 // A stream of more than `chunk` tiles is shared between up to nsplit workgroups: f32 partials, added in order by packed_attn_dkv_join_kernel.
@@ -1067,7 +1075,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP == 64 ? 3 : waves_per_si
         store_rows<T, DP>(a.dk + krow * a.sdk.rs + (long)kvh * a.sdk.hs, live, dk, a.scale, a.D, oh);
         store_rows<T, DP>(a.dv + krow * a.sdv.rs + (long)kvh * a.sdv.hs, live, dv, 1.f, a.D, oh);
     } else {
-        float* p = a.part + ((((long)ti * a.hkv + kvh) * a.nsplit + split) * 2 * TILE + orow) * DP;
+        float* p = a.part + ((dkv_slot(a, rec, ti, kvh) + split) * 2 * TILE + orow) * DP;
         store_rows<float, DP>((char*)p, true, dk, a.scale, DP, oh);
         store_rows<float, DP>((char*)(p + (long)TILE * DP), true, dv, 1.f, DP, oh);
     }
@@ -1083,7 +1091,7 @@ __global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(PAttnArgs a) 
     const int ns = dkv_parts(per * (a.hq / a.hkv), a.nsplit, a.chunk);
     const int i = at * 256 + threadIdx.x, which = i / (TILE * DP / 8), row = i / (DP / 8) % TILE, d = i % (DP / 8) * 8;
     if (ns == 1 || row >= rows || d >= a.D) return;
-    const float* p = a.part + (((long)ti * a.hkv + kvh) * a.nsplit * 2 + which) * TILE * DP + row * DP + d;
+    const float* p = a.part + (dkv_slot(a, rec, ti, kvh) * 2 + which) * TILE * DP + row * DP + d;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int x = 0; x < ns; ++x) {
@@ -1150,6 +1158,13 @@ int dkv_chunk(const Plan& p, int hq, int D, int causal, int dtype) {
 int dkv_splits(const Plan& p, int hq, int hkv, int D, int causal, int dtype) {
     const long longest = (p.max_q + KT - 1) / KT * (hq / hkv), c = dkv_chunk(p, hq, D, causal, dtype);
     return longest > c ? (int)((longest + c - 1) / c) : 1;
+}
+// Parts of dk/dv to reserve per key head (dkv_slot; 0: nothing is cut). Only tiles of more than `chunk` steps are cut, the first n of the list, which is in the
+// order of their steps: the last of them ends at most at ceil(all steps / chunk) + n - 1. That is at most twice the parts the work is cut into.
+long dkv_slots(const Plan& p, int hq, int hkv, int D, int causal, int dtype) {
+    if (dkv_splits(p, hq, hkv, D, causal, dtype) == 1) return 0;
+    const long steps = (causal ? p.k_work_causal : p.k_work) * (hq / hkv), c = dkv_chunk(p, hq, D, causal, dtype), n = steps / c < p.k_tiles ? steps / c : p.k_tiles;
+    return (steps + c - 1) / c + (n > 1 ? n - 1 : 0);
 }
 bool delta_pass(int dtype, bool table_grad) { return table_grad && dtype == PSELD_BF16; }
 
@@ -1238,6 +1253,7 @@ int run_bwd(PAttnArgs& a, const Plan& p, float* dtable, int accumulate, hipStrea
     a.bias_heads = BIAS ? (DP == 128 || 2 * nd > 12288 ? 1 : min(a.hq / a.hkv, 12288 / nd)) : 0;      // (two workgroups per CU stay possible)
     a.nsplit = dkv_splits(p, a.hq, a.hkv, a.D, a.causal, dtype);
     a.chunk = dkv_chunk(p, a.hq, a.D, a.causal, dtype);
+    a.slots = dkv_slots(p, a.hq, a.hkv, a.D, a.causal, dtype);
     PA_LAUNCH((packed_attn_dkv_kernel<T, DP, BIAS>), p.k_tiles * a.hkv * a.nsplit, 256, 4 * TB + 4 * KT * 4 + 4096 * (dkv_lds_frags<T, DP, BIAS>()) + a.bias_heads * nd, a);
     if (a.nsplit > 1) PA_LAUNCH((packed_attn_dkv_join_kernel<T, DP>), p.k_tiles * a.hkv * (TILE * DP / 1024), 256, 0, a);
     return PSELD_OK;
@@ -1293,13 +1309,11 @@ extern "C" int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, co
     return PSELD_OK;
 }
 
-extern "C" long pseld_packed_attn_bwd_workspace(const long* plan, int hq, int hkv, int D, int causal, int buckets) {
+extern "C" long pseld_packed_attn_bwd_workspace(int dtype, const long* plan, int hq, int hkv, int D, int causal, int buckets) {
     if (!plan || hkv <= 0 || hq < hkv || hq % hkv) return 0;
     const Plan p = plan_of(plan);
-    long n = dkv_splits(p, hq, hkv, D, causal, PSELD_BF16);
-    const long n4 = dkv_splits(p, hq, hkv, D, causal, PSELD_F32);
-    if (n4 > n) n = n4;
-    return ((p.rows * hq + 3) / 4 * 4 + 2 * p.q_tiles * hq * buckets + 4 + (n > 1 ? p.k_tiles * hkv * n * 2 * TILE * pad_of(D) : 0)) * (long)sizeof(float);
+    const long q_tiles = p.q_tiles * (dtype == PSELD_F32 ? key_split<float>() : key_split<bf16_t>());
+    return ((p.rows * hq + 3) / 4 * 4 + q_tiles * hq * buckets + 4 + hkv * dkv_slots(p, hq, hkv, D, causal, dtype) * 2 * TILE * pad_of(D)) * (long)sizeof(float);
 }
 
 extern "C" int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
@@ -1327,7 +1341,7 @@ extern "C" int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q,
         for (const void* x : others) PSELD_CHECK_ARG(!x || x != results[i], "%s: a gradient must not be an operand or another gradient", n);
     }
     PSELD_CHECK_ARG(!rows || lse, "packed_attn_bwd: null pointer (lse)");
-    const long need = pseld_packed_attn_bwd_workspace(plan, hq, hkv, D, causal, dtable ? buckets : 0);
+    const long need = pseld_packed_attn_bwd_workspace(dtype, plan, hq, hkv, D, causal, dtable ? buckets : 0);
     PSELD_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, "packed_attn_bwd: workspace too small");
     a.dout = (const char*)dout; a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (const char*)out; a.lse = const_cast<float*>(lse);
     a.dq = (char*)dq; a.dk = (char*)dk; a.dv = (char*)dv;

@@ -1599,21 +1599,8 @@ class PackedPlan:
             self.device = torch.device('cuda', torch.cuda.current_device())
         self._index = self.device.index
         q_start, k_start = np.cumsum(q) - q, np.cumsum(cap) - cap
-        # work lists, heaviest tile first: every 128-row tile of queries and of keys, ordered for full attention (by the other side's length)
-        # and for causal attention (by how much of the other side the mask leaves)
-        per = np.stack([q_start, q, k_start, cap, np.zeros_like(q), np.zeros_like(q)], 1)
-
-        def tiles(lens, full, causal):
-            n = -(-lens // _PACKED_TILE)
-            s = np.repeat(np.arange(seqs), n)
-            first = (np.arange(len(s)) - np.repeat(np.cumsum(n) - n, n)) * _PACKED_TILE
-            rec = np.concatenate([s[:, None], first[:, None], per[s]], 1)
-            weights = full(s), causal(s, first)
-            return [rec[np.argsort(-w, kind='stable')] for w in weights], weights
-        (qf, qc), _ = tiles(q, lambda s: cap[s], lambda s, first: cap[s] - q[s] + first)
-        (kf, kc), weights = tiles(cap, lambda s: q[s], lambda s, first: np.minimum(q[s], cap[s] - first))
+        (qf, qc), (kf, kc), work = _packed_work(q, cap)
         self.q_tiles, self.k_tiles = len(qf), len(kf)
-        work = [int((-(-np.maximum(w, 0) // 64)).sum()) for w in weights]      # 64-query tiles that a key tile meets, summed
         host, at, end = [], {}, 0
         for name, values in (('q_start', q_start), ('q_len', q), ('k_start', k_start), ('k_cap', cap), ('k_len', k), ('q_tile', qf),
                              ('q_tile_causal', qc), ('k_tile', kf), ('k_tile_causal', kc)):
@@ -1628,6 +1615,32 @@ class PackedPlan:
 
 
 _PACKED_TILE = 128
+
+
+def _packed_work(q, cap):
+    """The work lists of recordings with q queries and slabs of cap keys: 128-row tiles of queries and of keys, each ordered for full attention (by the
+    other side's length) and for causal attention (by how much of the other side the mask leaves), heaviest first; and the 64-query tiles that the
+    key tiles meet, summed, full and causal. A key tile's record ends with the sum over the tiles before it, in two halves."""
+    q_start, k_start = np.cumsum(q) - q, np.cumsum(cap) - cap
+    per = np.stack([q_start, q, k_start, cap, np.zeros_like(q), np.zeros_like(q)], 1)
+
+    def tiles(lens):
+        n = -(-lens // _PACKED_TILE)
+        s = np.repeat(np.arange(len(lens)), n)
+        first = (np.arange(len(s)) - np.repeat(np.cumsum(n) - n, n)) * _PACKED_TILE
+        return s, first, np.concatenate([s[:, None], first[:, None], per[s]], 1)
+    s, first, rec = tiles(q)
+    queries = [rec[np.argsort(-w, kind='stable')] for w in (cap[s], cap[s] - q[s] + first)]
+    s, first, rec = tiles(cap)
+    keys, work = [], []
+    for w, start in ((q[s], np.zeros_like(first)), (np.minimum(q[s], cap[s] - first), np.maximum(0, first - cap[s] + q[s]) // 64 * 64)):
+        met = -(-np.maximum(0, q[s] - start) // 64)
+        order = np.lexsort((-w, -met))
+        listed, before = rec[order], np.cumsum(met[order]) - met[order]
+        listed[:, 6], listed[:, 7] = before & 0xffffffff, before >> 32
+        keys.append(listed)
+        work.append(int(met.sum()))
+    return queries, keys, work
 
 
 def packed_plan(q_lens, k_lens=None, k_cap=None, device='cuda'):
@@ -1865,7 +1878,7 @@ def packed_attn_bwd(dout, q, k, v, out, lse, plan, causal=False, scale=None, bia
         raise _lib.PseldError("packed_attn_bwd: dbias_table must be contiguous float32 of bias_table's shape, beside bias_table and buckets")
     L = _lib.lib()
     table, lut, nb, md = _table_args(bias_table, buckets)
-    nbytes = L.pseld_packed_attn_bwd_workspace(plan._desc, hq, hkv, D, 1 if causal else 0, nb if dbias_table is not None else 0)
+    nbytes = L.pseld_packed_attn_bwd_workspace(dtype_code(q), plan._desc, hq, hkv, D, 1 if causal else 0, nb if dbias_table is not None else 0)
     ws = torch.empty((nbytes + 15) // 16 * 4, dtype=torch.float32, device=plan.device)
     strides = _LONGS16(*[n for t in (dout, q, k, v, out, dq, dk, dv) for n in t.stride()[:2]])
     rc = L.pseld_packed_attn_bwd(dtype_code(q), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(),

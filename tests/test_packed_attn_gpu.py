@@ -571,3 +571,81 @@ def test_a_nan_query_shows_in_its_own_row_alone(dev, dtype, q_lens, k_lens, row)
     assert torch.equal(torch.isnan(lse), want) and not torch.isinf(lse).any()
     for t in (out, dq):
         assert torch.equal(torch.isnan(t).all(-1), want) and torch.equal(torch.isnan(t).any(-1), want)
+
+
+def _plan_array(q, cap):
+    """The host array of a plan with these lengths (addresses that are never followed), and its key lists."""
+    import ctypes
+    import numpy as np
+    from pseldnets_amd import ops
+    (qf, _), keys, work = ops._packed_work(np.array(q), np.array(cap))
+    return (ctypes.c_long * 18)(len(q), sum(q), max(q), sum(cap), max(cap), len(qf), len(keys[0]), *work, *[4096] * 9), keys, work
+
+
+def test_backward_workspace_follows_the_work():
+    """Packs of long and short recordings: what the parts of dk and dv take is bounded by the number of parts that the work is cut into (at most 700, twice that
+    with the tiles' ends), 128 x 2 x 128 floats each, whatever the longest recording times the number of tiles would be. It was 1.7 and 3.3 GB."""
+    import os
+    from pseldnets_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("libpseld_hip.so not built")
+    for q, hq, hkv in (([6000] + [500] * 60, 8, 1), ([12000] + [2000] * 100, 16, 2), ([8191], 16, 2), ([1] * 1000 + [30000], 4, 4)):
+        plan, _, _ = _plan_array(q, q)
+        for dtype, parts in ((0, 700), (1, 400)):
+            for causal in (0, 1):
+                size = _lib.lib().pseld_packed_attn_bwd_workspace(dtype, plan, hq, hkv, 128, causal, 0)
+                assert size <= 2 * parts * 2 * 128 * 128 * 4 + 4 * sum(q) * hq + 64, (q[0], dtype, causal)
+
+
+def test_parts_of_dk_and_dv_have_places_of_their_own():
+    """What the dk/dv kernel writes and its joining launch reads, computed here from the lists: over every kind of pack, and with caches that are shorter than their
+    capacity when the call is made, the places of two key tiles' parts never meet and all lie inside the workspace."""
+    import os
+    import random
+    from pseldnets_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("libpseld_hip.so not built")
+    rng, cut = random.Random(3), 0
+    for case_ in range(150):
+        n = rng.randint(1, 12)
+        q = [rng.choice([0, 1, rng.randint(0, 500), rng.randint(0, 9000)]) for _ in range(n)]
+        cap = list(q) if case_ % 3 == 0 else [max(0, x + rng.randint(-300, 900)) if rng.random() < 0.7 else rng.randint(0, 9000) for x in q]
+        hkv = rng.choice([1, 2, 4])
+        G = rng.choice([1, 2, 8])
+        D = rng.choice([32, 64, 128])
+        pad = 32 if D <= 32 else 64 if D <= 64 else 128
+        plan, keys, work = _plan_array(q, cap)
+        for causal in (0, 1):
+            for dtype in (0, 1):
+                parts, least = (700, 1) if dtype == 0 else (400 if D > 64 else 600, 4)
+                steps = work[causal] * hkv * G
+                chunk = max(least, min(1 << 20, -(-steps // parts)))
+                longest = -(-max(q) // 64) * G
+                most = -(-longest // chunk) if longest > chunk else 1
+                size = _lib.lib().pseld_packed_attn_bwd_workspace(dtype, plan, hkv * G, hkv, D, causal, 0) - 4 * ((sum(q) * hkv * G + 3) // 4 * 4) - 16
+                assert size % (hkv * 2 * 128 * pad * 4) == 0
+                slots = size // (hkv * 2 * 128 * pad * 4)
+                for k_len in (cap, [rng.randint(0, c) for c in cap]):
+                    end = 0
+                    for t, (s, first, _, q_len, _, k_cap, low, high) in enumerate(keys[causal].tolist()):
+                        start = q_len if first >= k_len[s] else max(0, first - (k_len[s] - q_len)) // 64 * 64 if causal else 0
+                        total = (-(-(q_len - start) // 64) if start < q_len else 0) * G
+                        ns = max(1, min(most, -(-total // chunk)))
+                        if ns == 1:
+                            continue
+                        cut += 1
+                        place = (low + (high << 32)) * G // chunk + t
+                        assert place >= end and place + ns <= slots
+                        end = place + ns
+    assert cut > 1000
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_long_recording_among_short_ones(dev, dtype, D):
+    """Some key tiles are cut into many parts, some into a few, most into none."""
+    lens = [40, 1500, 7, 300, 130, 1, 0, 65, 129] + [50] * 6
+    case(dev, dtype, lens, 4, 1, D, True)
+    case(dev, dtype, lens, 4, 2, D, False, bias=(32, 128, True))
+    case(dev, dtype, [700, 3, 90, 0], 4, 1, D, True, bias=(16, 50, False), k_lens=[1100, 64, 0, 12], cap=[1400, 64, 300, 700])
