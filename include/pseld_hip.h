@@ -512,7 +512,7 @@ int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void* g, long l
  *   lse[row, head] = log sum exp S;  a row without keys: out 0, lse -inf. Query i of a recording stands at position i + k_len - q_len; causal: keys
  *   behind a query's position are masked. |table| / scale is taken to be below 1e37.
  * plan: HOST array of 18 longs {seqs, rows, max_q, k_rows, max_k, q_tiles, k_tiles, the 64-query tiles that the key tiles meet, summed: full and
- * causal, then device int arrays as addresses: q_start[seqs], q_len[seqs], k_start[seqs], k_cap[seqs], k_len[seqs], q_tile[q_tiles][8], q_tile_causal, k_tile[k_tiles][8], k_tile_causal}: a tile is 128 rows
+ * causal, then device int arrays as addresses: q_start[seqs], q_len[seqs], k_start[seqs], k_cap[seqs] (slabs one behind the other, in order), k_len[seqs], q_tile[q_tiles][8], q_tile_causal, k_tile[k_tiles][8], k_tile_causal}: a tile is 128 rows
  * of queries or of capacity, {recording s, first row, q_start[s], q_len[s], k_start[s], k_cap[s], low, high}, heaviest first; low, high: 0 for queries, for keys the 64-query tiles
  * that the key tiles before it in its list meet, summed, in 64 bits (key tiles stand in the order of the query tiles they meet; a key tile at row r meets those
  * from row max(0, r - k_cap + q_len) / 64 * 64 on when causal, all otherwise). k_len may change between calls; it is held to 0 .. k_cap.

@@ -45,7 +45,7 @@ struct PAttnArgs {
     const float* table; const int* lut; const int* ranges;      // [buckets, hq]; bucket of distance -max .. max; [buckets, 2] first and last distance
     int buckets, maxd;
     float* part;                // dtable: [tiles, hq, buckets]; split dk/dv: [hkv, slots, 2, TILE, DP]; few rows: see there
-    long slots;                 // dk, dv: parts reserved per key head
+    long slots;                 // dk, dv: parts reserved per key head; few rows: chunks
     int max_rows;               // few rows: rows reserved per key head
     int bias_heads;             // dk, dv: heads whose bias LDS has room for
 };
@@ -505,6 +505,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void packed_attn_fw
 // waves 32-key blocks in turn; a wave streams its own blocks through its own LDS (no barrier in the loop) and the waves' maxima, sums
 // and outputs are joined through LDS. More than one chunk per recording: f32 partials and a joining launch, both in a fixed order. HBM
 // bound: K and V are read once for all rows that share them.
+// The place of a recording's first chunk: slabs lie one behind the other, so those before this one, of k_start rows together, take the sum of ceil(capacity / chunk)
+// places, which floor(k_start / chunk) + their number is never less than.
+__device__ __forceinline__ long few_slot(const PAttnArgs& a, int seq, int kvh) { return kvh * a.slots + (unsigned)a.k_start[seq] / (unsigned)a.chunk + seq; }
 template <typename T, int DP, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
     using I = Image<T, DP>;
@@ -601,7 +604,7 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_few_kernel(PAttnArgs a) {
             *(f32x4*)(oi + r * PITCH + dt * 32 + 8 * gg + 4 * h2) = f32x4{sm.ot[dt][4 * gg] * f, sm.ot[dt][4 * gg + 1] * f, sm.ot[dt][4 * gg + 2] * f, sm.ot[dt][4 * gg + 3] * f};
     if (wave == 0 && h2 == 0) { all[r] = mt; all[32 + r] = lt; }
     __syncthreads();
-    const long pslot = ((long)(seq * a.hkv + kvh) * a.nsplit + split) * a.max_rows;
+    const long pslot = (few_slot(a, seq, kvh) + split) * a.max_rows;
     for (int i = threadIdx.x; i < rows * (a.D / 4); i += 64 * NW) {
         const int row = i / (a.D / 4), d = (i - row * (a.D / 4)) * 4;
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
@@ -630,7 +633,7 @@ __global__ __launch_bounds__(64) void packed_attn_join_kernel(PAttnArgs a) {
     if (row >= a.q_len[seq] * G) return;
     const int k_len = max(0, min(a.k_len[seq], a.k_cap[seq]));
     const int n = max(1, (k_len + a.chunk - 1) / a.chunk);
-    const float* p = a.part + ((long)(seq * a.hkv + kvh) * a.nsplit * a.max_rows + row) * (a.D + 4);
+    const float* p = a.part + (few_slot(a, seq, kvh) * a.max_rows + row) * (a.D + 4);
     const long step = (long)a.max_rows * (a.D + 4);
     float m = -__builtin_inff();
     for (int i = lane; i < n; i += 64) m = fmaxf(m, p[i * step]);
@@ -1144,6 +1147,11 @@ int few_chunk(const Plan& p, int hkv) {
     return (int)((c < least ? least : c > most ? most : c) + 127) / 128 * 128;
 }
 int few_splits(const Plan& p, int hkv) { const int c = few_chunk(p, hkv); return p.max_k > c ? (int)((p.max_k + c - 1) / c) : 1; }
+// Chunks to reserve per key head (few_slot; 0: no recording is cut). A recording without capacity has one too, which answers for its rows.
+long few_slots(const Plan& p, int hkv) {
+    const long c = few_chunk(p, hkv);
+    return p.max_k <= c ? 0 : p.seqs > 1 ? p.k_rows / c + p.seqs : (p.k_rows + c - 1) / c;
+}
 // Query tiles per workgroup of the dk/dv kernel: the whole work is cut into equal parts where the key tiles alone would not fill the chip or end
 // unevenly: as many as about four fifths of the places (the tiles' odd ends take the rest), so that all run at once. Two workgroups fit a CU at heads
 // above 64 (1 x 8191, 16/2 heads of 128, forward + backward: 256 parts 1577 us, 330 1372, 400 1283, 460 1608), three below (12 x 100-1200, 16/4
@@ -1216,6 +1224,7 @@ int run_fwd(PAttnArgs& a, const Plan& p, hipStream_t s) {
         const int G = a.hq / a.hkv;
         a.chunk = few_chunk(p, a.hkv);
         a.nsplit = few_splits(p, a.hkv);
+        a.slots = few_slots(p, a.hkv);
         a.max_rows = (int)p.max_q * G;
         const int lds = NW * 4 * WR * DP * (int)sizeof(T) + (NW + 1) * 256 + (BIAS ? a.buckets * G * 4 + (2 * a.maxd + 1) * 2 : 0);
         PA_LAUNCH((packed_attn_few_kernel<T, DP, NW, BIAS>), p.seqs * a.nsplit * a.hkv, 64 * NW, lds, a);
@@ -1277,8 +1286,7 @@ extern "C" long pseld_packed_attn_fwd_workspace(const long* plan, int hq, int hk
     if (!plan || hkv <= 0 || hq < hkv || hq % hkv) return 0;
     const Plan p = plan_of(plan);
     if (!few_rows(p, hq, hkv, buckets)) return 0;
-    const long n = few_splits(p, hkv);
-    return n > 1 ? p.seqs * hkv * n * p.max_q * (hq / hkv) * (D + 4) * (long)sizeof(float) : 0;
+    return few_slots(p, hkv) * hkv * p.max_q * (hq / hkv) * (D + 4) * (long)sizeof(float);
 }
 
 extern "C" int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const long* strides,

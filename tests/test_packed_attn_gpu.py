@@ -649,3 +649,45 @@ def test_a_long_recording_among_short_ones(dev, dtype, D):
     case(dev, dtype, lens, 4, 1, D, True)
     case(dev, dtype, lens, 4, 2, D, False, bias=(32, 128, True))
     case(dev, dtype, [700, 3, 90, 0], 4, 1, D, True, bias=(16, 50, False), k_lens=[1100, 64, 0, 12], cap=[1400, 64, 300, 700])
+
+
+def test_chunks_of_unequal_caches_have_places_of_their_own():
+    """Few rows over caches of different capacities: what the chunks take follows the rows of all caches together (it was the longest cache's chunks for every
+    recording, more than the caches themselves: 448 MB beside 257), and no two recordings' chunks meet, with empty caches among them and behind."""
+    import os
+    import random
+    from pseldnets_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("libpseld_hip.so not built")
+    size = _lib.lib().pseld_packed_attn_fwd_workspace
+    for caps, q, hq, hkv, D, most in (([131072] + [600] * 200, 8, 16, 4, 64, 12e6), ([1 << 20] + [512] * 999, 1, 32, 8, 128, 21e6)):
+        assert size(_plan_array([q] * len(caps), caps)[0], hq, hkv, D, 0) <= most
+    rng, cut = random.Random(5), 0
+    for _ in range(200):
+        n, hkv, D = rng.randint(1, 20), rng.choice([1, 2, 8]), rng.choice([8, 64, 128])
+        caps = [rng.choice([0, 1, 256 * rng.randint(0, 40), rng.randint(0, 30000)]) for _ in range(n)]
+        total = sum(caps)
+        need = size(_plan_array([1] * n, caps)[0], hkv, hkv, D, 0)
+        chunk = 512 if max(caps) <= 512 else max(256, min(8192, -(-((total * hkv + 511) // 512) // 128) * 128))      # keys per chunk
+        if max(caps) <= chunk:
+            assert need == 0
+            continue
+        slots, rest = divmod(need, hkv * (D + 4) * 4)
+        assert rest == 0
+        first, end = 0, 0
+        for s, cap in enumerate(caps):
+            place = first // chunk + s
+            assert place >= end
+            end = place + max(1, -(-cap // chunk))
+            assert end <= slots
+            first += cap
+            cut += cap > chunk
+    assert cut > 300
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+def test_few_rows_over_unequal_caches(dev, dtype):
+    """Recordings cut into many chunks beside empty ones, an empty one last behind whole chunks."""
+    case(dev, dtype, [1, 2, 1, 3], 8, 2, 64, True, bias=(32, 128, False), k_lens=[5000, 0, 700, 0], cap=[5120, 0, 768, 0], backward=False)
+    case(dev, dtype, [1, 1, 0, 1, 1], 4, 4, 128, False, k_lens=[1, 3000, 40, 0, 513], cap=[300, 3333, 600, 0, 600], backward=False)
