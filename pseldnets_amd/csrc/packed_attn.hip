@@ -1303,7 +1303,7 @@ extern "C" int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, co
     PA_TRY(check_result("packed_attn_fwd", "out", dtype, out, strides + 6, a.so, p.rows, hq, D));
     PSELD_CHECK_ARG(!rows || lse, "packed_attn_fwd: null pointer (lse)");
     const long need = pseld_packed_attn_fwd_workspace(plan, hq, hkv, D, table ? buckets : 0);
-    PSELD_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "packed_attn_fwd: workspace too small");
+    PSELD_CHECK_ARG(need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need), "packed_attn_fwd: workspace too small or not on a 16-byte boundary");
     PSELD_CHECK_ARG(!rows || (out != q && out != k && out != v), "packed_attn_fwd: out must not be an operand");
     if (!rows) return PSELD_OK;
     a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.out = (char*)out; a.lse = lse; a.part = workspace;
@@ -1350,7 +1350,7 @@ extern "C" int pseld_packed_attn_bwd(int dtype, const void* dout, const void* q,
     }
     PSELD_CHECK_ARG(!rows || lse, "packed_attn_bwd: null pointer (lse)");
     const long need = pseld_packed_attn_bwd_workspace(dtype, plan, hq, hkv, D, causal, dtable ? buckets : 0);
-    PSELD_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, "packed_attn_bwd: workspace too small");
+    PSELD_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, "packed_attn_bwd: workspace too small or not on a 16-byte boundary");
     a.dout = (const char*)dout; a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (const char*)out; a.lse = const_cast<float*>(lse);
     a.dq = (char*)dq; a.dk = (char*)dk; a.dv = (char*)dv;
     a.delta = workspace;

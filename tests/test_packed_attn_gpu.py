@@ -691,3 +691,22 @@ def test_few_rows_over_unequal_caches(dev, dtype):
     """Recordings cut into many chunks beside empty ones, an empty one last behind whole chunks."""
     case(dev, dtype, [1, 2, 1, 3], 8, 2, 64, True, bias=(32, 128, False), k_lens=[5000, 0, 700, 0], cap=[5120, 0, 768, 0], backward=False)
     case(dev, dtype, [1, 1, 0, 1, 1], 4, 4, 128, False, k_lens=[1, 3000, 40, 0, 513], cap=[300, 3333, 600, 0, 600], backward=False)
+
+
+def test_c_entry_refuses_a_workspace_off_its_boundary():
+    """Both directions read their workspaces in 16-byte pieces."""
+    import ctypes
+    import os
+    from pseldnets_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("libpseld_hip.so not built")
+    L = _lib.lib()
+    A = [4096 * i for i in range(1, 12)]                     # addresses that are never followed
+    plan, st = _plan_array([1], [100000])[0], (ctypes.c_long * 16)(*[256, 64] * 8)
+    assert L.pseld_packed_attn_fwd_workspace(plan, 4, 4, 64, 0) > 0
+    for off in (4, 8):
+        assert L.pseld_packed_attn_fwd(0, A[0], A[1], A[2], A[3], A[9], st, plan, 4, 4, 64, 0, 1.0, None, None, 0, 0, A[10] + off, 1 << 40, None) == -1
+        assert b"boundary" in L.pseld_last_error()
+        assert L.pseld_packed_attn_bwd(0, A[4], A[0], A[1], A[2], A[3], A[9], A[5], A[6], A[7], st, plan, 4, 4, 64, 0, 1.0, None, None, 0, 0, None, 0,
+                                       A[10] + off, 1 << 40, None) == -1
+        assert b"boundary" in L.pseld_last_error()
