@@ -1725,7 +1725,8 @@ def linrec_bwd(dh, g, n, saved, plan, dh_last=None, h0=None, reverse=False, dg=N
     C = g.shape[1]
     _state_ok("linrec_bwd", plan, C, h0, dh_last)
     L = _lib.lib()
-    if saved is None or tuple(saved.shape) != (L.pseld_linrec_states(plan.rows, plan.seqs), C) or saved.dtype != torch.float32 or saved.device != plan.device:
+    if saved is None or tuple(saved.shape) != (L.pseld_linrec_states(plan.rows, plan.seqs), C) or saved.dtype != torch.float32 or saved.device != plan.device or \
+            not saved.is_contiguous():
         raise _lib.PseldError("linrec_bwd: saved must be what linrec_fwd(need_saved=True) returned for this plan")
     dg = g.new_empty((plan.rows, C)) if dg is None else dg
     dn = g.new_empty((plan.rows, C)) if dn is None else dn

@@ -265,3 +265,21 @@ def test_plan_fails_loudly_without_gpu():
     with pytest.raises(_lib.PseldError):
         ops.packed_plan([3, 4], device='cpu')
     assert not t.cuda.is_available() or ops.packed_plan([3, 4]).rows == 7
+
+
+@pytest.mark.gpu
+def test_backward_refuses_states_whose_rows_lie_apart(dev):
+    """A strided view of the kept states has their shape and would be read as if it were packed: wrong gradients without an error."""
+    from pseldnets_amd import _lib, ops
+    lens, C = [100, 30], 16
+    both, dh, _, _ = make(dev, torch.float32, lens, C, 9)
+    g, n = both[:, :C], both[:, C:]
+    plan = ops.packed_plan(lens, device=dev)
+    _, _, saved = ops.linrec_fwd(g, n, plan)
+    apart = torch.stack([saved, saved + 1], 1)[:, 0]
+    assert torch.equal(apart, saved) and not apart.is_contiguous()
+    with pytest.raises(_lib.PseldError):
+        ops.linrec_bwd(dh, g, n, apart, plan)
+    want = ops.linrec_bwd(dh, g, n, saved, plan)
+    got = ops.linrec_bwd(dh, g, n, apart.contiguous(), plan)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
