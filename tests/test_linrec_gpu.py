@@ -283,3 +283,18 @@ def test_backward_refuses_states_whose_rows_lie_apart(dev):
     want = ops.linrec_bwd(dh, g, n, saved, plan)
     got = ops.linrec_bwd(dh, g, n, apart.contiguous(), plan)
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_states_into_a_view_of_the_caller(dev, dtype):
+    from pseldnets_amd import ops
+    lens, C = [65, 0, 300], 40
+    both, _, h0, _ = make(dev, dtype, lens, C, 10)
+    plan = ops.packed_plan(lens, device=dev)
+    wide = torch.full((sum(lens), 3 * C), float('nan'), dtype=dtype, device=dev)
+    for reverse in (False, True):
+        want, last, _ = ops.linrec_fwd(both[:, :C], both[:, C:], plan, h0=h0, reverse=reverse)
+        got, last2, _ = ops.linrec_fwd(both[:, :C], both[:, C:], plan, h0=h0, reverse=reverse, out=wide[:, C:2 * C])
+        assert got.data_ptr() == wide[:, C:].data_ptr() and torch.equal(got, want) and torch.equal(last, last2)
+        assert bool(torch.isnan(wide[:, :C]).all()) and bool(torch.isnan(wide[:, 2 * C:]).all())

@@ -710,3 +710,35 @@ def test_c_entry_refuses_a_workspace_off_its_boundary():
         assert L.pseld_packed_attn_bwd(0, A[4], A[0], A[1], A[2], A[3], A[9], A[5], A[6], A[7], st, plan, 4, 4, 64, 0, 1.0, None, None, 0, 0, None, 0,
                                        A[10] + off, 1 << 40, None) == -1
         assert b"boundary" in L.pseld_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("q_lens,k_lens", [([70, 1, 130], None), ([2, 1, 1], [600, 9, 1300])])
+def test_head_major_operands_and_results_of_the_caller(dev, dtype, q_lens, k_lens):
+    """Heads outside rows, for operands and for every result that a caller may pass (out=, dq=, dk=, dv=); whole recordings and few rows."""
+    from pseldnets_amd import ops
+    hq, hkv, D = 4, 2, 64
+    plan = ops.packed_plan(q_lens, k_lens, device=dev)
+    heads_out = lambda rows, heads, seed: rnd((heads, rows, D), seed, dtype, dev).transpose(0, 1)      # noqa: E731
+    q, k, v, dout = heads_out(plan.rows, hq, 1), heads_out(plan.k_rows, hkv, 2), heads_out(plan.k_rows, hkv, 3), heads_out(plan.rows, hq, 4)
+    kept, dq, dk, dv = (torch.full_like(t, float('nan')) for t in (q, q, k, v))
+    assert kept.stride() == (D, plan.rows * D, 1)
+    out, lse = ops.packed_attn_fwd(q, k, v, plan, causal=True, out=kept)
+    grads = ops.packed_attn_bwd(dout, q, k, v, out, lse, plan, causal=True, dq=dq, dk=dk, dv=dv)
+    assert out is kept and all(a is b for a, b in zip(grads, (dq, dk, dv)))
+    kl = k_lens if k_lens is not None else q_lens
+    want = reference(q, k, v, dout, q_lens, kl, starts_of(kl), True, D ** -0.5)
+    compare(dict(out=out, lse=lse, dq=dq, dk=dk, dv=dv), want)
+    rows_out = torch.full((plan.rows, 3, hq, D), float('nan'), dtype=dtype, device=dev)      # heads inside rows, rows apart
+    again, lse2 = ops.packed_attn_fwd(q.contiguous(), k.contiguous(), v.contiguous(), plan, causal=True, out=rows_out[:, 1])
+    assert torch.equal(again, out) and torch.equal(lse2, lse) and bool(torch.isnan(rows_out[:, 0::2]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+def test_one_frame_of_heads_or_buckets_past_the_few_rows_kernel(dev, dtype):
+    """More than 32 query heads a key head, more table entries than the few-rows kernel holds: the query-tiled kernel answers for single frames too."""
+    case(dev, dtype, [1, 3, 1], 64, 1, 64, True, k_lens=[300, 40, 0], cap=320)
+    case(dev, dtype, [1, 1], 40, 1, 32, False, bias=(32, 128, True), k_lens=[900, 33], cap=1000, backward=False)
+    case(dev, dtype, [1, 1], 16, 1, 64, True, bias=(320, 800, False), k_lens=[900, 33], cap=1000, backward=False)

@@ -273,3 +273,22 @@ def test_replays_up_to_the_capacity_and_past_it(dev):
             assert bool(torch.isnan(y).all()) and held.plan.k_len.tolist() == [cap] * S, t
         if not counted:
             assert bool(torch.isnan(dec.step(slot, held)).all())
+
+
+def test_einv2_network_with_the_stream_decoder_trains(dev):
+    """EINV2: the parameters of all six decoders get a gradient."""
+    from types import SimpleNamespace as A
+    from oracle import crnn as oc
+    from pseldnets_amd.models import einv2
+    cfg = A(data=A(n_mels=64, sample_rate=24000, hoplen=240), model=A(decoder='stream', num_decoder_layers=1), adapt=A())
+    net = einv2.CRNN(cfg, 3, 7, encoder='CNN12', pretrained_path=None, num_features=[8, 16, 16, 32, 32, 64])
+    net.to(dev).train()
+    pred = net(oc.random_features(2, seed=1).to(dev))
+    (pred['sed'].float().square().mean() + pred['doa'].float().square().mean()).backward()
+    seen = set()
+    for name, p in net.named_parameters():
+        assert p.grad is not None and bool(torch.isfinite(p.grad).all()), name
+        if '.decoder.' in name:
+            assert p.grad.abs().max().item() > 0, name
+            seen.add(name.split('.')[0])
+    assert len(seen) == 6
