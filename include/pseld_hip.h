@@ -521,6 +521,7 @@ int pseld_linrec_bwd(int dtype, const void* dh, long lddh, const void* g, long l
  * -max_distance .. max_distance, then [buckets][2] first and last distance of each (none: first > last).
  * bwd: dq, dk, dv (rows between k_len and k_cap get zeros) and, where dtable is not NULL, dtable (f32, accumulate: added to). With bf16 operands and a
  * table gradient the sums that enter it are formed from f32 probabilities. Deterministic (no floating atomics between lanes).
+ * Single frames up to 32 query rows per key head (and 4096 table entries) share a recording's keys between workgroups; other calls walk them by one workgroup per 128 queries and head.
  * workspace: the matching *_workspace bytes (buckets = 0: no table; bwd: no table gradient), 16-byte aligned. */
 long pseld_packed_attn_fwd_workspace(const long* plan, int hq, int hkv, int D, int buckets);
 int pseld_packed_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const long* strides,

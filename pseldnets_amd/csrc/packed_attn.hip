@@ -7,15 +7,16 @@
 //
 // No score matrix exists in HBM. Scores are computed TRANSPOSED in the forward and dq kernels (accumulator rows = keys, lanes = queries), so a
 // query's maximum and sum are lane-local but for one exchange of the wave's halves, and the probabilities are the B operand of the second
-// product as they stand; the dk/dv kernel has lanes = keys for the same reason. K / V (Q / dO) tiles of 64 rows reach LDS by LDS-DMA, two
-// buffers, one barrier per tile; rows are lane-linear with their 16-byte pieces XOR-swizzled on the source address (image_swizzle),
+// product as they stand; the dk/dv kernel has lanes = keys for the same reason. K / V (Q / dO) tiles of 64 rows reach LDS by LDS-DMA, into two
+// buffers with one barrier per tile (dq with the table's gradient for heads above 32: one buffer, two barriers, dq_buffers); rows are lane-linear with their 16-byte pieces XOR-swizzled on the source address (image_swizzle),
 // which leaves both the row reads and the transposed reads free of bank conflicts without padding. Rows past a recording's end are never
 // addressed: the DMA repeats the last row and the mask drops it, so what a cache holds behind its length does not matter.
 //
 // bias: the table column of the workgroup's head is laid out by DISTANCE in LDS once (dist_fill); a tile whose distances are all at or past the
 // last bucket adds one constant instead (it goes into the exponent's offset for free), the others read their diagonal's values.
-// Its gradient: every wave adds its dS to LDS sums by distance, one copy per half wave, so that no two lanes of an instruction meet and
-// the order of additions is fixed; sums per workgroup are folded to buckets, and a last launch adds the workgroups in order, in 64 bits.
+// Its gradient: every wave sums its dS along the diagonals of a tile and adds them to LDS sums by distance, a copy per wave (add_diagonals): no two
+// lanes of an instruction meet and the order of additions is fixed; sums per workgroup are folded to buckets, and a last launch adds the workgroups
+// in order, in 64 bits.
 // With bf16 operands O comes from rounded probabilities, so delta = dO O would be off by 2^-9 of itself - too coarse for the table's f32
 // gradient, whose sums cancel. There delta = sum_j P dP is computed in its own pass over the keys (DELTA mode) from f32 P and dP.
 #include "common.h"
@@ -1135,10 +1136,13 @@ Plan plan_of(const long* p) {
 int pad_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 constexpr int FEW_TABLE = 4096;          // table entries of one key head's group that the few-rows kernel keeps in LDS
 
-// The few-rows kernel takes the call when one key head's query rows of every recording fit its 32-row operand.
+// The few-rows kernel takes the call when one key head's query rows of every recording fit its 32-row operand and its LDS the group's part of the table. Other
+// calls go to the query-tiled kernel, which does not share a recording's keys between workgroups: 9 frames of 4 grouped heads over one cache of 131072 keys are
+// one workgroup a query head.
 bool few_rows(const Plan& p, int hq, int hkv, int buckets) { return p.max_q * (hq / hkv) <= WR && (long)buckets * (hq / hkv) <= FEW_TABLE; }
-// keys per workgroup: two workgroups per CU by the capacities, whole rounds of the four waves' blocks (3 streams of 60-131 k keys, 16/4 heads of
-// 64: 2048 workgroups 73 us, 1024 72, 512 68; 48 of 100-4096, 16/2 heads of 128: 48, 34, 33); a recording of up to 512 keys stays
+// keys per workgroup: 512 workgroups by the capacities, whole rounds of the four waves' blocks (3 streams of 60-131 k keys, 16/4 heads of
+// 64: 2048 workgroups 73 us, 1024 72, 512 68; 48 of 100-4096, 16/2 heads of 128: 48, 34, 33). Two fit a CU up to heads of 64 in bf16, above LDS holds one. The
+// cut knows the capacities alone: of the 48 unequal streams some 322 workgroups have keys, 1.26 rounds of the 256 places. A recording of up to 512 keys stays
 // whole (one launch instead of two). At most 16384 chunks, whose weights fit the joining launch's LDS.
 int few_chunk(const Plan& p, int hkv) {
     if (p.max_k <= 512) return 512;
@@ -1152,12 +1156,13 @@ long few_slots(const Plan& p, int hkv) {
     const long c = few_chunk(p, hkv);
     return p.max_k <= c ? 0 : p.seqs > 1 ? p.k_rows / c + p.seqs : (p.k_rows + c - 1) / c;
 }
-// Query tiles per workgroup of the dk/dv kernel: the whole work is cut into equal parts where the key tiles alone would not fill the chip or end
-// unevenly: as many as about four fifths of the places (the tiles' odd ends take the rest), so that all run at once. Two workgroups fit a CU at heads
-// above 64 (1 x 8191, 16/2 heads of 128, forward + backward: 256 parts 1577 us, 330 1372, 400 1283, 460 1608), three below (12 x 100-1200, 16/4
-// heads of 64: 500 parts 208 us, 600 184, 700 199, 900 194). Below 4 tiles a part would spend longer on its f32 partials than on its tiles. f32
-// tiles take longer: parts of any length (6 x 30-600, 8 heads of 64: 350 parts 196 us, 500 208, 700 196, 1500 197; 3 x 1000 causal, 4 heads of 128,
-// backward: 170 parts 344 us, 700 312).
+// Query tiles per workgroup of the dk/dv kernel: each key tile's stream is cut into parts of at most this many, where the key tiles alone would not fill the
+// chip or end unevenly. 400 and 600 parts of the whole work were the fastest of those tried (1 x 8191, 16/2 heads of 128, forward + backward, two
+// workgroups a CU: 256 parts 1577 us, 330 1372, 400 1283, 460 1608; 12 x 100-1200, 16/4 heads of 64, three a CU: 500 parts 208 us, 600 184, 700 199, 900 194): with
+// the tiles' odd ends those packs make 464 workgroups for 512 places and 684 for 768. Other packs end otherwise: 2 x 3000, 8/8 heads of 128, causal, makes 576 for
+// 512, 1 x 4000 + 60 x 100, 16/4 heads of 64, 832 for 768, and the last of them wait for a place. Below 4 tiles a part would spend longer on its f32
+// partials than on its tiles. f32 tiles take longer: parts of any length (6 x 30-600, 8 heads of 64: 350 parts 196 us, 500 208, 700 196, 1500 197; 3 x 1000
+// causal, 4 heads of 128, backward: 170 parts 344 us, 700 312).
 int dkv_chunk(const Plan& p, int hq, int D, int causal, int dtype) {
     const long work = (causal ? p.k_work_causal : p.k_work) * hq;
     const long parts = dtype == PSELD_F32 ? 700 : D > 64 ? 400 : 600, c = (work + parts - 1) / parts, least = dtype == PSELD_F32 ? 1 : 4;

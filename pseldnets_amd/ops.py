@@ -1831,7 +1831,9 @@ def packed_attn_fwd(q, k, v, plan, causal=False, scale=None, bias_table=None, bu
     stands at position i + k_len - q_len; causal masks the keys behind a query's position. A row without keys gives 0 and -inf. scale: D^-1/2 where None.
     bias_table f32 [buckets, query heads] with buckets = relpos_buckets(...): bias_table[bucket(key position - query position), head]
     is added to the scaled scores (-inf masks a bucket; finite entries stay below 1e37 scale). Key rows past a recording's k_len are never read. A value that
-    is not finite reaches, times a probability of 0, also the rows of its 64-key tile whose mask hides it. out must not overlap the operands."""
+    is not finite reaches, times a probability of 0, also the rows of its 64-key tile whose mask hides it. out must not overlap the operands. Calls whose longest
+    recording has at most 32 query rows per key head (frames x query heads / key heads), and a table of at most 4096 entries per key head, share the keys of long caches
+    between workgroups; beyond that a recording's keys are walked by one workgroup per 128 queries and head: split longer prompts over long caches into such calls."""
     stream, index = _on_plan("packed_attn_fwd", plan), plan._index
     key = (q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(), None if buckets is None else buckets.num_buckets)
     known = plan._layouts.get(key)
@@ -1861,7 +1863,8 @@ def packed_attn_fwd(q, k, v, plan, causal=False, scale=None, bias_table=None, bu
 def packed_attn_bwd(dout, q, k, v, out, lse, plan, causal=False, scale=None, bias_table=None, buckets=None, dbias_table=None, accumulate=False,
                     dq=None, dk=None, dv=None):
     """Gradients of packed_attn_fwd (same plan, lengths and options; out and lse are what it returned): (dq, dk, dv). dbias_table f32 [buckets, query heads]:
-    written (accumulate: added to) where given. dq, dk, dv: optional outputs (e.g. the parts of the projection's gradient), apart from the operands."""
+    written (accumulate: added to) where given. dq, dk, dv: optional outputs (e.g. the parts of the projection's gradient), apart from the operands. A key, value,
+    query or gradient that is not finite reaches, times a score gradient or probability of 0, also the other rows of its tile, as it does in the plain products."""
     what = "packed_attn_bwd"
     stream = _on_plan(what, plan)
     dtype, hq, hkv, D, scale = _packed_attn_args(what, plan, q, k, v, scale, bias_table, buckets)
