@@ -9,7 +9,7 @@ if sys.argv[1] == 'build':
     os.makedirs(out, exist_ok=True)
     for spec in sys.argv[2:]:
         name, _, defs = spec.partition(':')
-        cmd = ['hipcc', '--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wno-unused-result', '-shared'] + [d for d in defs.split(',') if d] + \
+        cmd = ['hipcc', '--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wno-unused-result', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '-shared'] + [d for d in defs.split(',') if d] + \
               [os.path.join(root, 'pseldnets_amd/csrc/feature.hip'), os.path.join(root, 'pseldnets_amd/csrc/runtime.hip'), '-o', os.path.join(out, name + '.so')]
         subprocess.check_call(cmd)
         print('built', name)

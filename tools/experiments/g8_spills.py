@@ -6,7 +6,7 @@ import os, re, subprocess, sys, tempfile
 root = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 pat = re.compile(sys.argv[1] if len(sys.argv) > 1 else r'gemm8_kernelILi[45]E')
 out = os.path.join(tempfile.gettempdir(), 'g8_spills.s')
-subprocess.check_call(['hipcc', '--offload-arch=gfx950', '-O3', '-std=c++17', '--cuda-device-only', '-S', os.path.join(root, 'pseldnets_amd/csrc/gemm8.hip'), '-o', out])
+subprocess.check_call(['hipcc', '--offload-arch=gfx950', '-O3', '-std=c++17', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '--cuda-device-only', '-S', os.path.join(root, 'pseldnets_amd/csrc/gemm8.hip'), '-o', out])
 lines = open(out).read().split('\n')
 for i0, l in enumerate(lines):
     m = re.match(r'(_ZN\S*gemm8_kernel\S*):', l)
