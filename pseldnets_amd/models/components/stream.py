@@ -146,15 +146,14 @@ class StreamDecoder:
         if state.remaining() < 1:
             raise _lib.PseldError(f"stream decoder: the streams' caches hold {state.capacity} frames and are full")
         x = x.contiguous()
-        room = plan.k_len < state.capacity
-        at = state.first + plan.k_len.clamp(max=state.capacity - 1)      # a replay past the capacity stays inside the slabs
-        plan.k_len.add_(room)
+        at = state.first + plan.k_len.clamp(0, state.capacity - 1)      # a replay past the capacity stays inside the slabs
+        plan.k_len.add_(1)
         try:
             x, states = self._step(x, state, at)
-            x.masked_fill_(~room[:, None], math.nan)
+            x.masked_fill_((plan.k_len > state.capacity)[:, None], math.nan)
         except BaseException:
             if not capturing:
-                plan.k_len.sub_(room.int())
+                plan.k_len.sub_(1)
             raise
         for kept, last in zip(state.states, states):
             kept.copy_(last)
