@@ -12,10 +12,11 @@
 // reference never exist in memory.
 //
 // Roofline: the HBM floor (5.634 MB algorithmic bytes per 10 s chunk: 3.84 MB in + 1.794 MB out -> 0.2 ms per 192 chunks) is NOT
-// what binds this kernel. Rounds 1-4 it was VALU-issue-bound (3 590, then 1 993 vector instructions per frame; profiles/r02_pmc_feature.json,
+// what binds this kernel. At first it was VALU-issue-bound (3 590, then 1 993 vector instructions per frame; profiles/r02_pmc_feature.json,
 // r04 / r05_pmc_feature.json). Then the complex arithmetic was written out half by half without moves between register pairs (in packed
-// fp32 first, in scalar instructions since: the same time, 0.92 against 0.93 ms inside the step) and the workgroups became persistent (tables built
-// once per CU): 1.22 -> 0.9 ms per 192 chunks. What is left is latency: 2 waves per SIMD (150 KB of LDS per workgroup = one workgroup per CU) walk a chain of four LDS exchanges
+// fp32 first, in scalar instructions since: the same time, 0.92-0.96 against 0.93 ms inside the step) and the workgroups became persistent
+// (tables built once per CU): 1.22 -> 0.9 ms per 192 chunks. What is left is latency: 2 waves per SIMD (150 KB of LDS per workgroup = one
+// workgroup per CU) walk a chain of four LDS exchanges
 // per frame; neither the VALU (~0.40 ms of issue) nor the LDS pipe (~0.43 ms incl. bank conflicts) is saturated. Inside the step the kernel
 // is NOT hidden by the second stream it runs on: with the features cached the step is 0.9 ms shorter (tools/experiments/feature_cost.py).
 #include "common.h"
